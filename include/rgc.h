@@ -24,6 +24,7 @@
  *   rgc_exec_save_slots/_load_slots checkpoint.py:37-105 safetensors checkpoints, device <-> file
  *   rgc_exec_step_timed         metal.rs:692-700      `step_timed`
  *   rgc_exec_breakdown_json     metal.rs:701-712      `breakdown`
+ *   rgc_token_log_prob, rgc_policy_loss, .. (new) objectives over logits in device memory
  *   rgc_dist_*                  (new) data-parallel communicator for the gradient all-reduce step
  *
  * Plans cross the ABI as one byte string (the "plan blob"): magic "RGPL", u32 version 1, then
@@ -143,6 +144,75 @@ uint64_t rgc_program_launches(const rgc_program* p);
  * may overlap on the GPU race. The first call on a device does set-up (looks up the array's
  * address, loads the kernels): make it before beginning any stream capture. */
 int rgc_sum_noalloc(const void* src, int64_t n, int dtype, void* dst, void* stream);
+
+/* Objectives over logits that are already in device memory (no counterpart in the reference, whose
+ * programs compute them inside a plan; plans reach the same kernels through their token_log_prob,
+ * policy_loss, preference_loss and distillation_loss operations). All pointers are device memory of the
+ * current device, contiguous unless a stride is given, with the logits' dtype where not int32_t.
+ * Work is enqueued on `stream` (a cudaStream_t of that device; NULL = the legacy default stream);
+ * nothing is allocated, nothing synchronises and nothing is kept between calls, so calls may be
+ * captured into CUDA graphs and run at the same time on several streams as long as they write
+ * different outputs (and workspaces). The same inputs give the same bits on every call. Refused
+ * arguments return RGC_ERR_INVALID before any launch.
+ *
+ * Logits: outer x inner rows of `vocab` adjacent elements, row (a, b) at data + a * outer_stride +
+ * b * inner_stride elements. dtype 0 = float32, 1 = float64. Labels and indices are clamped to
+ * [0, vocab). For a row x: m = max x, s = sum exp(x - m), p = exp(x - m) / s, lp = x[label] - m - log s.
+ * A gradient goes to outer x inner rows of its own strides; it may be the logits themselves (same
+ * data and strides), and must not overlap them otherwise. Rows with weight 0 are not read: they count
+ * nothing, whatever they hold, and their gradient is 0. */
+typedef struct {
+  const void* data;
+  int64_t outer, inner, vocab;
+  int64_t outer_stride, inner_stride;
+  int dtype;
+} rgc_logits;
+
+typedef struct {
+  void* data; /* NULL: no gradient is computed */
+  int64_t outer_stride, inner_stride;
+} rgc_gradient;
+
+/* logp[row] = lp; stats[row] = (m, s), which the gradient takes. Either may be NULL. */
+int rgc_token_log_prob(const rgc_logits* logits, const int32_t* labels, void* logp, void* stats, void* stream);
+/* grad[row] = dlogp[row] * (onehot(label) - p); rows with dlogp 0 are not read. */
+int rgc_token_log_prob_grad(const rgc_logits* logits, const int32_t* labels, const void* stats, const void* dlogp, const rgc_gradient* grad,
+                            void* stream);
+
+/* With r = exp(lp - old_logp), A = advantage, d = ref_logp - lp, per row:
+ * terms = weight * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)); loss = their sum.
+ * ref_logp is read only when kl is not 0. loss: one element; terms: one per row; logp (may be NULL): lp. */
+typedef struct {
+  const void *old_logp, *advantage, *weight, *ref_logp;
+  double clip_low, clip_high, kl;
+} rgc_policy;
+int rgc_policy_loss(const rgc_logits* logits, const int32_t* labels, const rgc_policy* policy, void* loss, void* terms, void* logp,
+                    const rgc_gradient* grad, void* stream);
+
+/* outer = 2 n sequences of inner positions, the n chosen ones first. S = sum weight * lp of a sequence,
+ * h = beta ((S - ref_logp) of pair k's chosen sequence - the same of its rejected one), loss = mean over
+ * pairs of -(1 - smoothing) log sigma(h) - smoothing log sigma(-h). ref_logp: one per sequence. margins (n,
+ * may be NULL) = h, logp (2 n, may be NULL) = S. workspace: rgc_preference_workspace bytes that no
+ * other call uses at the same time; its contents need not survive between calls. */
+typedef struct {
+  const void *weight, *ref_logp;
+  double beta, smoothing;
+} rgc_preference;
+size_t rgc_preference_workspace(int64_t sequences, int64_t length, int dtype);
+int rgc_preference_loss(const rgc_logits* logits, const int32_t* labels, const rgc_preference* preference, void* loss, void* margins, void* logp,
+                        const rgc_gradient* grad, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A row's `entries` (1 to 1024) teacher logits at `index`: q = softmax(teacher / T), p = softmax(x / T),
+ * terms = weight T^2 sum q (log q - log p[index]), loss = their sum. Entries of -inf are absent; an index
+ * given twice counts twice; a row without entries counts nothing. */
+typedef struct {
+  const int32_t* index;
+  const void *teacher, *weight;
+  int64_t entries;
+  double temperature;
+} rgc_distillation;
+int rgc_distillation_loss(const rgc_logits* logits, const rgc_distillation* distillation, void* loss, void* terms, const rgc_gradient* grad,
+                          void* stream);
 
 /* Data parallelism: one process per GPU; rank 0 creates the id, every rank joins. */
 int rgc_dist_unique_id(uint8_t id[128]);

@@ -2,6 +2,7 @@
 // checker and the timed CPU baseline. Each kernel cites the arm of src/plan.rs it follows.
 // Built with -ffp-contract=off: rg (Rust) never fuses a multiply and an add, so neither may we.
 #include "interp.h"
+#include "../rustautograd_b200/csrc/host/objective.h"
 #include "../rustautograd_b200/csrc/host/rowchain.h"
 
 #include <algorithm>
@@ -938,6 +939,131 @@ template <typename T> void attn_bwd(const Instr& i, std::vector<Buf>& s) {
   }
 }
 
+// Objectives over rows of logits (the device's own ops, no counterpart in rg): the CPU definition
+// the device's kernels are checked against. Row statistics run in index order in T, per-sequence
+// and per-batch sums in double.
+template <typename T> struct LogitRow {
+  T m = -std::numeric_limits<T>::infinity(), s = (T)0;
+  LogitRow(const T* x, size_t v, T scale) {
+    for (size_t j = 0; j < v; ++j) {
+      const T z = x[j] * scale;
+      m = z > m || std::isnan(z) ? z : m;
+    }
+    for (size_t j = 0; j < v; ++j) s = s + std::exp(x[j] * scale - m);
+  }
+};
+size_t clamp_label(int32_t l, size_t v) { return l < 0 ? 0 : (size_t)l >= v ? v - 1 : (size_t)l; }
+
+template <typename T> void target_grad(T* g, const T* x, size_t v, size_t label, T c, T m, T s) {
+  for (size_t j = 0; j < v; ++j) g[j] = c == (T)0 ? (T)0 : c * ((j == label ? (T)1 : (T)0) - std::exp(x[j] - m) / s);
+}
+
+template <typename T> void objective(const Instr& i, std::vector<Buf>& s) {
+  std::vector<DType> dts;
+  for (size_t a : i.args) dts.push_back(s[a].dtype);
+  Objective o;
+  std::string why;
+  if (!objective_of(i.op, i.arg_shapes, dts, &o, &why)) throw std::runtime_error(std::string(i.op.name()) + ": " + why);
+  const T* X = S<T>(s[i.args[0]]);
+  const int32_t* L = S<int32_t>(s[i.args[1]]);
+  const size_t rows = o.rows, v = o.vocab;
+  auto arg = [&](size_t k) { return S<T>(s[i.args[k]]); };
+  if (i.op.kind == OpKind::LogProbGrad) {
+    for (size_t r = 0; r < rows; ++r) target_grad(S<T>(s[i.dst]) + r * v, X + r * v, v, clamp_label(L[r], v), arg(3)[r], arg(2)[2 * r], arg(2)[2 * r + 1]);
+    return;
+  }
+  // Every result, then copies to the slots that are asked for (no slot of them is an operand's).
+  std::vector<std::vector<T>> out;
+  for (auto& sh : o.outs) out.emplace_back(product(sh), (T)0);
+  auto label_of = [&](size_t r) { return clamp_label(L[r], v); };
+  auto logp_of = [&](size_t r, const LogitRow<T>& st) { return (X[r * v + label_of(r)] - st.m) - std::log(st.s); };
+  switch (i.op.kind) {
+    case OpKind::LogProb:
+      for (size_t r = 0; r < rows; ++r) {
+        const LogitRow<T> st(X + r * v, v, (T)1);
+        out[0][r] = logp_of(r, st);
+        out[1][2 * r] = st.m;
+        out[1][2 * r + 1] = st.s;
+      }
+      break;
+    case OpKind::PolicyLoss: {
+      const T low = (T)(1 - objective_attr(i.op, 0)), high = (T)(1 + objective_attr(i.op, 1)), kl = (T)objective_attr(i.op, 2);
+      double total = 0;
+      for (size_t r = 0; r < rows; ++r) {
+        const T w = arg(4)[r], a = arg(3)[r];
+        if (w == (T)0) continue;
+        const LogitRow<T> st(X + r * v, v, (T)1);
+        const T lp = logp_of(r, st), ratio = std::exp(lp - arg(2)[r]), held = ratio < low ? low : ratio > high ? high : ratio;
+        T term = ratio * a > held * a ? -(held * a) : -(ratio * a);
+        T c = (a >= (T)0 ? ratio <= high : ratio >= low) ? -(ratio * a) : (T)0;
+        if (kl != (T)0) {
+          const T d = arg(5)[r] - lp, e = std::exp(d);
+          term = term + kl * (e - d - (T)1);
+          c = c + kl * ((T)1 - e);
+        }
+        out[1][r] = w * term;
+        out[2][r] = lp;
+        total += (double)out[1][r];
+        target_grad(out[3].data() + r * v, X + r * v, v, label_of(r), w * c, st.m, st.s);
+      }
+      out[0][0] = (T)total;
+      break;
+    }
+    case OpKind::PreferenceLoss: {
+      const double beta = objective_attr(i.op, 0), eps = objective_attr(i.op, 1);
+      const size_t pairs = o.outer / 2, t = o.inner;
+      std::vector<LogitRow<T>> st;
+      std::vector<double> sum(o.outer, 0.0);
+      for (size_t r = 0; r < rows; ++r) {
+        st.emplace_back(X + r * v, v, (T)1);
+        if (arg(2)[r] != (T)0) sum[r / t] += (double)arg(2)[r] * (double)logp_of(r, st.back());
+      }
+      double total = 0;
+      for (size_t k = 0; k < pairs; ++k) {
+        const double h = beta * ((sum[k] - (double)arg(3)[k]) - (sum[pairs + k] - (double)arg(3)[pairs + k]));
+        const double tail = std::log1p(std::exp(-std::fabs(h))), up = 1 / (1 + std::exp(-h)), down = 1 / (1 + std::exp(h));
+        total += std::isnan(h) ? h : (1 - eps) * (tail + std::max(-h, 0.0)) + eps * (tail + std::max(h, 0.0));
+        out[1][k] = (T)h;
+        const T c = (T)(beta * (eps * up - (1 - eps) * down) / (double)pairs);
+        for (size_t side = 0; side < 2; ++side)
+          for (size_t p = 0; p < t; ++p) {
+            const size_t r = (k + side * pairs) * t + p;
+            const T w = arg(2)[r];
+            target_grad(out[3].data() + r * v, X + r * v, v, label_of(r), w == (T)0 ? (T)0 : (side ? -c : c) * w, st[r].m, st[r].s);
+          }
+      }
+      for (size_t b = 0; b < o.outer; ++b) out[2][b] = (T)sum[b];
+      out[0][0] = (T)(total / (double)pairs);
+      break;
+    }
+    default: {
+      const T temp = (T)objective_attr(i.op, 0), inv = (T)(1 / objective_attr(i.op, 0));
+      double total = 0;
+      for (size_t r = 0; r < rows; ++r) {
+        const T w = arg(3)[r];
+        const LogitRow<T> q(arg(2) + r * o.k, o.k, inv);
+        if (w == (T)0 || q.m == -std::numeric_limits<T>::infinity()) continue;
+        const LogitRow<T> st(X + r * v, v, inv);
+        double kl = 0;
+        T* g = out[2].data() + r * v;
+        for (size_t j = 0; j < v; ++j) g[j] = std::exp(X[r * v + j] * inv - st.m) / st.s;
+        for (size_t e = 0; e < o.k; ++e) {
+          const T qe = std::exp(arg(2)[r * o.k + e] * inv - q.m) / q.s;
+          if (qe == (T)0) continue;
+          const size_t l = clamp_label(L[r * o.k + e], v);
+          kl += (double)(qe * (std::log(qe) - ((X[r * v + l] * inv - st.m) - std::log(st.s))));
+          g[l] = g[l] - qe;
+        }
+        for (size_t j = 0; j < v; ++j) g[j] = w * temp * g[j];
+        out[1][r] = w * temp * temp * (T)kl;
+        total += (double)out[1][r];
+      }
+      out[0][0] = (T)total;
+    }
+  }
+  for (auto& [index, slot] : i.outs) std::memcpy(s[slot].data(), out.at(index).data(), out[index].size() * sizeof(T));
+}
+
 void copy_prefix(Buf& d, const Buf& s, size_t n) { std::memcpy(d.data(), s.data(), n * dtype_size(s.dtype)); }
 void copy_range(Buf& d, size_t at, const Buf& s, size_t from, size_t n) {
   size_t es = dtype_size(s.dtype);
@@ -972,6 +1098,7 @@ void step_int(const Instr& i, std::vector<Buf>& s) {
 // plan.rs:692-712
 void exec_instr(const Instr& i, std::vector<Buf>& s) {
   if (i.op.is_control_flow()) return run_control(i, s);
+  if (i.op.is_objective()) return i.dtype == DType::F32 ? objective<float>(i, s) : objective<double>(i, s);
   switch (i.op.kind) {
     case OpKind::Cast: return cast(i, s);
     case OpKind::ArgTopK:

@@ -29,6 +29,8 @@
 #include "gemm_tc.cuh"
 #include "jit.h"
 #include "kernels.cuh"
+#include "objective.h"
+#include "objectives.cuh"
 #include "rgc.h"
 #include "rowkernel.h"
 
@@ -597,6 +599,12 @@ struct Builder {
       case OpKind::AttnFwd:
       case OpKind::AttnBwd:
         return attention(i);
+      case OpKind::LogProb:
+      case OpKind::LogProbGrad:
+      case OpKind::PolicyLoss:
+      case OpKind::PreferenceLoss:
+      case OpKind::DistillLoss:
+        return objective(i);
       case OpKind::Scan:
       case OpKind::While:
       case OpKind::Cond:
@@ -668,6 +676,102 @@ struct Builder {
                       c.f->prog->tc_error, c.s);
       };
     }
+    return l;
+  }
+
+  // The objectives over rows of logits (graph.h, objectives.cuh). Results that no step reads have no
+  // slot: the gradient of a loss that is only evaluated is then not computed.
+  Lowered objective(const Instr& i) {
+    Lowered l;
+    std::vector<DType> dts;
+    for (size_t a : i.args) dts.push_back(p->plan.slots[a].first);
+    rg::Objective o;
+    std::string why;
+    if (!rg::objective_of(i.op, i.arg_shapes, dts, &o, &why)) throw std::runtime_error(std::string(i.op.name()) + ": " + why);
+    auto fits = [&](size_t slot, size_t n, DType d) {
+      if (p->plan.slots[slot].second < n || p->plan.slots[slot].first != d) throw std::runtime_error(std::string(i.op.name()) + ": a slot does not fit");
+    };
+    for (size_t k = 0; k < i.args.size(); ++k) fits(i.args[k], rg::product(i.arg_shapes[k]), dts[k]);
+    const DType dt = dts[0];
+    const EType t = et(dt);
+    RowView x;
+    x.outer = (long long)o.outer;
+    x.inner = (long long)o.inner;
+    x.vocab = x.si = (long long)o.vocab;
+    x.so = (long long)(o.inner * o.vocab);
+    const auto a = i.args;
+    if (i.op.kind == OpKind::LogProbGrad) {
+      const size_t dst = i.dst;
+      fits(dst, o.rows * o.vocab, dt);
+      l.run = [=](Ctx& c) {
+        RowView v = x;
+        v.data = c.f->ptr[a[0]];
+        ck(token_log_prob_grad(t, v, (const int32_t*)c.f->ptr[a[1]], c.f->ptr[a[2]], c.f->ptr[a[3]], RowOut{c.f->ptr[dst], v.so, v.si}, c.s),
+           "token_log_prob_grad");
+      };
+      return l;
+    }
+    // The slot of each result (SIZE_MAX: not needed); a result asked for twice is copied.
+    std::vector<size_t> out(o.outs.size(), SIZE_MAX);
+    std::vector<std::tuple<size_t, size_t, size_t>> copies;  // to, from, bytes
+    for (auto& [index, slot] : i.outs) {
+      if (index >= out.size()) throw std::runtime_error(std::string(i.op.name()) + ": no such result");
+      fits(slot, rg::product(o.outs[index]), dt);
+      if (out[index] == SIZE_MAX) out[index] = slot;
+      else copies.emplace_back(slot, out[index], rg::product(o.outs[index]) * rg::dtype_size(dt));
+    }
+    const bool grad = o.grad_out != SIZE_MAX && out[o.grad_out] != SIZE_MAX;
+    // Per-row terms are summed to the loss: in the frame's scratch when no step reads them.
+    const size_t terms_out = i.op.kind == OpKind::PolicyLoss || i.op.kind == OpKind::DistillLoss ? 1 : SIZE_MAX;
+    if (terms_out != SIZE_MAX && out[terms_out] == SIZE_MAX) scratch = std::max(scratch, o.rows * rg::dtype_size(dt));
+    if (i.op.kind == OpKind::PreferenceLoss) scratch = std::max(scratch, preference_workspace_bytes(t, x.outer, x.inner));
+    l.kernels = i.op.kind == OpKind::LogProb ? 1 : i.op.kind == OpKind::PreferenceLoss ? 3 + grad : 2;
+    const rg::Op op = i.op;
+    const long long teacher = (long long)o.k;
+    const size_t grad_out = o.grad_out;
+    l.run = [=](Ctx& c) {
+      auto at = [&](size_t index) -> void* { return out[index] == SIZE_MAX ? nullptr : c.f->ptr[out[index]]; };
+      RowView v = x;
+      v.data = c.f->ptr[a[0]];
+      const int32_t* labels = (const int32_t*)c.f->ptr[a[1]];
+      RowOut g;
+      if (grad) g = RowOut{at(grad_out), v.so, v.si};
+      switch (op.kind) {
+        case OpKind::LogProb: ck(token_log_prob(t, v, labels, at(0), at(1), c.s), op.name()); break;
+        case OpKind::PolicyLoss: {
+          PolicyArgs pa;
+          pa.old_logp = c.f->ptr[a[2]];
+          pa.advantage = c.f->ptr[a[3]];
+          pa.weight = c.f->ptr[a[4]];
+          pa.ref_logp = a.size() > 5 ? c.f->ptr[a[5]] : nullptr;
+          pa.clip_low = rg::objective_attr(op, 0);
+          pa.clip_high = rg::objective_attr(op, 1);
+          pa.kl = rg::objective_attr(op, 2);
+          ck(policy_loss(t, v, labels, pa, at(0), at(1) ? at(1) : c.f->scratch, at(2), g, c.s), op.name());
+          break;
+        }
+        case OpKind::PreferenceLoss: {
+          PreferenceArgs pa;
+          pa.weight = c.f->ptr[a[2]];
+          pa.ref_logp = c.f->ptr[a[3]];
+          pa.beta = rg::objective_attr(op, 0);
+          pa.smoothing = rg::objective_attr(op, 1);
+          ck(preference_loss(t, v, labels, pa, at(0), at(1), at(2), g, c.f->scratch, c.s), op.name());
+          break;
+        }
+        default: {
+          DistillArgs da;
+          da.index = labels;
+          da.teacher = c.f->ptr[a[2]];
+          da.weight = c.f->ptr[a[3]];
+          da.k = teacher;
+          da.temperature = rg::objective_attr(op, 0);
+          ck(distill_loss(t, v, da, at(0), at(1) ? at(1) : c.f->scratch, g, c.s), op.name());
+        }
+      }
+      for (auto& [to, from, bytes] : copies)
+        if (bytes) ck(cudaMemcpyAsync(c.f->ptr[to], c.f->ptr[from], bytes, cudaMemcpyDeviceToDevice, c.s), op.name());
+    };
     return l;
   }
 
@@ -1972,7 +2076,7 @@ __attribute__((visibility("default"))) int rgc_exec_step_checked(rgc_exec* e, in
     };
     for (size_t k = 0; k < n; ++k) {
       const rg::Step& st = plan.steps[k];
-      if (!st.fused && (st.instr.op.kind == OpKind::Take || st.instr.op.kind == OpKind::TakeAlong)) {
+      if (!st.fused && (st.instr.op.kind == OpKind::Take || st.instr.op.kind == OpKind::TakeAlong || st.instr.op.kind == OpKind::LogProb)) {
         const Instr& i = st.instr;
         const size_t dim = i.op.kind == OpKind::Take ? i.arg_shapes[0][i.op.index] : i.arg_shapes[0].back();
         index_outside((const int32_t*)e->f->ptr[i.args[1]], (long long)rg::product(i.arg_shapes[1]), (long long)dim, dflags + n + k, s);
@@ -1980,7 +2084,7 @@ __attribute__((visibility("default"))) int rgc_exec_step_checked(rgc_exec* e, in
       p->steps[k].run(c);
       if (st.fused) {
         for (auto& o : st.group.outputs) check(o.second, st.group.n, dflags + k);
-      } else if (st.instr.op.is_control_flow()) {
+      } else if (st.instr.op.multi_output()) {
         for (auto& [index, slot] : st.instr.outs) {
           (void)index;
           check(slot, plan.slots[slot].second, dflags + k);

@@ -223,6 +223,54 @@ void module_extra(py::module_& m) {
     if (!cuda()->available()) throw std::runtime_error("no sm_100 CUDA device is available to evaluate on");
     return run_once(*cuda(), p, in);
   });
+  // The objectives over logits in device memory (rustautograd_b200.losses): pointers as integers, the
+  // logits and the gradient as (pointer, outer, inner, vocab, outer stride, inner stride, dtype) and
+  // (pointer, outer stride, inner stride). A refused call raises ValueError.
+  using Ptr = uintptr_t;
+  using LogitsArg = std::tuple<Ptr, int64_t, int64_t, int64_t, int64_t, int64_t, int>;
+  using GradArg = std::tuple<Ptr, int64_t, int64_t>;
+  struct Call {
+    static rgc_logits logits(const LogitsArg& a) {
+      auto& [p, outer, inner, vocab, so, si, dt] = a;
+      return rgc_logits{(const void*)p, outer, inner, vocab, so, si, dt};
+    }
+    static rgc_gradient grad(const GradArg& a) { return rgc_gradient{(void*)std::get<0>(a), std::get<1>(a), std::get<2>(a)}; }
+    static void done(int rc) {
+      if (rc == RGC_ERR_INVALID) throw py::value_error(rgc_last_error());
+      if (rc != RGC_OK) throw std::runtime_error(rgc_last_error());
+    }
+  };
+  m.def("token_log_prob", [](const LogitsArg& x, Ptr labels, Ptr logp, Ptr stats, Ptr stream) {
+    const rgc_logits l = Call::logits(x);
+    Call::done(rgc_token_log_prob(&l, (const int32_t*)labels, (void*)logp, (void*)stats, (void*)stream));
+  });
+  m.def("token_log_prob_grad", [](const LogitsArg& x, Ptr labels, Ptr stats, Ptr dlogp, const GradArg& grad, Ptr stream) {
+    const rgc_logits l = Call::logits(x);
+    const rgc_gradient g = Call::grad(grad);
+    Call::done(rgc_token_log_prob_grad(&l, (const int32_t*)labels, (const void*)stats, (const void*)dlogp, &g, (void*)stream));
+  });
+  m.def("policy_loss", [](const LogitsArg& x, Ptr labels, Ptr old_logp, Ptr advantage, Ptr weight, Ptr ref_logp, double low, double high, double kl,
+                          Ptr loss, Ptr terms, Ptr logp, const GradArg& grad, Ptr stream) {
+    const rgc_logits l = Call::logits(x);
+    const rgc_gradient g = Call::grad(grad);
+    const rgc_policy p{(const void*)old_logp, (const void*)advantage, (const void*)weight, (const void*)ref_logp, low, high, kl};
+    Call::done(rgc_policy_loss(&l, (const int32_t*)labels, &p, (void*)loss, (void*)terms, (void*)logp, &g, (void*)stream));
+  });
+  m.def("preference_workspace", &rgc_preference_workspace);
+  m.def("preference_loss", [](const LogitsArg& x, Ptr labels, Ptr weight, Ptr ref_logp, double beta, double smoothing, Ptr loss, Ptr margins, Ptr logp,
+                              const GradArg& grad, Ptr workspace, size_t bytes, Ptr stream) {
+    const rgc_logits l = Call::logits(x);
+    const rgc_gradient g = Call::grad(grad);
+    const rgc_preference p{(const void*)weight, (const void*)ref_logp, beta, smoothing};
+    Call::done(rgc_preference_loss(&l, (const int32_t*)labels, &p, (void*)loss, (void*)margins, (void*)logp, &g, (void*)workspace, bytes, (void*)stream));
+  });
+  m.def("distillation_loss", [](const LogitsArg& x, Ptr index, Ptr teacher, Ptr weight, int64_t entries, double temperature, Ptr loss, Ptr terms,
+                                const GradArg& grad, Ptr stream) {
+    const rgc_logits l = Call::logits(x);
+    const rgc_gradient g = Call::grad(grad);
+    const rgc_distillation p{(const int32_t*)index, (const void*)teacher, (const void*)weight, entries, temperature};
+    Call::done(rgc_distillation_loss(&l, &p, (void*)loss, (void*)terms, &g, (void*)stream));
+  });
   m.def("cuda_available", [] { return rgc_available() == 1; });
   m.def("dist_unique_id", [] {
     uint8_t id[128];

@@ -2,6 +2,8 @@
 // Rule forms are kept node for node, since they decide the rounding of every gradient.
 #include "autodiff.h"
 
+#include "objective.h"
+
 #include <algorithm>
 #include <map>
 #include <stdexcept>
@@ -250,6 +252,42 @@ Pairs vjp_control(Graph& g, size_t i, const std::map<size_t, uint32_t>& cots, co
     if (rel[target]) out.emplace_back(target, output_of(g, back, n_ct + n_acc + a, g.shape(target), g.dtype(target)));
   }
   return out;
+}
+
+// The gradient of an objective with respect to its logits (the other operands are data: no gradient
+// flows to them). `cots`: the cotangents of its outputs.
+Pairs vjp_objective(Graph& g, size_t i, const std::map<size_t, uint32_t>& cots) {
+  const Node node = g.nodes[i];
+  std::vector<std::vector<size_t>> shapes;
+  std::vector<DType> dts;
+  for (auto x : node.inputs) {
+    shapes.push_back(g.shape(x));
+    dts.push_back(g.dtype(x));
+  }
+  Objective obj;
+  std::string why;
+  objective_of(node.op, shapes, dts, &obj, &why);
+  for (auto& [index, ct] : cots) {
+    (void)ct;
+    if (index == 0) continue;
+    Json obs = Json::object();
+    obs["output"] = index;
+    throw DiagError(diag("GRAD_UNSUPPORTED", "error", g.node_json((uint32_t)i), obs, "only_the_first_result_of_an_objective_is_differentiable", "verified"));
+  }
+  // Its other results are Output nodes made with it.
+  auto output = [&](size_t index) {
+    for (size_t o = i + 1; o < g.nodes.size(); ++o) {
+      const Node& n = g.nodes[o];
+      if (n.op.kind == OpKind::Output && n.inputs[0] == i && n.op.index == index) return (uint32_t)o;
+    }
+    return output_of(g, (uint32_t)i, index, obj.outs[index], node.dtype);
+  };
+  const uint32_t ct = cots.at(0), x = node.inputs[0];
+  if (node.op.kind == OpKind::LogProb) {
+    const uint32_t stats = output(1);
+    return {{x, g.add(Op::make(OpKind::LogProbGrad), {x, node.inputs[1], stats, ct})}};
+  }
+  return {{x, add2(g, OpKind::Mul, ct, output(obj.grad_out))}};
 }
 
 // Transposes the last two axes.
@@ -520,6 +558,11 @@ Pairs vjp(Graph& g, size_t i, uint32_t ct, const std::vector<bool>& rel) {
       out.emplace_back(x, g.add(std::move(o), {ct}));
       break;
     }
+    case OpKind::LogProbGrad: {
+      Json obs = Json::object();
+      obs["alternative"] = "a composition of log_softmax and take_along";
+      throw DiagError(diag("GRAD_UNSUPPORTED", "error", g.node_json((uint32_t)i), obs, "second_derivative_of_token_log_prob", "verified"));
+    }
     case OpKind::MatMulT: throw std::logic_error("optimizer output is never differentiated");
     default: throw std::logic_error("rule table reached control flow");
   }
@@ -557,6 +600,8 @@ std::vector<uint32_t> grad(Graph& g, uint32_t y, const std::vector<uint32_t>& wr
       for (auto& r : n.op.rules) flows = flows || rel[r.first];
     } else if (n.op.is_control_flow()) {
       for (auto x : n.inputs) flows = flows || rel[x];
+    } else if (n.op.multi_output()) {
+      flows = rel[n.inputs[0]];  // an objective: to its logits only
     } else if (!blocks_gradient(n.op)) {
       for (auto x : n.inputs) flows = flows || rel[x];
     }
@@ -573,7 +618,7 @@ std::vector<uint32_t> grad(Graph& g, uint32_t y, const std::vector<uint32_t>& wr
     }
   };
   for (size_t i = end + 1; i-- > 0;) {
-    if (g.nodes[i].op.is_control_flow()) {
+    if (g.nodes[i].op.multi_output()) {
       if (!rel[i]) continue;
       std::map<size_t, uint32_t> cots;
       for (size_t o = i + 1; o <= end; ++o) {
@@ -583,7 +628,7 @@ std::vector<uint32_t> grad(Graph& g, uint32_t y, const std::vector<uint32_t>& wr
       if (cots.empty()) continue;
       g.cur_source = g.nodes[i].source;
       g.cur_origin = (uint32_t)i;
-      accumulate(vjp_control(g, i, cots, rel));
+      accumulate(g.nodes[i].op.is_control_flow() ? vjp_control(g, i, cots, rel) : vjp_objective(g, i, cots));
       continue;
     }
     if (cot[i] < 0) continue;

@@ -183,7 +183,7 @@ struct Reader {
   Op op() {
     Op o;
     uint8_t k = u8();
-    if (k > (uint8_t)OpKind::AttnBwd) throw std::runtime_error("plan blob has an unknown op");
+    if (k > (uint8_t)OpKind::DistillLoss) throw std::runtime_error("plan blob has an unknown op");
     o.kind = (OpKind)k;
     o.index = u64();
     o.shape = vec();
@@ -340,7 +340,7 @@ Plan decode_plan(const uint8_t* data, size_t len) {
         }
       } else {
         for (size_t a : st.instr.args) ok(a);
-        if (!st.instr.op.is_control_flow()) {
+        if (!st.instr.op.multi_output()) {
           ok(st.instr.dst);
           if (pl.slots[st.instr.dst].second < st.instr.n) throw std::runtime_error("destination slot too small");
         }

@@ -5,6 +5,7 @@
 #include <cstdio>
 #include <set>
 
+#include "objective.h"
 #include "optimize.h"
 #include "plan.h"
 
@@ -66,6 +67,11 @@ const char* Op::name() const {
     case OpKind::AllReduce: return "all_reduce";
     case OpKind::AttnFwd: return "attention";
     case OpKind::AttnBwd: return "attention_grad";
+    case OpKind::LogProb: return "token_log_prob";
+    case OpKind::LogProbGrad: return "token_log_prob_grad";
+    case OpKind::PolicyLoss: return "policy_loss";
+    case OpKind::PreferenceLoss: return "preference_loss";
+    case OpKind::DistillLoss: return "distillation_loss";
   }
   return "?";
 }
@@ -104,7 +110,7 @@ bool Op::is_nonsmooth() const {
   switch (kind) {
     case OpKind::Abs: case OpKind::Sign: case OpKind::Floor: case OpKind::Max: case OpKind::Min:
     case OpKind::Gt: case OpKind::Ge: case OpKind::Where: case OpKind::Custom: case OpKind::ArgTopK:
-    case OpKind::Cond:
+    case OpKind::Cond: case OpKind::PolicyLoss:
       return true;
     case OpKind::Reduce: return reduce != ReduceKind::Sum;
     default: return false;
@@ -285,7 +291,7 @@ uint32_t Graph::add(Op op, const std::vector<uint32_t>& inputs) {
     case OpKind::AttnFwd: arity = op.value && op.value->n() == 3 ? 2 : 4; break;
     case OpKind::AttnBwd: arity = op.value && op.value->n() == 3 ? 4 : 6; break;
     default:
-      if (op.is_control_flow()) arity = inputs.size();
+      if (op.is_control_flow() || op.is_objective()) arity = inputs.size();
       else if (op.is_binary_elementwise()) arity = 2;
       else arity = 1;
   }
@@ -306,6 +312,23 @@ uint32_t Graph::add(Op op, const std::vector<uint32_t>& inputs) {
   }
   std::vector<DType> dts;
   for (uint32_t i : inputs) dts.push_back(dtype(i));
+  if (op.is_objective()) {
+    std::vector<std::vector<size_t>> shapes;
+    for (uint32_t i : inputs) shapes.push_back(nodes[i].shape);
+    Objective obj;
+    std::string why;
+    if (!objective_of(op, shapes, dts, &obj, &why)) {
+      Json names = Json::array();
+      for (auto d : dts) names.push(dtype_name(d));
+      Json o = Json::object();
+      o["input_shapes"] = shapes_json(shapes);
+      o["input_dtypes"] = names;
+      static_err("OBJECTIVE_OPERANDS", op, o, why);
+    }
+    // Several results: the node itself holds none (its dtype is the logits').
+    auto shape = op.multi_output() ? std::vector<size_t>{} : shapes[0];
+    return push(std::move(op), inputs, std::move(shape), dts[0]);
+  }
   bool indexes = op.kind == OpKind::Take || op.kind == OpKind::TakeAlong || op.kind == OpKind::TakeGrad || op.kind == OpKind::TakeAlongGrad;
   if (indexes && dts[1] != DType::I32) {
     Json o = Json::object();
@@ -685,6 +708,28 @@ void Graph::check_control_flow(const Op& op, const std::vector<uint32_t>& inputs
     }
     default: throw std::logic_error("only control flow is checked here");
   }
+}
+
+std::vector<uint32_t> Graph::objective(Op op, const std::vector<uint32_t>& inputs) {
+  const uint32_t node = add(op, inputs);
+  std::vector<std::vector<size_t>> shapes;
+  std::vector<DType> dts;
+  for (uint32_t i : inputs) {
+    shapes.push_back(nodes[i].shape);
+    dts.push_back(nodes[i].dtype);
+  }
+  Objective obj;
+  std::string why;
+  objective_of(op, shapes, dts, &obj, &why);
+  std::vector<uint32_t> outs;
+  for (size_t k = 0; k < obj.outs.size(); ++k) {
+    Op o = Op::make(OpKind::Output);
+    o.index = k;
+    o.shape = obj.outs[k];
+    o.dtype = dts[0];
+    outs.push_back(add(std::move(o), {node}));
+  }
+  return outs;
 }
 
 std::vector<bool> Graph::reachable(const std::vector<uint32_t>& outputs) const {

@@ -47,6 +47,25 @@ enum class OpKind : uint8_t {
   // AttnBwd gives the gradient of qkv, (B, T, 3, H, d). No head-split copies are needed.
   AttnFwd,
   AttnBwd,
+  // Objectives over rows of logits (no counterpart in rg; objective.h has their shapes, with lp, m, s, p
+  // the label's log-probability, the row's maximum, exp-sum and softmax, labels clamped to the
+  // row). All but LogProbGrad have several results, each an Output of the node.
+  // LogProb(logits, labels): 0 lp, 1 the statistics (m, s) packed along a last axis of 2.
+  // LogProbGrad(logits, labels, stats, ct): ct (onehot(label) - p).
+  // PolicyLoss(logits, labels, old, advantage, weight[, ref]) with value = [low, high, kl]: with
+  // r = exp(lp - old) and d = ref - lp, terms w (-min(r A, clip(r, 1 - low, 1 + high) A) + kl (exp(d) - d - 1));
+  // 0 their sum, 1 the terms, 2 lp, 3 the gradient of 0 with respect to the logits.
+  // PreferenceLoss(logits, labels, weight, ref) with value = [beta, smoothing], chosen sequences
+  // before the rejected ones: S = sum w lp per sequence, h = beta ((S - ref) - (S' - ref')) per pair;
+  // 0 the mean of -(1 - smoothing) log sigma(h) - smoothing log sigma(-h), 1 h, 2 S, 3 the gradient of 0.
+  // DistillLoss(logits, index, teacher, weight) with value = [T]: q = softmax(teacher / T) at the k given
+  // indices, p = softmax(logits / T), terms w T^2 sum q (log q - log p); 0 their sum, 1 the
+  // terms, 2 the gradient of 0. Rows with w = 0 count nothing, whatever they hold.
+  LogProb,
+  LogProbGrad,
+  PolicyLoss,
+  PreferenceLoss,
+  DistillLoss,
 };
 
 struct Op {
@@ -60,7 +79,7 @@ struct Op {
   bool flag_a = false;          // MatMulT ta, Reduce keepdims, Cumsum/Scan reverse
   bool flag_b = false;          // MatMulT tb
   ReduceKind reduce = ReduceKind::Sum;
-  TensorP value;                // Const
+  TensorP value;                // Const; attributes of the device's own operations
   BodyP body, body2;            // Scan body / While cond+body / Cond then+else
   size_t n_carry = 0, n_x = 0, length = 0, max_iterations = 0;
   uint32_t placeholder = 0;     // Custom
@@ -75,6 +94,12 @@ struct Op {
   bool is_unary_elementwise() const;
   bool is_binary_elementwise() const;
   bool is_control_flow() const { return kind == OpKind::Scan || kind == OpKind::While || kind == OpKind::Cond; }
+  bool is_objective() const {
+    return kind == OpKind::LogProb || kind == OpKind::LogProbGrad || kind == OpKind::PolicyLoss || kind == OpKind::PreferenceLoss ||
+           kind == OpKind::DistillLoss;
+  }
+  // Results are Output nodes, allocated with the node's step.
+  bool multi_output() const { return is_control_flow() || (is_objective() && kind != OpKind::LogProbGrad); }
   bool int_ok() const;
   bool is_nonsmooth() const;
   // Key for common-subexpression elimination: equal keys mean interchangeable nodes
@@ -124,6 +149,8 @@ struct Graph {
   uint32_t constant(Tensor t);
   uint32_t constant(TensorP t);
   uint32_t scalar(DType d, double x) { return constant(Tensor::full(d, {}, x)); }
+  // An objective with several results: the ids of its Output nodes, in order.
+  std::vector<uint32_t> objective(Op op, const std::vector<uint32_t>& inputs);
   const std::vector<size_t>& shape(uint32_t id) const { return nodes[id].shape; }
   DType dtype(uint32_t id) const { return nodes[id].dtype; }
   // Appends a node after checking arity, dtypes and shapes (graph.rs:316-383).

@@ -578,7 +578,7 @@ Plan Plan::build_with(const Graph& g, const std::vector<uint32_t>& outputs, bool
     }
     size_t i = item.node;
     const Node& node = g.nodes[i];
-    if (node.op.kind == OpKind::Output) continue;  // allocated with its control-flow step
+    if (node.op.kind == OpKind::Output) continue;  // allocated with the step of its node
     if (is_alias(g, i)) {
       size_t x = node.inputs[0];
       size_t s = value_slot[x];
@@ -607,7 +607,7 @@ Plan Plan::build_with(const Graph& g, const std::vector<uint32_t>& outputs, bool
     for (auto x : dying)
       if (inplace(x)) a.release(value_slot[x]);
     size_t dst;
-    if (node.op.is_control_flow()) {
+    if (node.op.multi_output()) {
       for (size_t o = 0; o < total; ++o) {
         const Node& out = g.nodes[o];
         if (keep[o] && out.op.kind == OpKind::Output && !out.inputs.empty() && out.inputs[0] == i) {

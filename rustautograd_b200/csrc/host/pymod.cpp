@@ -88,6 +88,27 @@ template <typename T> T attr(const py::dict* a, const char* key) {
   }
 }
 
+// The attributes of an objective (graph.h), in their order.
+Op parse_objective(const std::string& name, const py::dict* a) {
+  static const std::pair<const char*, std::pair<OpKind, std::vector<const char*>>> kinds[] = {
+      {"token_log_prob", {OpKind::LogProb, {}}},
+      {"policy_loss", {OpKind::PolicyLoss, {"clip_low", "clip_high", "kl"}}},
+      {"preference_loss", {OpKind::PreferenceLoss, {"beta", "smoothing"}}},
+      {"distillation_loss", {OpKind::DistillLoss, {"temperature"}}},
+  };
+  for (auto& [n, k] : kinds) {
+    if (name != n) continue;
+    Op o = Op::make(k.first);
+    if (!k.second.empty()) {
+      Buf b(DType::F64, k.second.size());
+      for (size_t i = 0; i < k.second.size(); ++i) b.f64()[i] = attr<double>(a, k.second[i]);
+      o.value = std::make_shared<const Tensor>(std::vector<size_t>{k.second.size()}, std::move(b));
+    }
+    return o;
+  }
+  throw py::value_error("unknown objective " + name);
+}
+
 // python.rs:88-133
 Op parse_op(const std::string& name, const py::dict* a) {
   auto reduce = [&](ReduceKind k) {
@@ -206,6 +227,12 @@ PYBIND11_MODULE(RG_MODULE_NAME, m) {
             Op op = parse_op(name, attrs ? &*attrs : nullptr);
             self.g.cur_source = src(source);
             return guarded([&] { return self.g.add(std::move(op), inputs); });
+          }, py::arg("name"), py::arg("inputs"), py::arg("attrs") = py::none(), py::arg("source") = py::none())
+      // Not in rg's module: an objective over rows of logits; the ids of its results.
+      .def("objective", [](PyGraph& self, const std::string& name, std::vector<uint32_t> inputs, std::optional<py::dict> attrs, std::optional<std::string> source) {
+            Op op = parse_objective(name, attrs ? &*attrs : nullptr);
+            self.g.cur_source = src(source);
+            return guarded([&] { return self.g.objective(std::move(op), inputs); });
           }, py::arg("name"), py::arg("inputs"), py::arg("attrs") = py::none(), py::arg("source") = py::none())
       .def("grad", [](PyGraph& self, uint32_t y, std::vector<uint32_t> wrts, std::optional<std::string> source) {
             self.check_id(y);

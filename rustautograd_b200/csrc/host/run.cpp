@@ -121,6 +121,16 @@ std::vector<StepCost> step_costs(const Plan& p) {
       c.kind = "attention";
       c.flops = 2.0 * batch * t * t * (i.op.kind == OpKind::AttnFwd ? d + dv : 3.0 * d + 2.0 * dv);
       c.bytes = in_bytes + (double)i.n * es;
+    } else if (i.op.is_objective()) {
+      // The logits once (a preference's gradient reads them again), the gradient, and the small
+      // operands; an exponential, a maximum and a sum per element, a product more for a gradient.
+      c.kind = "objective";
+      const double logits = (double)product(i.arg_shapes[0]);
+      bool grad = i.op.kind == OpKind::LogProbGrad;
+      for (auto& o : i.outs) grad = grad || p.slots[o.second].second >= product(i.arg_shapes[0]);
+      const bool twice = grad && i.op.kind == OpKind::PreferenceLoss;
+      c.bytes = in_bytes + (grad ? logits * es : 0.0) + (twice ? logits * es : 0.0);
+      c.flops = logits * (grad ? 6.0 : 3.0);
     } else if (i.op.kind == OpKind::Reduce) {
       c.flops = in_bytes / es;
       c.bytes = in_bytes + (double)i.n * es;

@@ -253,7 +253,7 @@ Compiled::Observed Compiled::observed(const std::vector<Tensor>& inputs) const {
     // Index check (validate.rs:177-190).
     size_t dim = 0;
     if (i.op.kind == OpKind::Take) dim = i.arg_shapes[0][i.op.index];
-    else if (i.op.kind == OpKind::TakeAlong) dim = i.arg_shapes[0].back();
+    else if (i.op.kind == OpKind::TakeAlong || i.op.kind == OpKind::LogProb) dim = i.arg_shapes[0].back();
     if (dim) {
       size_t n = product(i.arg_shapes[1]);
       Stats s = stats(e->prefix(i.args[1], n), n);
@@ -266,9 +266,9 @@ Compiled::Observed Compiled::observed(const std::vector<Tensor>& inputs) const {
         o.hard.push_back(diag("INDEX_OUT_OF_RANGE", "error", raw.node_json(i.node), obs, "index_outside_axis", "verified"));
       }
     }
-    if (i.op.is_control_flow()) {
+    if (i.op.multi_output()) {
       // Bodies run as one step here; a non-finite value they produce is reported at the
-      // control-flow node itself.
+      // control-flow node itself. An objective's results are reported at its node too.
       for (auto& [index, slot] : i.outs) {
         (void)index;
         size_t n = product(raw_plan.slots[slot].second == 0 ? std::vector<size_t>{0} : std::vector<size_t>{raw_plan.slots[slot].second});

@@ -22,7 +22,7 @@ import math
 from . import nn, random
 from .optim import AdamW
 from .program import compile, run, value_and_grad
-from .tracing import all_reduce, arange, concatenate, full, ones, take, tensor, tril, where, zeros
+from .tracing import abs, all_reduce, arange, concatenate, full, ones, take, tensor, tril, where, zeros
 from .trees import tree_map
 
 STD = 0.02
@@ -135,6 +135,63 @@ def make_train_step(model, opt, batch, world=1, rank=0):
         params, opt_state = opt.update(grads, state["opt"], state["params"])
         return {"params": params, "opt": opt_state, "key": keys[0]}, loss
     return step
+
+
+# Training steps after pretraining (no counterpart in rg), of the same contract as make_train_step:
+# `(state, batch) -> (state, aux)` with state {"params", "opt"}. Token rows hold T + 1 tokens; position t
+# predicts token t + 1, so the other per-position arrays have T columns.
+
+def _updated(opt, state, grads):
+    params, opt_state = opt.update(grads, state["opt"], state["params"])
+    return {"params": params, "opt": opt_state}
+
+
+def make_policy_step(model, opt, clip_low=0.2, clip_high=0.2, kl=0.0):
+    """A clipped policy update. batch: {"tokens" (N, T + 1) int32, "old_logp", "advantages", "weights" (N, T)} and,
+    with kl != 0, "ref_logp" (N, T). aux: the loss and the mean of logp - old_logp under the weights."""
+    def loss_of(params, batch):
+        tokens = batch["tokens"]
+        loss, _, logp = nn.policy_loss(model(params, tokens[:, :-1]), tokens[:, 1:], batch["old_logp"], batch["advantages"], batch["weights"],
+                                       batch["ref_logp"] if kl else None, clip_low, clip_high, kl)
+        drift = where(abs(batch["weights"]) > 0.0, batch["weights"] * (logp - batch["old_logp"]), 0.0).sum()
+        return loss, drift
+
+    def step(state, batch):
+        (loss, drift), grads = value_and_grad(loss_of, has_aux=True)(state["params"], batch)
+        return _updated(opt, state, grads), {"loss": loss, "drift": drift}
+    return step
+
+
+def make_preference_step(model, opt, beta=0.1, smoothing=0.0):
+    """A preference update over pairs. batch: {"tokens" (2 n, T + 1) int32 with the chosen rows first,
+    "weights" (2 n, T), "ref_logp" (2 n)}. aux: the loss and the share of pairs with a positive margin."""
+    def loss_of(params, batch):
+        tokens = batch["tokens"]
+        loss, margins, _ = nn.preference_loss(model(params, tokens[:, :-1]), tokens[:, 1:], batch["weights"], batch["ref_logp"], beta, smoothing)
+        return loss, (margins > 0.0).mean()
+
+    def step(state, batch):
+        (loss, right), grads = value_and_grad(loss_of, has_aux=True)(state["params"], batch)
+        return _updated(opt, state, grads), {"loss": loss, "accuracy": right}
+    return step
+
+
+def make_distillation_step(model, opt, temperature=1.0):
+    """A distillation update. batch: {"tokens" (N, T) int32, "index" (N, T, k) int32, "teacher" (N, T, k),
+    "weights" (N, T)}. aux: the loss."""
+    def loss_of(params, batch):
+        return nn.distillation_loss(model(params, batch["tokens"]), batch["index"], batch["teacher"], batch["weights"], temperature)[0]
+
+    def step(state, batch):
+        loss, grads = value_and_grad(loss_of)(state["params"], batch)
+        return _updated(opt, state, grads), loss
+    return step
+
+
+def compile_scorer(model, params, tokens, device=None):
+    """A compiled `(params, tokens (N, T + 1)) -> (N, T)`: the log-probability of each next token, as the
+    old and reference values of the steps above."""
+    return compile(lambda p, t: nn.token_log_prob(model(p, t[:, :-1]), t[:, 1:]), (params, tokens), validate="basic", device=device)
 
 
 def compile_sampler(model, params, temperature=1.0, top_k=None, top_p=None, device=None):

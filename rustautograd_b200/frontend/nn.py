@@ -4,10 +4,19 @@ filters. Each is written as the same sequence of primitive ops as rg's python/rg
 (softmax nn.py:40-42, log-softmax and logsumexp nn.py:29-37, cross-entropy nn.py:78-84, GELU
 nn.py:25-27, filters nn.py:60-72), so the device receives the plan rg would build; the row
 statistics go through `stop_gradient`, as in rg, so autodiff emits rg's backward chains.
+
+Below them, the objectives that rg has no counterpart for: the log-probability of given tokens, the
+clipped policy loss with a KL term, the preference loss over pairs of sequences and the distillation
+from a teacher's top logits. Each is one operation of the engine. They take logits (..., V), int32 labels
+of the leading shape (clamped to [0, V), as indices are everywhere) and operands of the leading shape in
+the logits' dtype. Gradients flow to the logits only; the other operands are data. Only the first result
+of a loss is differentiable, the others are for reporting (differentiating them is an error). Positions
+with weight 0 count nothing, whatever they hold. A loss computes its gradient in the same pass over the
+logits, so it is an output of the forward step; a loss that is only evaluated does not compute it.
 """
 import math
 
-from .tracing import argsort, cumsum, exp, stop_gradient, take_along_axis, tanh, top_k, where
+from .tracing import argsort, cumsum, exp, objective, stop_gradient, take_along_axis, tanh, top_k, where
 
 _GELU_C = math.sqrt(2.0 / math.pi)
 
@@ -53,3 +62,35 @@ def top_p_logits(logits, p):
     probs = softmax(take_along_axis(logits, order))
     kept = (cumsum(probs) - probs) < p
     return where(take_along_axis(kept, argsort(order.cast(logits.dtype))), logits, -1e9)
+
+
+def token_log_prob(logits, labels):
+    """log_softmax(logits) at `labels`, without the full log_softmax: -token_log_prob(logits, labels).mean()
+    is the cross-entropy. The gradient may weight each position differently."""
+    return objective("token_log_prob", logits, labels)[0]
+
+
+def policy_loss(logits, labels, old_logp, advantages, weights, ref_logp=None, clip_low=0.2, clip_high=0.2, kl=0.0):
+    """`(loss, terms, logp)` of the clipped policy loss: with r = exp(logp - old_logp) and d = ref_logp - logp,
+    terms = weights * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)) and loss their
+    sum. The weights carry the mask and the averaging; `ref_logp` goes with a kl != 0."""
+    if (kl != 0) != (ref_logp is not None):
+        raise ValueError("ref_logp goes with a kl coefficient that is not 0")
+    data = (labels, old_logp, advantages, weights) + (() if ref_logp is None else (ref_logp,))
+    return objective("policy_loss", logits, *data, clip_low=float(clip_low), clip_high=float(clip_high), kl=float(kl))[:3]
+
+
+def preference_loss(logits, labels, weights, ref_logp, beta=0.1, smoothing=0.0):
+    """`(loss, margins, logp)` of the paired preference loss over 2 n sequences, logits (2 n, T, V), chosen
+    ones first: logp = S = (weights * token log-probability).sum over T (2 n), margins = h =
+    beta ((S - ref_logp) of the chosen - of the rejected one) (n), loss the mean over pairs of
+    -(1 - smoothing) log sigma(h) - smoothing log sigma(-h). `ref_logp` (2 n) is the reference's S."""
+    return objective("preference_loss", logits, labels, weights, ref_logp, beta=float(beta), smoothing=float(smoothing))[:3]
+
+
+def distillation_loss(logits, index, teacher, weights, temperature=1.0):
+    """`(loss, terms)` of the distillation from a teacher's k top logits, `teacher` (..., k) at vocabulary
+    positions `index` (..., k): with q = softmax(teacher / T) and p = softmax(logits / T), terms =
+    weights * T^2 * sum q (log q - log p) and loss their sum. Teacher entries of -inf are absent, an index
+    given twice counts twice, k is at most 1024."""
+    return objective("distillation_loss", logits, index, teacher, weights, temperature=float(temperature))[:2]

@@ -143,6 +143,19 @@ def op(name, *operands, **attrs):
     return Tensor(scratch.graph.eval([node])[0])
 
 
+def objective(name, *operands, **attrs):
+    """The results of objective `name` (the engine's operations over rows of logits), as a tuple of
+    arrays: recorded as one node and its outputs, or evaluated at once."""
+    dtype = dtype_of(operands)
+    frame = recording()
+    if frame is not None:
+        ids = [frame.node(o, dtype) for o in operands]
+        return tuple(Traced(frame, i) for i in frame.graph.objective(name, ids, attrs or None, caller()))
+    scratch = Frame(native().Graph())
+    ids = [scratch.node(o, dtype) for o in operands]
+    return tuple(Tensor(t) for t in scratch.graph.eval(scratch.graph.objective(name, ids, attrs or None, caller())))
+
+
 # ---------------------------------------------------------------------------------------------
 # Arrays
 # ---------------------------------------------------------------------------------------------

@@ -1,0 +1,221 @@
+"""Objectives over logits that are already on the GPU, as torch tensors: the calls of include/rgc.h
+(rgc_token_log_prob .. rgc_distillation_loss) with outputs allocated by torch, on torch's current stream of
+the logits' device. Compiled programs have the same objectives in `frontend.nn`.
+
+Every function takes logits of shape (..., V), float32 or float64, whose last axis is contiguous and whose
+leading axes fold into at most two strides (a model's output, or a slice of its positions such as
+`logits[:, :-1]`). Labels and indices are int32 of the leading shape and are clamped to [0, V); all other
+operands have the logits' dtype and the leading shape. Positions with weight 0 are not read: they count
+nothing, whatever they hold (padding may be NaN, with labels of -100), and their gradient is 0.
+
+`grad=False` computes the loss alone. `out` receives the gradient: a tensor of the logits' shape and dtype,
+which may be the logits themselves (they are then overwritten). A refused argument raises ValueError or
+TypeError before anything is launched. Nothing synchronises, so the calls can be captured into CUDA graphs.
+"""
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import load_native
+
+_DTYPES = {torch.float32: 0, torch.float64: 1}
+_rg = None
+
+
+def _native():
+    global _rg
+    if _rg is None:
+        _rg = load_native()
+    return _rg
+
+
+def _two_strides(x, what):
+    """(outer, inner, outer stride, inner stride) of the leading axes of `x`."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) < 1:
+        raise ValueError(f"{what} needs a last axis")
+    if stride[-1] != 1 and shape[-1] != 1:
+        raise ValueError(f"the last axis of {what} must be contiguous")
+    groups = []  # [extent, stride], slowest first; axes that chain share a group
+    for n, s in zip(shape[:-1], stride[:-1]):
+        if n == 1:
+            continue
+        if groups and groups[-1][1] == n * s:
+            groups[-1] = [groups[-1][0] * n, s]
+        else:
+            groups.append([n, s])
+    if len(groups) > 2:
+        raise ValueError(f"the leading axes of {what} have more than two independent strides; make it contiguous")
+    while len(groups) < 2:
+        groups.append([1, 0])
+    (outer, so), (inner, si) = groups
+    return outer, inner, so, si
+
+
+class _Call:
+    """The logits of a call and the stream it runs on."""
+
+    def __init__(self, logits, sequences=False):
+        if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+            raise TypeError("logits must be a CUDA tensor")
+        self.dtype = _DTYPES.get(logits.dtype)
+        if self.dtype is None:
+            raise TypeError(f"logits must be float32 or float64, not {logits.dtype}")
+        self.logits, self.device = logits, logits.device
+        self.lead = logits.shape[:-1]
+        if sequences:
+            if logits.dim() != 3:
+                raise ValueError("logits must be (sequences, positions, vocabulary)")
+            outer, inner, vocab = logits.shape
+            so, si, last = logits.stride()
+            if last != 1 and vocab != 1:
+                raise ValueError("the last axis of logits must be contiguous")
+        else:
+            outer, inner, so, si = _two_strides(logits, "logits")
+            vocab = logits.shape[-1]
+        self.rows = (outer, inner)
+        self.args = (logits.data_ptr(), outer, inner, vocab, so, si, self.dtype)
+
+    def per_row(self, t, what, shape=None, dtype=None):
+        """A contiguous operand on the logits' device."""
+        if not isinstance(t, torch.Tensor) or t.device != self.device:
+            raise TypeError(f"{what} must be a tensor on {self.device}")
+        want = self.logits.dtype if dtype is None else dtype
+        if t.dtype != want:
+            raise TypeError(f"{what} must be {want}, not {t.dtype}")
+        if t.shape != (self.lead if shape is None else shape):
+            raise ValueError(f"{what} has shape {tuple(t.shape)}, not {tuple(self.lead if shape is None else shape)}")
+        return t if t.is_contiguous() else t.contiguous()
+
+    def new(self, *shape):
+        return torch.empty(shape, dtype=self.logits.dtype, device=self.device)
+
+    def gradient(self, grad, out, sequences=False):
+        """(tensor, call argument) of the gradient."""
+        if not grad:
+            if out is not None:
+                raise ValueError("out is given but no gradient is asked for")
+            return None, (0, 0, 0)
+        if out is None:
+            out = self.new(*self.logits.shape)
+        elif not isinstance(out, torch.Tensor) or out.device != self.device or out.dtype != self.logits.dtype or out.shape != self.logits.shape:
+            raise ValueError("out must have the logits' shape, dtype and device")
+        if sequences:
+            if out.stride(2) != 1 and out.shape[2] != 1:
+                raise ValueError("the last axis of out must be contiguous")
+            return out, (out.data_ptr(), out.stride(0), out.stride(1))
+        if out.is_contiguous():
+            outer, inner = self.rows
+            v = self.logits.shape[-1]
+            return out, (out.data_ptr(), inner * v, v)
+        outer, inner, so, si = _two_strides(out, "out")
+        if (outer, inner) != self.rows:
+            raise ValueError("out's strides do not split its rows as the logits' strides do; make it contiguous")
+        return out, (out.data_ptr(), so, si)
+
+    def run(self, call, *args):
+        if self.device.index == torch.cuda.current_device():
+            call(*args, torch.cuda.current_stream(self.device).cuda_stream)
+        else:
+            with torch.cuda.device(self.device):
+                call(*args, torch.cuda.current_stream(self.device).cuda_stream)
+
+
+def token_log_prob(logits, labels, *, stats=False):
+    """log softmax(logits) at `labels`; with `stats=True` also the row statistics (..., 2) = (maximum, sum of
+    exp(logits - maximum)) that `token_log_prob_grad` takes."""
+    c = _Call(logits)
+    labels = c.per_row(labels, "labels", dtype=torch.int32)
+    logp = c.new(*c.lead)
+    st = c.new(*c.lead, 2) if stats else None
+    c.run(_native().token_log_prob, c.args, labels.data_ptr(), logp.data_ptr(), st.data_ptr() if stats else 0)
+    return (logp, st) if stats else logp
+
+
+def token_log_prob_grad(logits, labels, stats, dlogp, *, out=None):
+    """The gradient with respect to `logits` of token_log_prob for the cotangent `dlogp`."""
+    c = _Call(logits)
+    labels = c.per_row(labels, "labels", dtype=torch.int32)
+    stats = c.per_row(stats, "stats", shape=(*c.lead, 2))
+    dlogp = c.per_row(dlogp, "dlogp")
+    grad, g = c.gradient(True, out)
+    c.run(_native().token_log_prob_grad, c.args, labels.data_ptr(), stats.data_ptr(), dlogp.data_ptr(), g)
+    return grad
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor            # scalar: the sum of the terms
+    terms: torch.Tensor           # per position, weighted
+    logp: torch.Tensor            # log-probabilities of the labels (0 where the weight is 0)
+    grad: Optional[torch.Tensor]  # of the loss with respect to the logits
+
+
+def policy_loss(logits, labels, old_logp, advantages, weights, *, ref_logp=None, clip_low=0.2, clip_high=0.2, kl=0.0, grad=True, out=None):
+    """The clipped policy loss: with r = exp(logp - old_logp) and d = ref_logp - logp, the sum over positions
+    of weights * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)). The weights carry the
+    mask and the averaging (mask / mask.sum() for a mean over tokens). `ref_logp` goes with a kl != 0."""
+    if (kl != 0) != (ref_logp is not None):
+        raise ValueError("ref_logp goes with a kl coefficient that is not 0")
+    c = _Call(logits)
+    labels = c.per_row(labels, "labels", dtype=torch.int32)
+    old = c.per_row(old_logp, "old_logp")
+    adv = c.per_row(advantages, "advantages")
+    w = c.per_row(weights, "weights")
+    ref = c.per_row(ref_logp, "ref_logp") if ref_logp is not None else None
+    g, ga = c.gradient(grad, out)
+    loss, terms, logp = c.new(), c.new(*c.lead), c.new(*c.lead)
+    c.run(_native().policy_loss, c.args, labels.data_ptr(), old.data_ptr(), adv.data_ptr(), w.data_ptr(), 0 if ref is None else ref.data_ptr(),
+          clip_low, clip_high, kl, loss.data_ptr(), terms.data_ptr(), logp.data_ptr(), ga)
+    return PolicyLoss(loss, terms, logp, g)
+
+
+class PreferenceLoss(NamedTuple):
+    loss: torch.Tensor            # scalar: the mean over pairs
+    margins: torch.Tensor         # (n,) beta times the difference of the log ratios
+    logp: torch.Tensor            # (2 n,) weighted log-probability of each sequence
+    grad: Optional[torch.Tensor]  # of the loss with respect to the logits
+
+
+def preference_loss(logits, labels, weights, ref_logp, *, beta=0.1, smoothing=0.0, grad=True, out=None):
+    """The paired preference loss over 2 n sequences, logits (2 n, T, V), the n chosen ones before the n rejected
+    ones: S = sum over positions of weights * logp, h = beta ((S - ref_logp)[chosen] - (S - ref_logp)[rejected]),
+    and the mean over pairs of -(1 - smoothing) log sigma(h) - smoothing log sigma(-h). `ref_logp` (2 n,) holds the
+    reference's S; weights are the mask of the answers' tokens (divided by their number for a mean per token)."""
+    c = _Call(logits, sequences=True)
+    n, t = c.rows
+    if n < 2 or n % 2:
+        raise ValueError("logits must hold pairs of sequences: an even number of at least 2")
+    labels = c.per_row(labels, "labels", dtype=torch.int32)
+    w = c.per_row(weights, "weights")
+    ref = c.per_row(ref_logp, "ref_logp", shape=(n,))
+    g, ga = c.gradient(grad, out, sequences=True)
+    nbytes = _native().preference_workspace(n, t, c.dtype)
+    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=c.device)
+    loss, margins, logp = c.new(), c.new(n // 2), c.new(n)
+    c.run(_native().preference_loss, c.args, labels.data_ptr(), w.data_ptr(), ref.data_ptr(), beta, smoothing, loss.data_ptr(), margins.data_ptr(),
+          logp.data_ptr(), ga, workspace.data_ptr(), nbytes)
+    return PreferenceLoss(loss, margins, logp, g)
+
+
+class DistillationLoss(NamedTuple):
+    loss: torch.Tensor            # scalar: the sum of the terms
+    terms: torch.Tensor           # per position, weighted
+    grad: Optional[torch.Tensor]  # of the loss with respect to the logits
+
+
+def distillation_loss(logits, index, teacher, weights, *, temperature=1.0, grad=True, out=None):
+    """Distillation from a teacher's top logits: `teacher` (..., k) at the vocabulary positions `index` (..., k).
+    With q = softmax(teacher / T) and p = softmax(logits / T), the sum over positions of
+    weights * T^2 * sum_k q (log q - log p). Entries of -inf are absent (rows may hold fewer than k), an
+    index given twice counts twice, and k is at most 1024."""
+    c = _Call(logits)
+    if not isinstance(index, torch.Tensor) or index.dim() < 1:
+        raise TypeError("index must be a tensor with a last axis of teacher entries")
+    k = index.shape[-1]
+    index = c.per_row(index, "index", shape=(*c.lead, k), dtype=torch.int32)
+    teacher = c.per_row(teacher, "teacher", shape=(*c.lead, k))
+    w = c.per_row(weights, "weights")
+    g, ga = c.gradient(grad, out)
+    loss, terms = c.new(), c.new(*c.lead)
+    c.run(_native().distillation_loss, c.args, index.data_ptr(), teacher.data_ptr(), w.data_ptr(), k, temperature, loss.data_ptr(), terms.data_ptr(), ga)
+    return DistillationLoss(loss, terms, g)
