@@ -69,4 +69,15 @@ struct DistillArgs {
 };
 cudaError_t distill_loss(EType t, const RowView& x, const DistillArgs& a, void* loss, void* terms, const RowOut& grad, cudaStream_t s);
 
+// The same by type.
+template <typename T> struct Objectives {
+  static cudaError_t log_prob(const RowView& x, const int32_t* labels, void* logp, void* stats, cudaStream_t s);
+  static cudaError_t log_prob_grad(const RowView& x, const int32_t* labels, const void* stats, const void* dlogp, const RowOut& grad, cudaStream_t s);
+  static cudaError_t policy(const RowView& x, const int32_t* labels, const PolicyArgs& a, void* loss, void* terms, void* logp, const RowOut& grad,
+                            cudaStream_t s);
+  static cudaError_t preference(const RowView& x, const int32_t* labels, const PreferenceArgs& a, void* loss, void* margins, void* logp, const RowOut& grad,
+                                void* workspace, cudaStream_t s);
+  static cudaError_t distill(const RowView& x, const DistillArgs& a, void* loss, void* terms, const RowOut& grad, cudaStream_t s);
+};
+
 }  // namespace rgc

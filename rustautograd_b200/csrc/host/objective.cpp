@@ -7,7 +7,7 @@ namespace rg {
 namespace {
 
 constexpr size_t MAX_TEACHER = 1024;  // teacher entries per row the device's kernel holds
-constexpr size_t MAX_VOCAB = 0x7fffffff;
+constexpr size_t MAX_VOCAB = size_t(1) << 30;
 
 bool attrs_ok(const Op& op, size_t n) {
   if (!op.value || op.value->n() != n) return false;

@@ -29,52 +29,63 @@ def _native():
     return _rg
 
 
-def _two_strides(x, what):
-    """(outer, inner, outer stride, inner stride) of the leading axes of `x`."""
-    shape, stride = x.shape, x.stride()
-    if len(shape) < 1:
-        raise ValueError(f"{what} needs a last axis")
-    if stride[-1] != 1 and shape[-1] != 1:
-        raise ValueError(f"the last axis of {what} must be contiguous")
-    groups = []  # [extent, stride], slowest first; axes that chain share a group
-    for n, s in zip(shape[:-1], stride[:-1]):
+def _rows(x, out=None):
+    """The leading axes of `x` as (outer, inner, outer stride, inner stride), and the same strides of `out`:
+    axes that chain in both are one."""
+    if x.dim() < 1:
+        raise ValueError("logits need a last axis")
+    shape = x.shape
+    strides = [x.stride()] if out is None else [x.stride(), out.stride()]
+    for s in strides:
+        if s[-1] != 1 and shape[-1] != 1:
+            raise ValueError("the last axis of the logits and of out must be contiguous")
+    groups = []  # (extent, stride of each), slowest first
+    for axis, n in enumerate(shape[:-1]):
         if n == 1:
             continue
-        if groups and groups[-1][1] == n * s:
-            groups[-1] = [groups[-1][0] * n, s]
+        at = [s[axis] for s in strides]
+        if groups and all(before == n * s for before, s in zip(groups[-1][1], at)):
+            groups[-1] = (groups[-1][0] * n, at)
         else:
-            groups.append([n, s])
+            groups.append((n, at))
     if len(groups) > 2:
-        raise ValueError(f"the leading axes of {what} have more than two independent strides; make it contiguous")
-    while len(groups) < 2:
-        groups.append([1, 0])
-    (outer, so), (inner, si) = groups
+        raise ValueError("the leading axes of the logits (and of out) have more than two independent strides; make them contiguous")
+    none = (1, [0] * len(strides))
+    (outer, so), (inner, si) = groups + [none] * (2 - len(groups))
     return outer, inner, so, si
 
 
 class _Call:
-    """The logits of a call and the stream it runs on."""
+    """The logits of a call, where their gradient goes, and the stream it runs on. `sequences`: the leading
+    axes are (sequences, positions) as they are."""
 
-    def __init__(self, logits, sequences=False):
+    def __init__(self, logits, grad=False, out=None, sequences=False):
         if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
             raise TypeError("logits must be a CUDA tensor")
-        self.dtype = _DTYPES.get(logits.dtype)
-        if self.dtype is None:
+        dtype = _DTYPES.get(logits.dtype)
+        if dtype is None:
             raise TypeError(f"logits must be float32 or float64, not {logits.dtype}")
-        self.logits, self.device = logits, logits.device
-        self.lead = logits.shape[:-1]
-        if sequences:
-            if logits.dim() != 3:
-                raise ValueError("logits must be (sequences, positions, vocabulary)")
-            outer, inner, vocab = logits.shape
-            so, si, last = logits.stride()
-            if last != 1 and vocab != 1:
-                raise ValueError("the last axis of logits must be contiguous")
+        if sequences and logits.dim() != 3:
+            raise ValueError("logits must be (sequences, positions, vocabulary)")
+        self.logits, self.device, self.lead, self.dtype = logits, logits.device, logits.shape[:-1], dtype
+        if out is None:
+            self.grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
+        elif not grad:
+            raise ValueError("out is given but no gradient is asked for")
+        elif not isinstance(out, torch.Tensor) or out.device != logits.device or out.dtype != logits.dtype or out.shape != logits.shape:
+            raise ValueError("out must have the logits' shape, dtype and device")
         else:
-            outer, inner, so, si = _two_strides(logits, "logits")
-            vocab = logits.shape[-1]
-        self.rows = (outer, inner)
-        self.args = (logits.data_ptr(), outer, inner, vocab, so, si, self.dtype)
+            self.grad = out
+        if sequences:
+            strides = [logits.stride()] if self.grad is None else [logits.stride(), self.grad.stride()]
+            if any(s[2] != 1 for s in strides) and logits.shape[2] != 1:
+                raise ValueError("the last axis of the logits and of out must be contiguous")
+            outer, inner = logits.shape[:2]
+            so, si = [s[0] for s in strides], [s[1] for s in strides]
+        else:
+            outer, inner, so, si = _rows(logits, self.grad)
+        self.args = (logits.data_ptr(), outer, inner, logits.shape[-1], so[0], si[0], dtype)
+        self.grad_args = (0, 0, 0) if self.grad is None else (self.grad.data_ptr(), so[1], si[1])
 
     def per_row(self, t, what, shape=None, dtype=None):
         """A contiguous operand on the logits' device."""
@@ -89,29 +100,6 @@ class _Call:
 
     def new(self, *shape):
         return torch.empty(shape, dtype=self.logits.dtype, device=self.device)
-
-    def gradient(self, grad, out, sequences=False):
-        """(tensor, call argument) of the gradient."""
-        if not grad:
-            if out is not None:
-                raise ValueError("out is given but no gradient is asked for")
-            return None, (0, 0, 0)
-        if out is None:
-            out = self.new(*self.logits.shape)
-        elif not isinstance(out, torch.Tensor) or out.device != self.device or out.dtype != self.logits.dtype or out.shape != self.logits.shape:
-            raise ValueError("out must have the logits' shape, dtype and device")
-        if sequences:
-            if out.stride(2) != 1 and out.shape[2] != 1:
-                raise ValueError("the last axis of out must be contiguous")
-            return out, (out.data_ptr(), out.stride(0), out.stride(1))
-        if out.is_contiguous():
-            outer, inner = self.rows
-            v = self.logits.shape[-1]
-            return out, (out.data_ptr(), inner * v, v)
-        outer, inner, so, si = _two_strides(out, "out")
-        if (outer, inner) != self.rows:
-            raise ValueError("out's strides do not split its rows as the logits' strides do; make it contiguous")
-        return out, (out.data_ptr(), so, si)
 
     def run(self, call, *args):
         if self.device.index == torch.cuda.current_device():
@@ -134,13 +122,12 @@ def token_log_prob(logits, labels, *, stats=False):
 
 def token_log_prob_grad(logits, labels, stats, dlogp, *, out=None):
     """The gradient with respect to `logits` of token_log_prob for the cotangent `dlogp`."""
-    c = _Call(logits)
+    c = _Call(logits, True, out)
     labels = c.per_row(labels, "labels", dtype=torch.int32)
     stats = c.per_row(stats, "stats", shape=(*c.lead, 2))
     dlogp = c.per_row(dlogp, "dlogp")
-    grad, g = c.gradient(True, out)
-    c.run(_native().token_log_prob_grad, c.args, labels.data_ptr(), stats.data_ptr(), dlogp.data_ptr(), g)
-    return grad
+    c.run(_native().token_log_prob_grad, c.args, labels.data_ptr(), stats.data_ptr(), dlogp.data_ptr(), c.grad_args)
+    return c.grad
 
 
 class PolicyLoss(NamedTuple):
@@ -156,17 +143,16 @@ def policy_loss(logits, labels, old_logp, advantages, weights, *, ref_logp=None,
     mask and the averaging (mask / mask.sum() for a mean over tokens). `ref_logp` goes with a kl != 0."""
     if (kl != 0) != (ref_logp is not None):
         raise ValueError("ref_logp goes with a kl coefficient that is not 0")
-    c = _Call(logits)
+    c = _Call(logits, grad, out)
     labels = c.per_row(labels, "labels", dtype=torch.int32)
     old = c.per_row(old_logp, "old_logp")
     adv = c.per_row(advantages, "advantages")
     w = c.per_row(weights, "weights")
     ref = c.per_row(ref_logp, "ref_logp") if ref_logp is not None else None
-    g, ga = c.gradient(grad, out)
     loss, terms, logp = c.new(), c.new(*c.lead), c.new(*c.lead)
     c.run(_native().policy_loss, c.args, labels.data_ptr(), old.data_ptr(), adv.data_ptr(), w.data_ptr(), 0 if ref is None else ref.data_ptr(),
-          clip_low, clip_high, kl, loss.data_ptr(), terms.data_ptr(), logp.data_ptr(), ga)
-    return PolicyLoss(loss, terms, logp, g)
+          clip_low, clip_high, kl, loss.data_ptr(), terms.data_ptr(), logp.data_ptr(), c.grad_args)
+    return PolicyLoss(loss, terms, logp, c.grad)
 
 
 class PreferenceLoss(NamedTuple):
@@ -181,20 +167,19 @@ def preference_loss(logits, labels, weights, ref_logp, *, beta=0.1, smoothing=0.
     ones: S = sum over positions of weights * logp, h = beta ((S - ref_logp)[chosen] - (S - ref_logp)[rejected]),
     and the mean over pairs of -(1 - smoothing) log sigma(h) - smoothing log sigma(-h). `ref_logp` (2 n,) holds the
     reference's S; weights are the mask of the answers' tokens (divided by their number for a mean per token)."""
-    c = _Call(logits, sequences=True)
-    n, t = c.rows
+    c = _Call(logits, grad, out, sequences=True)
+    n, t = c.lead
     if n < 2 or n % 2:
         raise ValueError("logits must hold pairs of sequences: an even number of at least 2")
     labels = c.per_row(labels, "labels", dtype=torch.int32)
     w = c.per_row(weights, "weights")
     ref = c.per_row(ref_logp, "ref_logp", shape=(n,))
-    g, ga = c.gradient(grad, out, sequences=True)
     nbytes = _native().preference_workspace(n, t, c.dtype)
     workspace = torch.empty((nbytes,), dtype=torch.uint8, device=c.device)
     loss, margins, logp = c.new(), c.new(n // 2), c.new(n)
     c.run(_native().preference_loss, c.args, labels.data_ptr(), w.data_ptr(), ref.data_ptr(), beta, smoothing, loss.data_ptr(), margins.data_ptr(),
-          logp.data_ptr(), ga, workspace.data_ptr(), nbytes)
-    return PreferenceLoss(loss, margins, logp, g)
+          logp.data_ptr(), c.grad_args, workspace.data_ptr(), nbytes)
+    return PreferenceLoss(loss, margins, logp, c.grad)
 
 
 class DistillationLoss(NamedTuple):
@@ -208,14 +193,13 @@ def distillation_loss(logits, index, teacher, weights, *, temperature=1.0, grad=
     With q = softmax(teacher / T) and p = softmax(logits / T), the sum over positions of
     weights * T^2 * sum_k q (log q - log p). Entries of -inf are absent (rows may hold fewer than k), an
     index given twice counts twice, and k is at most 1024."""
-    c = _Call(logits)
+    c = _Call(logits, grad, out)
     if not isinstance(index, torch.Tensor) or index.dim() < 1:
         raise TypeError("index must be a tensor with a last axis of teacher entries")
     k = index.shape[-1]
     index = c.per_row(index, "index", shape=(*c.lead, k), dtype=torch.int32)
     teacher = c.per_row(teacher, "teacher", shape=(*c.lead, k))
     w = c.per_row(weights, "weights")
-    g, ga = c.gradient(grad, out)
     loss, terms = c.new(), c.new(*c.lead)
-    c.run(_native().distillation_loss, c.args, index.data_ptr(), teacher.data_ptr(), w.data_ptr(), k, temperature, loss.data_ptr(), terms.data_ptr(), ga)
-    return DistillationLoss(loss, terms, g)
+    c.run(_native().distillation_loss, c.args, index.data_ptr(), teacher.data_ptr(), w.data_ptr(), k, temperature, loss.data_ptr(), terms.data_ptr(), c.grad_args)
+    return DistillationLoss(loss, terms, c.grad)

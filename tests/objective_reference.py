@@ -3,9 +3,11 @@ rounding error of an implementation that works in `dtype`, to first order in its
 1.25 for the higher orders; exponentials and logarithms count two units in the last place, 4 u).
 
 The bound of a row: with z the (scaled) logits, m their maximum, s the sum of exp(z - m) and p = exp(z - m) / s,
-a computed exp(z_j - m) is off by u (|z_j - m| + 4) relatively, and by 2 u (|z_j| + |m|) more where the
-logits were scaled first. s is off by the p-weighted mean of that plus u per addition on the longest path of
-sums, `adds`. From those follow the bounds of log s, lp, p and of what is computed from them.
+a computed exp(z_j - m) is off by u (2.3 |z_j - m| + 4) relatively: the difference is rounded, the exponent
+of the power of two that stands for it is rounded (u each, times ln 2 log2 e = 1), and log2 e (or log2 e / T) as
+a float is off by at most 0.3 u of it. It is off by 2 u (|z_j| + |m|) more where the logits were scaled first. s is off by the p-weighted mean of that plus u per addition on the longest path of
+sums, `adds`. An exponential below the smallest normal number may be taken as 0, and so may the factor
+between two parts of a row: 2 tiny of p (s is at least 1). From those follow the bounds of log s, lp, p and of what is computed from them.
 """
 import numpy as np
 
@@ -26,7 +28,7 @@ class Rows:
             self.p = e / self.s
             far = np.where(np.isfinite(z), np.abs(z - self.m), 0)
             scaled = 0 if temperature == 1.0 else 2 * (np.where(np.isfinite(z), np.abs(z), 0) + np.abs(self.m))
-            self.rel_e = self.u * (far + scaled + 4)
+            self.rel_e = self.u * (2.3 * far + scaled + 4)
             self.rel_s = (self.p * self.rel_e).sum(-1, keepdims=True) + self.u * adds
             self.rel_p = self.rel_e + self.rel_s + 3 * self.u
             self.logs = np.log(self.s)
@@ -44,7 +46,7 @@ class Rows:
         hot = np.zeros_like(self.p)
         np.put_along_axis(hot, label, 1, -1)
         d = hot - self.p
-        return c * d, np.abs(c) * self.p * self.rel_p + 4 * self.u * np.abs(c * d) + dc * np.abs(d) + self.tiny
+        return c * d, np.abs(c) * self.p * self.rel_p + 4 * self.u * np.abs(c * d) + dc * np.abs(d) + self.tiny * (1 + 2 * np.abs(c))
 
 
 def _labels(labels, v):
@@ -153,7 +155,7 @@ def distillation(x, index, teacher, weight, temperature, dtype, adds):
         np.subtract.at(g[row], at[row], q.p[row])
         np.add.at(dg[row], at[row], q.p[row] * (q.rel_p[row] + (k + 2) * u) + r.p[row][at[row]] * 2 * u)
     c = (w * t)[:, None]
-    g, dg = c * g, np.abs(c) * dg + 4 * u * np.abs(c * g) + r.tiny
+    g, dg = c * g, np.abs(c) * dg + 4 * u * np.abs(c * g) + r.tiny * (1 + 2 * np.abs(c))
 
     def spread(values, like):
         out = np.zeros(like, L)

@@ -117,43 +117,54 @@ def test_distillation_loss(rows, v, dtype):
         check(alone[:2], want, r._fields, f"distillation without gradient {rows}x{v} {kind} k {k}")
 
 
-def all_calls(x, lab, rng, dtype, out=None):
-    """The four operators on the same (n, t, V) logits: a list of outputs, gradients last in each."""
+def all_calls(x, lab, rng, dtype):
+    """The four operators on (n, t, V) logits: a function of (logits, labels, out) to their outputs, gradients
+    last in each, and what the outputs should be (None for the statistics)."""
     n, t, v = x.shape
-    old, adv, w, ref = (torch.from_numpy(a).cuda().reshape(n, t) for a in R.policy_inputs(
-        rng, x.cpu().numpy().reshape(-1, v), lab.cpu().numpy().reshape(-1), dtype))
-    index = torch.from_numpy(rng.integers(0, v, (n, t, 6)).astype("int32")).cuda()
-    teacher = torch.from_numpy(rng.normal(size=(n, t, 6)).astype(dtype)).cuda()
-    seq = torch.from_numpy((-rng.random(n) * t).astype(dtype)).cuda()
+    hx, hl = x.cpu().numpy().reshape(-1, v), lab.cpu().numpy().reshape(-1)
+    old, adv, w, ref = R.policy_inputs(rng, hx, hl, dtype)
+    index, teacher = rng.integers(0, v, (n * t, 6)).astype("int32"), rng.normal(size=(n * t, 6)).astype(dtype)
+    seq = (-rng.random(n) * t).astype(dtype)
+    want = [*R.token_log_prob(hx, hl, adv, dtype, adds(v)), *R.policy(hx, hl, old, adv, w, ref, 0.2, 0.28, 0.05, dtype, adds(v)),
+            *R.preference(hx.reshape(n, t, v), hl.reshape(n, t), w.reshape(n, t), seq, 0.1, 0.0, dtype, adds(v)),
+            *R.distillation(hx, index, teacher, w, 1.0, dtype, adds(v))]
+    want.insert(1, None)
+    dold, dadv, dw, dref = (a.reshape(n, t) for a in put(old, adv, w, ref))
+    dindex, dteacher = (a.reshape(n, t, 6) for a in put(index, teacher))
+    dseq = put(seq)[0]
 
     def go(x, lab, out=None):
         logp, stats = losses.token_log_prob(x, lab, stats=True)
-        res = [logp, stats, losses.token_log_prob_grad(x, lab, stats, adv, out=out)]
-        if out is not None:
-            res[-1] = res[-1].clone()
-        for r in (lambda: losses.policy_loss(x, lab, old, adv, w, ref_logp=ref, kl=0.05, out=out), lambda: losses.preference_loss(x, lab, w, seq, out=out),
-                  lambda: losses.distillation_loss(x, index, teacher, w, out=out)):
-            got = list(r())
-            if out is not None:
-                got[-1] = got[-1].clone()
-            res += got
+        calls = [lambda: (logp, stats, losses.token_log_prob_grad(x, lab, stats, dadv, out=out)),
+                 lambda: losses.policy_loss(x, lab, dold, dadv, dw, ref_logp=dref, clip_high=0.28, kl=0.05, out=out),
+                 lambda: losses.preference_loss(x, lab, dw, dseq, out=out), lambda: losses.distillation_loss(x, dindex, dteacher, dw, out=out)]
+        res = []
+        for call in calls:
+            *some, grad = call()
+            res += [*some, grad if out is None else grad.clone()]
         return res
-    return go
+    return go, want
+
+
+def check_all(got, want, what):
+    for k, (g, w) in enumerate(zip(got, want)):
+        if w is not None:
+            R.assert_within(get(g), w, f"output {k} of {what}")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("v", [5, 96, 1003, 8192, 33001])
 def test_strides_alignment_and_neighbours(v, dtype):
     # Logits as positions of a longer output, from an odd address, with rows apart, and transposed; gradients
-    # into views whose surroundings stay as they were. The bits do not depend on any of it.
+    # into views whose surroundings stay as they were, with the bits of a gradient of its own.
     rng = np.random.default_rng(v)
     n, t = 4, 5
     x = torch.from_numpy(R.logits(rng, n * t, v, "normal", dtype)).cuda().reshape(n, t, v)
     lab = torch.from_numpy(rng.integers(0, v, (n, t)).astype("int32")).cuda()
-    go = all_calls(x, lab, rng, dtype)
-    want = go(x, lab)
+    go, want = all_calls(x, lab, rng, dtype)
     flat = torch.full((1 + (n * (t + 2) + 1) * (v + 3),), 7.0, dtype=x.dtype, device="cuda")
     views = {
+        "plain": x,
         "shifted": torch.full((n, t + 1, v), 7.0, dtype=x.dtype, device="cuda")[:, :t],
         "odd address": flat[1:1 + n * t * v].view(n, t, v),
         "apart": flat[1:1 + n * (t + 2) * (v + 3)].view(n, t + 2, v + 3)[:, 1:t + 1, 2:v + 2],
@@ -161,22 +172,25 @@ def test_strides_alignment_and_neighbours(v, dtype):
     }
     for name, view in views.items():
         view.copy_(x)
-        for k, (a, b) in enumerate(zip(go(view, lab), want)):
-            assert torch.equal(a, b), (name, k)
-        out = torch.full_like(view, 3.0) if name == "transposed" else view.clone()
-        if name in ("shifted", "apart"):
-            base = torch.full((n, t + 2, v + 3), 3.0, dtype=x.dtype, device="cuda")
-            out = base[:, 1:t + 1, 2:v + 2]
-        for k, (a, b) in enumerate(zip(go(view, lab, out), want)):
-            assert torch.equal(a, b), (name, "out", k)
-        if name in ("shifted", "apart"):
-            mark = torch.ones_like(base, dtype=torch.bool)
-            mark[:, 1:t + 1, 2:v + 2] = False
-            assert (base[mark] == 3.0).all(), name
-    # Labels and weights that are views of something longer.
+        got = go(view, lab)
+        check_all(got, want, f"{name} {v}")
+        outs = {"like": view.clone() if name != "transposed" else torch.full_like(view, 3.0)}
+        if name in ("plain", "shifted", "apart"):
+            for first in range(4):
+                base = torch.full((n, t + 2, v + 5), 3.0, dtype=x.dtype, device="cuda")
+                outs[first] = base[:, 1:t + 1, first:v + first]
+        for key, out in outs.items():
+            for k, (a, b) in enumerate(zip(go(view, lab, out), got)):
+                assert torch.equal(a, b), (name, key, k)
+            if key != "like":
+                base = out._base
+                mark = torch.ones_like(base, dtype=torch.bool)
+                mark[:, 1:t + 1, key:v + key] = False
+                assert (base[mark] == 3.0).all(), (name, key)
+    # Labels that are a view of something longer.
     wide = torch.zeros((n, t + 1), dtype=torch.int32, device="cuda")
     wide[:, 1:] = lab
-    assert torch.equal(losses.token_log_prob(x, wide[:, 1:]), want[0])
+    assert torch.equal(losses.token_log_prob(x, wide[:, 1:]), losses.token_log_prob(x, lab))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -200,26 +214,26 @@ def test_gradient_in_place_of_the_logits(v, dtype):
 
 
 def test_many_rows_and_offsets_past_32_bits():
-    # 2^31 elements and more: the last rows against the same rows alone.
+    # 2^31 elements and more: the last rows, the others without weight or uniform.
     rng = np.random.default_rng(0)
     v, rows = 50257, 43000
     x = torch.empty((rows, v), device="cuda")
     x[:-3] = 1.0
-    tail = torch.from_numpy(R.logits(rng, 3, v, "normal", "float32")).cuda()
-    x[-3:] = tail
-    lab = torch.from_numpy(rng.integers(0, v, rows).astype("int32")).cuda()
-    old, w = torch.full((rows,), -9.0, device="cuda"), torch.zeros(rows, device="cuda")
+    tail = R.logits(rng, 3, v, "normal", "float32")
+    x[-3:] = put(tail)[0]
+    lab = rng.integers(0, v, rows).astype("int32")
+    old, w, adv = np.full(rows, -9.0, "float32"), np.zeros(rows, "float32"), rng.normal(size=rows).astype("float32")
     w[-3:] = 0.5
-    adv = torch.from_numpy(rng.normal(size=rows).astype("float32")).cuda()
-    r = losses.policy_loss(x, lab, old, adv, w, out=x)
-    s = losses.policy_loss(tail, lab[-3:], old[-3:], adv[-3:], w[-3:])
-    assert torch.equal(r.grad[-3:], s.grad) and torch.equal(r.terms[-3:], s.terms) and torch.equal(r.loss, s.loss)
-    assert not r.grad[:-3].any()
+    want = R.policy(tail, lab[-3:], old[-3:], adv[-3:], w[-3:], None, 0.2, 0.2, 0.0, "float32", adds(v))
+    r = losses.policy_loss(x, *put(lab, old, adv, w), out=x)
+    check((r.loss, r.terms[-3:], r.logp[-3:], r.grad[-3:]), want, r._fields, "the last rows")
+    assert not r.grad[:-3].any() and not r.terms[:-3].any()
     del r
     x[:-3] = 1.0
-    x[-3:] = tail
-    logp, stats = losses.token_log_prob(x, lab, stats=True)
-    assert torch.equal(logp[-3:], losses.token_log_prob(tail, lab[-3:]))
+    x[-3:] = put(tail)[0]
+    logp, stats = losses.token_log_prob(x, put(lab)[0], stats=True)
+    (want_logp, off), _ = R.token_log_prob(tail, lab[-3:], adv[-3:], "float32", adds(v))
+    R.assert_within(get(logp[-3:]), (want_logp, off), "the last rows")
     # A uniform row: the statistics are exact up to the sum's rounding.
     assert (stats[:-3, 0] == 1.0).all() and ((stats[:-3, 1] - v).abs() <= v * (adds(v) + 4) * 2.0 ** -24).all()
 
@@ -293,7 +307,7 @@ def test_streams_graphs_and_repeats():
     for v in (96, 1009, 32000):
         x = torch.from_numpy(R.logits(rng, 24, v, "normal", "float32")).cuda().reshape(4, 6, v)
         lab = torch.from_numpy(rng.integers(0, v, (4, 6)).astype("int32")).cuda()
-        cases.append((x, lab, all_calls(x, lab, rng, "float32")))
+        cases.append((x, lab, all_calls(x, lab, rng, "float32")[0]))
     want = [go(x, lab) for x, lab, go in cases]
     torch.cuda.synchronize()
     # On two streams at once, and again: the same bits.

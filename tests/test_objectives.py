@@ -311,12 +311,16 @@ def test_call_refusals_without_a_gpu(product):
     with pytest.raises(TypeError, match="CUDA tensor"):
         losses.token_log_prob(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int32))
     x = torch.zeros(4, 5, 6, 8)
-    assert losses._two_strides(x, "x") == (120, 1, 8, 0)
-    assert losses._two_strides(x[:, :, :-1], "x") == (20, 5, 48, 8)
-    assert losses._two_strides(x[:, 0], "x") == (4, 6, 240, 8)
-    assert losses._two_strides(x[0, 0, 0], "x") == (1, 1, 0, 0)
-    assert losses._two_strides(x.transpose(0, 2)[:, :, 0], "x") == (6, 5, 8, 48)
+    rows = lambda *a: losses._rows(*a)
+    assert rows(x) == (120, 1, [8], [0])
+    assert rows(x[:, :, :-1]) == (20, 5, [48], [8])
+    assert rows(x[:, 0]) == (4, 6, [240], [8])
+    assert rows(x[0, 0, 0]) == (1, 1, [0], [0])
+    assert rows(x.transpose(0, 2)[:, :, 0]) == (6, 5, [8], [48])
+    assert rows(x[0], torch.zeros(5, 7, 8)[:, :6]) == (5, 6, [48, 56], [8, 8])
     with pytest.raises(ValueError, match="two independent strides"):
-        losses._two_strides(x[:, :-1, :-1], "x")
+        rows(x[:, :-1, :-1])
+    with pytest.raises(ValueError, match="two independent strides"):
+        rows(x[:, :, :-1], torch.zeros(4, 6, 5, 8)[:, :-1])
     with pytest.raises(ValueError, match="contiguous"):
-        losses._two_strides(x.transpose(2, 3), "x")
+        rows(x.transpose(2, 3))
