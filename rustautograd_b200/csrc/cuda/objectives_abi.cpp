@@ -63,7 +63,7 @@ Rows check_logits(const rgc_logits* x) {
   if (x->outer < 0 || x->inner < 0) refuse("negative row count");
   if (x->vocab < 1 || x->vocab > (int64_t(1) << 30)) refuse("vocab must be between 1 and 2^30");
   constexpr int64_t LIMIT = int64_t(1) << 40;
-  if (x->outer > LIMIT || x->inner > LIMIT || (x->inner && x->outer > LIMIT / x->inner)) refuse("too many rows");
+  if (x->inner && x->outer > INT32_MAX / x->inner) refuse("too many rows (at most 2^31 - 1)");
   if (x->outer_stride < 0 || x->inner_stride < 0 || x->outer_stride > LIMIT || x->inner_stride > LIMIT) refuse("strides must be between 0 and 2^40");
   Rows r;
   r.t = x->dtype == 1 ? EType::F64 : EType::F32;

@@ -73,12 +73,14 @@ template <> struct Num<float> {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * k));
     return r;
   }
+  static __device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }  // a NaN gives the other
   static float factor(double scale) { return (float)(scale * 1.4426950408889634074); }
 };
 template <> struct Num<double> {
   static constexpr int VEC = 2;
   using Vec = double2;
   static __device__ __forceinline__ double exps(double d, double k) { return exp(d * k); }
+  static __device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
   static double factor(double scale) { return scale; }
 };
 
@@ -100,8 +102,7 @@ template <int G, typename T> __device__ __forceinline__ Stat<T> join(Stat<T> a, 
   T m = a.m;
 #pragma unroll
   for (int d = G / 2; d; d >>= 1) {
-    const T o = __shfl_xor_sync(~0u, m, d);
-    m = o > m ? o : m;
+    m = Num<T>::most(m, __shfl_xor_sync(~0u, m, d));
   }
   T s = a.s * Num<T>::exps(a.m - base(m), k);
 #pragma unroll
@@ -111,15 +112,26 @@ template <int G, typename T> __device__ __forceinline__ Stat<T> join(Stat<T> a, 
 
 // ---- rows in memory ----
 
+// Quotients of row numbers (below 2^31) by run-time divisors: a multiplication and a shift (FDiv).
+__device__ __forceinline__ unsigned quotient(unsigned n, const FDiv& f) { return (unsigned)(((unsigned long long)__umulhi(n, f.m) + n) >> f.s); }
+
 template <typename T> struct View {
   const T* data;
-  long long inner, v, so, si;
-  __device__ const T* row(long long r) const { return data + (r / inner) * so + (r % inner) * si; }
+  FDiv inner;
+  long long v, so, si;
+  __device__ __forceinline__ const T* row(long long r) const {
+    const unsigned a = quotient((unsigned)r, inner);
+    return data + a * so + ((unsigned)r - a * inner.d) * si;
+  }
 };
 template <typename T> struct Out {
   T* data;
-  long long inner, so, si;
-  __device__ T* row(long long r) const { return data + (r / inner) * so + (r % inner) * si; }
+  FDiv inner;
+  long long so, si;
+  __device__ __forceinline__ T* row(long long r) const {
+    const unsigned a = quotient((unsigned)r, inner);
+    return data + a * so + ((unsigned)r - a * inner.d) * si;
+  }
 };
 
 // A row as 16-byte vectors from an aligned address: element j is element (j + off) % VEC of vector
@@ -140,77 +152,95 @@ template <typename T> struct Span {
     lo = max(lo, first * VEC);
     hi = min(hi, end * VEC);
   }
-  __device__ __forceinline__ bool whole(int i) const { return i * VEC >= lo && (i + 1) * VEC <= hi; }
-  __device__ __forceinline__ bool has(int i, int c) const {
-    const int j = i * VEC + c;
-    return j >= lo && j < hi;
-  }
+  // The 16 bytes from element j on are all the row's.
+  __device__ __forceinline__ bool whole(int j) const { return j >= lo && j <= hi - VEC; }
+  __device__ __forceinline__ bool has(int j) const { return j >= lo && j < hi; }
   // Vector i, or -inf for elements that are not the row's.
   __device__ __forceinline__ void load(int i, T* x) const {
-    if (whole(i)) {
+    if (whole(i * VEC)) {
       const typename Num<T>::Vec t = *reinterpret_cast<const typename Num<T>::Vec*>(base + (long long)i * VEC);
       memcpy(x, &t, 16);
     } else {
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) x[c] = has(i, c) ? base[(long long)i * VEC + c] : neg_inf<T>();
+      for (int c = 0; c < VEC; ++c) x[c] = has(i * VEC + c) ? base[(long long)i * VEC + c] : neg_inf<T>();
     }
   }
 };
 
-// Stores this lane's vector i (values y) of a row whose logits span `x`, to the row at `g`. Lanes 0 .. G - 1
-// of a group hold vectors i .. i + G - 1. Where the row is aligned to 16 bytes as the logits are, that is a
-// vector store; where it is not, each lane joins the end of its vector with the beginning of its right
-// neighbour's, which is an aligned vector of the output, and the group's ends go element by element.
-// (A shifted slice of logits with an odd vocabulary has every alignment.)
-template <typename T, int G> struct Store {
-  static constexpr int VEC = Num<T>::VEC;
-  T* g;   // element j of the row is g[j]
-  int sh; // element of a logits vector that begins an output vector
-  __device__ __forceinline__ Store(T* row, const Span<T>& x) : g(row) {
-    const int goff = (int)(((unsigned long long)row / sizeof(T)) % VEC);
-    sh = (x.off - goff + VEC) % VEC;
-  }
-  __device__ __forceinline__ void put(const Span<T>& x, int i, int lane, const T* y) const {
-    T* at = g + ((long long)i * VEC - x.off);
-    if (sh == 0) {
-      if (x.whole(i)) {
-        typename Num<T>::Vec t;
-        memcpy(&t, y, 16);
-        *reinterpret_cast<typename Num<T>::Vec*>(at) = t;
-      } else {
+// Stores the vectors first + lane + G * e (e < E, values y) of a row whose logits span `x` to the row at
+// `row`, G lanes together. Where that row is aligned to 16 bytes as the logits are, a logits vector is an
+// output vector; where it is not, an output vector begins SH elements into a logits vector and ends in
+// the next one, which the right neighbour holds (lane 0's next vector for the last lane). The elements
+// before the group's first whole output vector and behind its last go one by one.
+// (A slice of positions of logits with an odd vocabulary has every alignment.)
+// INSIDE: all of the group's vectors are the row's.
+template <typename T, int G, int E, int SH, bool INSIDE>
+__device__ __forceinline__ void store_shifted(T* at0, const Span<T>& x, int first, int lane, const T* y) {
+  constexpr int VEC = Num<T>::VEC;
+  const int end = min(x.hi, (first + G * E) * VEC);  // what the group holds
 #pragma unroll
-        for (int c = 0; c < VEC; ++c)
-          if (x.has(i, c)) at[c] = y[c];
-      }
-      return;
-    }
-    T next[VEC - 1];
-#pragma unroll
-    for (int c = 0; c < VEC - 1; ++c) next[c] = __shfl_down_sync(~0u, y[c], 1, G);
+  for (int e = 0; e < E; ++e) {
     T o[VEC];
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) {
-      // element sh + c of (y, next)
-      T t = next[VEC - 2];
+    for (int c = 0; c < VEC - SH; ++c) o[c] = y[e * VEC + SH + c];
 #pragma unroll
-      for (int q = 2 * VEC - 3; q >= 0; --q)
-        if (sh + c == q) t = q < VEC ? y[q] : next[q - VEC];
-      o[c] = t;
+    for (int c = 0; c < SH; ++c) {
+      const T ahead = e + 1 < E ? y[(e + 1 < E ? e + 1 : e) * VEC + c] : y[e * VEC + c];
+      o[VEC - SH + c] = __shfl_sync(~0u, lane == 0 ? ahead : y[e * VEC + c], (lane + 1) % G, G);
     }
-    const bool inner = lane < G - 1 && x.has(i, sh) && x.has(i + 1, sh - 1);
-    if (inner) {
+    const int j = (first + lane + G * e) * VEC + SH;
+    T* at = at0 + j;
+    if (INSIDE ? SH == 0 || e < E - 1 || lane < G - 1 : j >= x.lo && j <= end - VEC) {
       typename Num<T>::Vec t;
       memcpy(&t, o, 16);
-      *reinterpret_cast<typename Num<T>::Vec*>(at + sh) = t;
-    }
-    // The rest of what this lane holds: its first sh elements unless its left neighbour stored them, the
-    // others unless it did so itself.
-    const bool left = lane > 0 && x.has(i - 1, sh) && x.has(i, sh - 1);
+      *reinterpret_cast<typename Num<T>::Vec*>(at) = t;
+    } else {
 #pragma unroll
-    for (int c = 0; c < VEC; ++c)
-      if (x.has(i, c) && !(c < sh ? left : inner)) at[c] = y[c];
+      for (int c = 0; c < VEC; ++c)
+        if (INSIDE ? c < VEC - SH : j + c >= x.lo && j + c < end) at[c] = o[c];
+    }
+    if (SH > 0 && e == 0 && lane == 0) {
+#pragma unroll
+      for (int c = 0; c < SH; ++c)
+        if (INSIDE || x.has(j - SH + c)) at[c - SH] = y[c];
+    }
   }
-};
+}
+template <typename T, int G, int E, bool INSIDE> __device__ __forceinline__ void store(T* row, const Span<T>& x, int first, int lane, const T* y) {
+  constexpr int VEC = Num<T>::VEC;
+  const int goff = (int)(((unsigned long long)row / sizeof(T)) % VEC), sh = (x.off - goff + VEC) % VEC;
+  T* at0 = row - x.off;  // where element 0 of `x` would go
+  if (sh == 0) store_shifted<T, G, E, 0, INSIDE>(at0, x, first, lane, y);
+  else if (sh == 1) store_shifted<T, G, E, 1, INSIDE>(at0, x, first, lane, y);
+  if constexpr (VEC == 4) {
+    if (sh == 2) store_shifted<T, G, E, 2, INSIDE>(at0, x, first, lane, y);
+    else if (sh == 3) store_shifted<T, G, E, 3, INSIDE>(at0, x, first, lane, y);
+  }
+}
+
+// The same for the groups of a warp, each with a row of its own (and an alignment of its own).
+template <typename T, int G, int E> __device__ __forceinline__ void store_group(T* row, const Span<T>& x, int lane, const T* y) {
+  constexpr int VEC = Num<T>::VEC;
+  if constexpr (G == 32) {
+    store<T, G, E, false>(row, x, 0, lane, y);
+  } else {
+    const int goff = (int)(((unsigned long long)row / sizeof(T)) % VEC), sh = (x.off - goff + VEC) % VEC;
+    T* at0 = row - x.off;
+    if (__all_sync(~0u, sh == 0)) {
+      store_shifted<T, G, E, 0, false>(at0, x, 0, lane, y);
+      return;
+    }
+    // Some of the warp's rows are shifted: element by element.
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        const int j = (lane + G * e) * VEC + c;
+        if (x.has(j)) at0[j] = y[e * VEC + c];
+      }
+    }
+  }
+}
 
 __device__ __forceinline__ long long clamp_label(int l, long long v) { return l < 0 ? 0 : l >= v ? v - 1 : l; }
 
@@ -226,9 +256,10 @@ template <typename T> struct LogProbRow {
   T *logp, *stats;
   struct Meta {
     int label;
-    bool live;
+    T w;
+    __device__ __forceinline__ bool live() const { return w != (T)0; }
   };
-  __device__ __forceinline__ Meta meta(long long r) const { return {labels[r], true}; }
+  __device__ __forceinline__ Meta meta(long long r) const { return {labels[r], (T)1}; }
   __device__ void skip(long long) const {}
   __device__ __forceinline__ T coef(const Meta&, T, Stat<T>) const { return (T)0; }
   __device__ __forceinline__ void report(long long r, const Meta&, T xl, Stat<T> st) const {
@@ -248,18 +279,24 @@ template <typename T> struct PolicyRow {
   T *terms, *logp;
   struct Meta {
     int label;
-    bool live;
     T w, a, old, ref;
+    __device__ __forceinline__ bool live() const { return w != (T)0; }
   };
   __device__ __forceinline__ Meta meta(long long r) const {
     Meta m;
     m.w = weight[r];
-    m.live = m.w != (T)0;
     m.label = labels[r];
     m.a = advantage[r];
     m.old = old_logp[r];
     m.ref = kl != (T)0 ? ref_logp[r] : (T)0;
     return m;
+  }
+  // The same from one value per lane of a warp.
+  __device__ __forceinline__ T field(long long r, int lane) const {
+    return lane == 0 ? weight[r] : lane == 1 ? advantage[r] : lane == 2 ? old_logp[r] : lane == 3 && kl != (T)0 ? ref_logp[r] : (T)0;
+  }
+  __device__ __forceinline__ Meta gather(int label, T f) const {
+    return {label, __shfl_sync(~0u, f, 0), __shfl_sync(~0u, f, 1), __shfl_sync(~0u, f, 2), __shfl_sync(~0u, f, 3)};
   }
   __device__ void skip(long long r) const {
     terms[r] = (T)0;
@@ -295,21 +332,19 @@ template <typename T> struct GivenRow {
   static constexpr bool TARGETS = false, GIVEN = true;
   const int32_t* labels;
   const T *stats, *by_row, *by_sequence, *weight;
-  long long length;
+  FDiv length;
   struct Meta {
     int label;
-    bool live;
-    T c, m, s;
+    T w, c, m, s;
+    __device__ __forceinline__ bool live() const { return w != (T)0; }
   };
   __device__ __forceinline__ Meta meta(long long r) const {
     Meta q;
     if (by_row) {
-      q.c = by_row[r];
-      q.live = q.c != (T)0;
+      q.w = q.c = by_row[r];
     } else {
-      const T w = weight[r];
-      q.live = w != (T)0;
-      q.c = q.live ? by_sequence[r / length] * w : (T)0;
+      q.w = weight[r];
+      q.c = q.live() ? by_sequence[quotient((unsigned)r, length)] * q.w : (T)0;
     }
     q.label = labels[r];
     q.m = stats[2 * r];
@@ -319,6 +354,11 @@ template <typename T> struct GivenRow {
   __device__ void skip(long long) const {}
   __device__ __forceinline__ T coef(const Meta& q, T, Stat<T>) const { return q.c; }
   __device__ __forceinline__ void report(long long, const Meta&, T, Stat<T>) const {}
+};
+
+struct EntriesPart {
+  double a, q;
+  bool some;  // the row has entries
 };
 
 // The distillation: a row's targets are its teacher entries. `prepare` (one warp) gives q at shared arrays
@@ -334,16 +374,12 @@ template <typename T> struct DistillRow {
   T wt;            // T
   T* terms;
   struct Meta {
-    bool live;
     T w;
+    __device__ __forceinline__ bool live() const { return w != (T)0; }
   };
-  struct Part {
-    double a = 0, q = 0;
-    bool some = false;  // the row has entries
-  };
+  using Part = EntriesPart;
   __device__ __forceinline__ Meta meta(long long r) const {
-    const T w = weight[r];
-    return {w != (T)0, w};
+    return {weight[r]};
   }
   __device__ void skip(long long r) const { terms[r] = (T)0; }
   __device__ __forceinline__ void report(long long r, const Meta& m, Part p, Stat<T> st) const {
@@ -361,7 +397,7 @@ template <typename T> struct DistillRow {
       st.m = m;
     }
     st = join<32>(st, tk);
-    Part p;
+    Part p{0, 0, false};
     p.some = st.s != (T)0;  // all entries -inf: none
     const T inv = (T)1 / st.s;
     const double logs = log((double)st.s);
@@ -394,7 +430,7 @@ constexpr int GROUP_THREADS = 256;
 template <typename T, int N> __device__ __forceinline__ Stat<T> exponentials(T* x, T k) {
   Stat<T> a;
 #pragma unroll
-  for (int i = 0; i < N; ++i) a.m = x[i] > a.m ? x[i] : a.m;
+  for (int i = 0; i < N; ++i) a.m = Num<T>::most(x[i], a.m);
   const T b = base(a.m);
   // Two sums: half the rounding of one long chain, and half its latency.
   T s0 = (T)0, s1 = (T)0;
@@ -404,6 +440,32 @@ template <typename T, int N> __device__ __forceinline__ Stat<T> exponentials(T* 
     if (i % 2) s1 += x[i];
     else s0 += x[i];
   }
+  a.s = s0 + s1;
+  return a;
+}
+
+// The same of the first `turns` of E vectors.
+template <typename T, int E, int VEC> __device__ __forceinline__ Stat<T> exponentials(T* x, T k, int turns) {
+  Stat<T> a;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (e < turns) {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) a.m = Num<T>::most(x[e * VEC + c], a.m);
+    }
+  const T b = base(a.m);
+  T s0 = (T)0, s1 = (T)0;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (e < turns) {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        T& z = x[e * VEC + c];
+        z = Num<T>::exps(z - b, k);
+        if (c % 2) s1 += z;
+        else s0 += z;
+      }
+    }
   a.s = s0 + s1;
   return a;
 }
@@ -426,7 +488,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) k_group(View<T> x, long long ro
     const bool in = r < rows;
     typename Obj::Meta meta{};
     if (in) meta = obj.meta(r);
-    const bool live = in && meta.live;
+    const bool live = in && meta.live();
     const Span<T> row(x.row(in ? r : 0), in ? x.v : 0);
     T y[E * VEC];
 #pragma unroll
@@ -464,7 +526,6 @@ __global__ void __launch_bounds__(GROUP_THREADS) k_group(View<T> x, long long ro
         f = share(own.m, st, k, -c);
       }
       if (GRAD) {
-        const Store<T, G> out(g.row(in ? r : 0), row);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
 #pragma unroll
@@ -474,8 +535,8 @@ __global__ void __launch_bounds__(GROUP_THREADS) k_group(View<T> x, long long ro
             for (int q = 0; q < VEC; ++q)
               if (l % VEC == q) y[e * VEC + q] += c;
           }
-          out.put(row, lane + G * e, lane, y + e * VEC);
         }
+        store_group<T, G, E>(g.row(in ? r : 0), row, lane, y);
       }
       if (lane == 0 && in) {
         if (live) obj.report(r, meta, xl, st);
@@ -487,7 +548,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) k_group(View<T> x, long long ro
       T* q = hit + E * 32 * VEC;
       T* xk = q + obj.k;
       int* at = (int*)((T*)dyn + (GROUP_THREADS / 32) * (E * 32 * VEC + 2 * obj.k)) + (threadIdx.x / 32) * obj.k;
-      typename Obj::Part part;
+      typename Obj::Part part{0, 0, false};
       if (live) part = obj.prepare(r, x.row(r), x.v, lane, GRAD ? at : nullptr, q, xk);
       const bool some = live && part.some;
       if (GRAD && some) {
@@ -513,13 +574,12 @@ __global__ void __launch_bounds__(GROUP_THREADS) k_group(View<T> x, long long ro
       const Stat<T> st = join<G>(own, k);
       if (GRAD) {
         const T c = meta.w * obj.wt, f = some ? share(own.m, st, k, c) : (T)0;
-        const Store<T, G> out(g.row(in ? r : 0), row);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
 #pragma unroll
           for (int z = 0; z < VEC; ++z) y[e * VEC + z] = some ? y[e * VEC + z] * f - c * hit[(lane + 32 * e) * VEC + z] : (T)0;
-          out.put(row, lane + G * e, lane, y + e * VEC);
         }
+        store_group<T, G, E>(g.row(in ? r : 0), row, lane, y);
         __syncwarp();
       }
       if (lane == 0 && in) {
@@ -558,6 +618,10 @@ template <typename T> __device__ __forceinline__ void put_remote(Pair<T>* p, uns
 }
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+// With constant distances (bytes) from both addresses.
+template <int TO, int FROM> __device__ __forceinline__ void copy16_at(unsigned dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(dst), "l"(src), "n"(TO), "n"(FROM) : "memory");
 }
 template <int BYTES> __device__ __forceinline__ void copy_element(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(dst)), "l"(src), "n"(BYTES) : "memory");
@@ -598,44 +662,114 @@ template <typename T, int NW, bool CLUSTER> struct Table {
 // Entries of a row's distillation targets, kept until its gradient has been written.
 template <typename T> struct Kept {
   long long row = -1;
-  T c = 0, inv = 0, m = 0;  // the gradient at an entry: c (exp((x - m) k) inv - sum q)
+  T c = 0, scale = 0, m = 0;  // the gradient at an entry: exp((x - m) k) scale - c sum q
 };
 
-// A block of NT threads (or a cluster of such blocks, `slice` vectors each) per row; thread t holds vectors
-// t, t + NT, .. of its block's slice in registers. The copies of the next STAGES rows are under way meanwhile:
-// a thread copies exactly what it will read itself, so no barrier stands between copy and use.
+// f(0) .. f(N - 1) with compile-time numbers.
+template <int N, int I = 0, typename F> __device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<N, I + 1>(f);
+  }
+}
+
+// What a row's gradient needs, from one warp to all.
+template <typename T> struct Scalars {
+  T c, scale, m;  // c; the factor of exp((x - m) k); m
+  int at;         // the label's element, counted as a Span's; or whether the row has entries
+};
+
+// Calls, not inlined: one warp makes them while every warp's registers hold a row.
+template <typename T, class Obj> __device__ __noinline__ T coef_of(const Obj& obj, int label, T fields, T xl, Stat<T> st) {
+  return obj.coef(obj.gather(label, fields), xl, st);
+}
+template <typename T, class Obj> __device__ __noinline__ void report_of(const Obj& obj, long long r, int label, T fields, T xl, Stat<T> st) {
+  const typename Obj::Meta m = obj.gather(label, fields);
+  if (threadIdx.x % 32 == 0) obj.report(r, m, xl, st);
+}
+template <typename T, class Obj>
+__device__ __noinline__ void entries_of(const Obj& obj, long long r, const T* x, long long v, int* at, T* q, T* xk, typename Obj::Part* part) {
+  const typename Obj::Part p = obj.prepare(r, x, v, threadIdx.x % 32, at, q, xk);
+  if (threadIdx.x % 32 == 0) *part = p;
+}
+template <typename T, class Obj> __device__ __noinline__ void report_entries(const Obj& obj, long long r, const typename Obj::Part& part, Stat<T> st) {
+  if (threadIdx.x % 32 == 0) obj.report(r, obj.meta(r), part, st);
+}
+
+// A block of NT threads (or a cluster of such blocks, `slice` vectors each) per row. A warp holds 32 * turns
+// adjacent vectors of its block's slice in registers (turns <= E), as vectors of the gradient, which are stored
+// whole; the logits they need come through the warp's own piece of shared memory, where an offset between the
+// alignments of the two (a slice of positions of logits with an odd vocabulary has every one) costs element-wise
+// reads and nothing else. The copies of the next STAGES rows are under way meanwhile: a warp copies what it
+// will read itself, so no block-wide barrier stands between copy and use.
+// Issue slots are what is scarce (45 per logit and lane at the copy rate), so warps whose vectors are all inside
+// the row take a path without bounds, and what a row needs once is computed by one warp.
 template <typename T, int NT, int E, int STAGES, bool CLUSTER, class Obj>
-__global__ void __launch_bounds__(NT, 1024 / NT) k_block(View<T> x, long long rows, Obj obj, T k, Out<T> g, int slice) {
-  constexpr int VEC = Num<T>::VEC, NW = NT / 32;
+__global__ void __launch_bounds__(NT, 512 / NT)
+    k_block(const View<T> x, const long long rows, const __grid_constant__ Obj obj, const T k, const Out<T> g, const int slice, const int turns) {
+  constexpr int VEC = Num<T>::VEC, NW = NT / 32, PIECE = 32 * E + 1;  // a piece has one vector more for the offset
+  using Vec = typename Num<T>::Vec;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Table<T, NW, CLUSTER> table;
-  using Vec = typename Num<T>::Vec;
-  Vec* ring = (Vec*)dyn;
+  __shared__ Scalars<T> scalars;
   const unsigned rank = CLUSTER ? cluster_rank() : 0, blocks = CLUSTER ? cluster_size() : 1;
   const long long step = gridDim.x / blocks, first = blockIdx.x / blocks;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int begin = (int)rank * slice, at0 = begin + (int)threadIdx.x;  // this thread's vectors: at0 + NT * e
+  Vec* ring = (Vec*)dyn + warp * STAGES * PIECE;
+  // This warp's first vector; this thread's are warp0 + lane + 32 * e.
+  const int begin = (int)rank * slice, warp0 = begin + warp * 32 * turns;
   pdl_wait();
   if constexpr (CLUSTER) cluster_sync();  // every block's shared memory is there before another writes to it
 
+  // Row r, elements counted from the gradient's 16-byte boundary before it: element u is logit u - off. The
+  // warp's piece begins `shift` elements before its first element.
+  struct Place {
+    const T* from;  // the piece's first logit, 16-byte aligned
+    T* to;          // the gradient's element 0
+    int off, lo, hi, shift;
+  };
+  auto place = [&](long long r) {
+    Place q;
+    T* gr = g.row(r);
+    q.off = (int)(((unsigned long long)gr / sizeof(T)) % VEC);
+    q.to = gr - q.off;
+    q.lo = max(q.off, begin * VEC);
+    q.hi = min(q.off + (int)x.v, (begin + slice) * VEC);
+    const T* at = x.row(r) + ((long long)warp0 * VEC - q.off);
+    q.shift = (int)(((unsigned long long)at / sizeof(T)) % VEC);
+    q.from = at - q.shift;
+    return q;
+  };
+  const int last = warp0 + 32 * turns;
+  auto inside = [&](const Place& q) { return warp0 * VEC >= q.lo && last * VEC <= q.hi; };
   auto fetch = [&](long long r, int stage) {
-    Span<T> row(x.row(r), x.v);
-    row.clip(begin, begin + slice);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = at0 + NT * e;
-      Vec* to = &ring[(stage * E + e) * NT + threadIdx.x];
-      if (row.whole(i)) {
-        copy16(to, row.base + (long long)i * VEC);
-      } else {
-#pragma unroll
-        for (int c = 0; c < VEC; ++c)
-          if (row.has(i, c)) copy_element<sizeof(T)>((T*)to + c, row.base + (long long)i * VEC + c);
+    const Place q = place(r);
+    Vec* to = ring + stage * PIECE;
+    // The row's elements in the piece: from_lo .. from_hi - 1 of it.
+    const int from_lo = q.off - (warp0 * VEC - q.shift), from_hi = from_lo + (int)x.v, need = min(q.hi - warp0 * VEC, 32 * turns * VEC) + q.shift;
+    if (from_lo <= 0 && from_hi >= (32 * turns + 1) * VEC && need > 0) {
+      const unsigned d = smem_addr(to + lane);
+      const T* from = q.from + lane * VEC;
+      each<E>([&](auto e) {
+        if (e < turns) copy16_at<e * 512, e * 512>(d, from);
+      });
+      if (q.shift && lane == 0) copy16(to + 32 * turns, q.from + 32 * turns * VEC);
+    } else if (need > 0) {
+#pragma unroll 1
+      for (int i = lane; i * VEC < need; i += 32) {
+        const int j = i * VEC;
+        if (j >= from_lo && j + VEC <= from_hi) {
+          copy16(to + i, q.from + j);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < VEC; ++c)
+            if (j + c >= from_lo && j + c < from_hi) copy_element<sizeof(T)>((T*)(to + i) + c, q.from + j + c);
+        }
       }
     }
   };
   // Distillation: two halves of k entries each, the row they belong to, and what its gradient needs.
-  T* tq = (T*)(ring + STAGES * E * NT);
+  T* tq = (T*)((Vec*)dyn + NW * STAGES * PIECE);
   T* tx = nullptr;
   int* ti = nullptr;
   Kept<T> kept;
@@ -643,6 +777,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_block(View<T> x, long long ro
     tx = tq + 2 * obj.k;
     ti = (int*)(tx + 2 * obj.k);
   }
+  __shared__ typename std::conditional<Obj::TARGETS, EntriesPart, int>::type part;
   // After a barrier that orders the row's gradient before it: the entries of the row. The first entry
   // of an index writes its element, with the probabilities of all entries of that index in order.
   auto finish = [&](int half) {
@@ -651,140 +786,174 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_block(View<T> x, long long ro
       T* gr = g.row(kept.row);
       const int* ix = ti + half * obj.k;
       const T* q = tq + half * obj.k;
-      for (long long i = threadIdx.x; i < obj.k; i += NT) {
+#pragma unroll 1
+      for (int i = threadIdx.x; i < (int)obj.k; i += NT) {
         const int l = ix[i];
         T sum = (T)0;
         bool leads = true;
-        for (long long o = 0; o < obj.k; ++o) {
+#pragma unroll 1
+        for (int o = 0; o < (int)obj.k; ++o) {
           if (ix[o] != l) continue;
           leads = leads && o >= i;
           sum += q[o];
         }
-        if (leads) gr[l] = kept.c * (Num<T>::exps(tx[half * obj.k + i] - kept.m, k) * kept.inv - sum);
+        if (leads) gr[l] = Num<T>::exps(tx[half * obj.k + i] - kept.m, k) * kept.scale - kept.c * sum;
       }
     }
   };
 
-  // Row r's operands are read a turn before they are used.
-  typename Obj::Meta meta[STAGES + 1];
-  T target = (T)0;
+  // Row r's operands are read a turn before they are used: the weights by everyone, the rest by the first
+  // warp, whose lanes hold one value each.
+  T weight[STAGES + 1], fields = (T)0, target = (T)0;
+  int label = 0;
 #pragma unroll
-  for (int a = 0; a <= STAGES; ++a) {
-    meta[a] = typename Obj::Meta{};
-    if (first + a * step < rows) meta[a] = obj.meta(first + a * step);
-  }
+  for (int a = 0; a <= STAGES; ++a) weight[a] = first + a * step < rows ? obj.weight[first + a * step] : (T)0;
 #pragma unroll
   for (int a = 0; a < STAGES; ++a) {
-    const long long r = first + a * step;
-    if (r < rows && meta[a].live) fetch(r, a);
+    if (weight[a] != (T)0) fetch(first + a * step, a);
     copies_done_group();
   }
   if constexpr (!Obj::TARGETS)
-    if (first < rows && meta[0].live) target = x.row(first)[clamp_label(meta[0].label, x.v)];
+    if (warp == 0 && weight[0] != (T)0) {
+      label = obj.labels[first];
+      fields = obj.field(first, lane);
+      target = x.row(first)[clamp_label(label, x.v)];
+    }
   int stage = 0, half = 0;
   for (long long r = first; r < rows; r += step) {
-    const typename Obj::Meta now = meta[0];
-    const T xl = target;
+    const bool live = weight[0] != (T)0;
+    const T now_weight = weight[0], now_fields = fields, xl = target;
+    const int now_label = label;
 #pragma unroll
-    for (int a = 0; a < STAGES; ++a) meta[a] = meta[a + 1];
-    meta[STAGES] = typename Obj::Meta{};
-    if (r + (STAGES + 1) * step < rows) meta[STAGES] = obj.meta(r + (STAGES + 1) * step);
-    if constexpr (!Obj::TARGETS)
-      if (r + step < rows && meta[0].live) target = x.row(r + step)[clamp_label(meta[0].label, x.v)];
-    typename std::conditional<Obj::TARGETS, typename DistillRow<T>::Part, int>::type part{};
-    if (now.live) {
-      if constexpr (Obj::TARGETS) {
-        // The last warp of the cluster's first block: the row's entries (before any of its gradient is
-        // written, which may be in the logits' place).
-        if (rank == 0 && warp == NW - 1) {
-          part = obj.prepare(r, x.row(r), x.v, lane, ti + half * obj.k, tq + half * obj.k, tx + half * obj.k);
-          const Pair<T> some{part.some ? (T)1 : (T)0, (T)0};
-          if constexpr (CLUSTER) {
-            if (lane < (int)blocks) put_remote(&table.extra[half], (unsigned)lane, some);
-          } else {
-            if (lane == 0) table.extra[half] = some;
-          }
+    for (int a = 0; a < STAGES; ++a) weight[a] = weight[a + 1];
+    weight[STAGES] = r + (STAGES + 1) * step < rows ? obj.weight[r + (STAGES + 1) * step] : (T)0;
+    if constexpr (Obj::TARGETS) {
+      // The first warp of the cluster's first block: the row's entries (before any of its gradient is
+      // written, which may be in the logits' place).
+      if (live && rank == 0 && warp == 0) {
+        entries_of<T, Obj>(obj, r, x.row(r), x.v, ti + half * obj.k, tq + half * obj.k, tx + half * obj.k, &part);
+        __syncwarp();
+        const Pair<T> some{part.some ? (T)1 : (T)0, (T)0};
+        if constexpr (CLUSTER) {
+          if (lane < (int)blocks) put_remote(&table.extra[half], (unsigned)lane, some);
+        } else {
+          if (lane == 0) table.extra[half] = some;
         }
       }
+    } else if (warp == 0 && weight[0] != (T)0) {
+      label = obj.labels[r + step];
+      fields = obj.field(r + step, lane);
     }
-    Span<T> row(x.row(r), x.v);
-    row.clip(begin, begin + slice);
-    const Store<T, 32> out(g.row(r), row);
+    const Place row = place(r);
+    const bool fast = inside(row);
     T y[E * VEC];
+    Stat<T> own;
     copies_wait<STAGES - 1>();
+    __syncwarp();
+    if (live) {
+      const Vec* from = ring + stage * PIECE + lane;
+      if (row.shift == 0) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = at0 + NT * e;
-      if (now.live && row.whole(i)) {
-        const Vec t = ring[(stage * E + e) * NT + threadIdx.x];
-        memcpy(y + e * VEC, &t, 16);
+        for (int e = 0; e < E; ++e)
+          if (e < turns) {
+            const Vec t = from[32 * e];
+            memcpy(y + e * VEC, &t, 16);
+          }
       } else {
-        const T* from = (const T*)&ring[(stage * E + e) * NT + threadIdx.x];
+        const T* el = (const T*)from + row.shift;
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) y[e * VEC + c] = now.live && row.has(i, c) ? from[c] : neg_inf<T>();
+        for (int e = 0; e < E; ++e)
+          if (e < turns) {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) y[e * VEC + c] = el[32 * VEC * e + c];
+          }
       }
+      if (!fast) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (e < turns) {
+            const int u = (warp0 + lane + 32 * e) * VEC;
+            if (u < row.lo || u + VEC > row.hi) {
+#pragma unroll
+              for (int c = 0; c < VEC; ++c)
+                if (u + c < row.lo || u + c >= row.hi) y[e * VEC + c] = neg_inf<T>();
+            }
+          }
+      }
+      own = exponentials<T, E, VEC>(y, k, turns);
     }
-    Stat<T> own, st;
-    if (now.live) own = exponentials<T, E * VEC>(y, k);
     // All that was copied has been used: the next row into its place.
-    if (r + STAGES * step < rows && meta[STAGES - 1].live) fetch(r + STAGES * step, stage);
+    __syncwarp();
+    if (weight[STAGES - 1] != (T)0) fetch(r + STAGES * step, stage);
     copies_done_group();
     stage = stage + 1 == STAGES ? 0 : stage + 1;
-    if (!now.live) {
+    if constexpr (!Obj::TARGETS)
+      if (warp == 0 && weight[0] != (T)0) target = x.row(r + step)[clamp_label(label, x.v)];
+    if (!live) {
       if (rank == 0 && threadIdx.x == 0) obj.skip(r);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) y[e * VEC + c] = (T)0;
-      }
+      for (int q = 0; q < E * VEC; ++q) y[q] = (T)0;
     } else {
       table.write(half, join<32>(own, k), rank, blocks);
       if constexpr (CLUSTER) cluster_sync();
       else __syncthreads();
-      finish(half ^ 1);  // of the row before
-      st = table.read(half, blocks, k);
-      T c, f;
-      int l = -1;
-      if constexpr (Obj::TARGETS) {
-        const bool some = table.extra[half].m != (T)0;
-        c = now.w * obj.wt;
-        f = share(own.m, st, k, c);
-        if (!some) {  // a row without entries counts nothing
-#pragma unroll
-          for (int q = 0; q < E * VEC; ++q) y[q] = (T)0;
-          f = (T)0;
+      Stat<T> st;
+      if (warp == 0) {
+        st = table.read(half, blocks, k);
+        Scalars<T> s;
+        s.m = st.m;
+        if constexpr (Obj::TARGETS) {
+          // A row without entries counts nothing.
+          s.at = table.extra[half].m != (T)0;
+          s.c = now_weight * obj.wt;
+          s.scale = s.c / st.s;
+        } else {
+          s.at = (int)clamp_label(now_label, x.v);
+          s.c = coef_of<T, Obj>(obj, now_label, now_fields, xl, st);
+          s.scale = -s.c / st.s;
         }
-        kept.row = some ? r : -1;
-        kept.c = c;
-        kept.inv = (T)1 / st.s;
-        kept.m = st.m;
-      } else {
-        c = obj.coef(now, xl, st);
-        f = share(own.m, st, k, -c);
-        l = (int)clamp_label(now.label, x.v) + row.off;
+        if (lane == 0) scalars = s;
       }
+      finish(half ^ 1);  // of the row before
+      __syncthreads();
+      const Scalars<T> s = scalars;
+      const T fs = own.m == neg_inf<T>() ? (T)0 * s.scale : Num<T>::exps(own.m - base(s.m), k) * s.scale;
+      if constexpr (Obj::TARGETS) {
+        kept.row = s.at ? r : -1;
+        kept.c = s.c;
+        kept.scale = s.scale;
+        kept.m = s.m;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
+        for (int q = 0; q < E * VEC; ++q) y[q] = s.at ? y[q] * fs : (T)0;
+        if (rank == 0 && warp == 0) report_entries<T, Obj>(obj, r, part, st);
+      } else {
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) y[e * VEC + q] *= f;
-        if constexpr (!Obj::TARGETS)
-          if (at0 + NT * e == l / VEC) {
+        for (int q = 0; q < E * VEC; ++q) y[q] *= fs;
+        const int l = s.at + row.off - warp0 * VEC;  // within the warp's vectors
+        if (l >= 0 && l < 32 * turns * VEC && (l / VEC) % 32 == lane) {
 #pragma unroll
-            for (int q = 0; q < VEC; ++q)
-              if (l % VEC == q) y[e * VEC + q] += c;
-          }
+          for (int q = 0; q < E * VEC; ++q)
+            if (q == l / (32 * VEC) * VEC + l % VEC) y[q] += s.c;
+        }
+        if (rank == 0 && warp == 0) report_of<T, Obj>(obj, r, now_label, now_fields, xl, st);
       }
       half ^= 1;
     }
+    T* to = row.to + (long long)(warp0 + lane) * VEC;
 #pragma unroll
-    for (int e = 0; e < E; ++e) out.put(row, at0 + NT * e, lane, y + e * VEC);
-    if (now.live) {
-      if constexpr (Obj::TARGETS) {
-        if (rank == 0 && warp == NW - 1 && lane == 0) obj.report(r, now, part, st);
-      } else {
-        if (rank == 0 && threadIdx.x == NT - 1) obj.report(r, now, xl, st);
+    for (int e = 0; e < E; ++e)
+      if (e < turns) {
+        const int u = (warp0 + lane + 32 * e) * VEC;
+        if (fast || (u >= row.lo && u + VEC <= row.hi)) {
+          Vec t;
+          memcpy(&t, y + e * VEC, 16);
+          *reinterpret_cast<Vec*>(to + 32 * VEC * e) = t;
+        } else {
+#pragma unroll
+          for (int c = 0; c < VEC; ++c)
+            if (u + c >= row.lo && u + c < row.hi) to[32 * VEC * e + c] = y[e * VEC + c];
+        }
       }
-    }
   }
   if constexpr (Obj::TARGETS) {
     if constexpr (CLUSTER) cluster_sync();
@@ -816,14 +985,14 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
   for (; r < rows; r += step) {
     const typename Obj::Meta now = next;
     if (r + step < rows) next = obj.meta(r + step);
-    if (!now.live) {
+    if (!now.live()) {
       if (rank == 0 && threadIdx.x == 0) obj.skip(r);
       continue;
     }
     Span<T> row(x.row(r), x.v);
     row.clip(begin, begin + slice);
     T xl = (T)0;
-    typename std::conditional<Obj::TARGETS, typename DistillRow<T>::Part, int>::type part{};
+    typename std::conditional<Obj::TARGETS, EntriesPart, int>::type part{};
     if constexpr (Obj::TARGETS) {
       if (reports) part = obj.prepare(r, x.row(r), x.v, lane, nullptr, nullptr, nullptr);
     } else {
@@ -863,32 +1032,44 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_grad(View<T> x, long long rows
   constexpr int VEC = Num<T>::VEC, NT = GRAD_THREADS;
   pdl_wait();
   const int lane = threadIdx.x % 32;
-  for (long long w = blockIdx.x; w < rows * pieces; w += gridDim.x) {
-    const long long r = w / pieces;
-    const int first = (int)(w % pieces) * NT * U;
+  // Piece p of row r; then gridDim.x pieces on.
+  const long long step_r = gridDim.x / (unsigned)pieces;
+  const int step_p = (int)(gridDim.x % (unsigned)pieces);
+  long long r = blockIdx.x / (unsigned)pieces;
+  for (int p = (int)(blockIdx.x % (unsigned)pieces); r < rows; r += step_r + (p + step_p >= pieces), p = p + step_p >= pieces ? p + step_p - pieces : p + step_p) {
+    const int first = p * NT * U;
     const typename GivenRow<T>::Meta q = obj.meta(r);
     Span<T> row(x.row(r), x.v);
     row.clip(first, first + NT * U);
-    const Store<T, 32> out(g.row(r), row);
+    const int warp0 = first + (int)threadIdx.x / 32 * 32 * U;  // this warp's vectors: warp0 + lane + 32 * u
     T y[U * VEC];
-    if (q.live) {
+    const bool inside = warp0 * VEC >= row.lo && (warp0 + 32 * U) * VEC <= row.hi;
+    if (q.live()) {
+      const T* from = row.base + (long long)(warp0 + lane) * VEC;
 #pragma unroll
-      for (int u = 0; u < U; ++u) row.load(first + (int)threadIdx.x + NT * u, y + u * VEC);
+      for (int u = 0; u < U; ++u) {
+        if (inside) {
+          const typename Num<T>::Vec t = *reinterpret_cast<const typename Num<T>::Vec*>(from + u * 32 * VEC);
+          memcpy(y + u * VEC, &t, 16);
+        } else {
+          row.load(warp0 + lane + 32 * u, y + u * VEC);
+        }
+      }
     }
     const T f = -q.c / q.s;
     const int l = (int)clamp_label(q.label, x.v) + row.off;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = first + (int)threadIdx.x + NT * u;
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) y[u * VEC + c] = q.live ? Num<T>::exps(y[u * VEC + c] - q.m, k) * f : (T)0;
-      if (q.live && i == l / VEC) {
+      for (int c = 0; c < VEC; ++c) y[u * VEC + c] = q.live() ? Num<T>::exps(y[u * VEC + c] - q.m, k) * f : (T)0;
+      if (q.live() && warp0 + lane + 32 * u == l / VEC) {
 #pragma unroll
         for (int c = 0; c < VEC; ++c)
           if (l % VEC == c) y[u * VEC + c] += q.c;
       }
-      out.put(row, i, lane, y + u * VEC);
     }
+    if (inside) store<T, 32, U, true>(g.row(r), row, warp0, lane, y);
+    else store<T, 32, U, false>(g.row(r), row, warp0, lane, y);
   }
 }
 
@@ -911,15 +1092,14 @@ template <typename T, class Obj> __global__ void __launch_bounds__(LONG_THREADS)
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const typename Obj::Meta now = obj.meta(r);
     const Span<T> row(x.row(r), x.v);
-    const Store<T, 32> out(g.row(r), row);
-    // A multiple of 32 vectors more, so that whole warps take each turn.
+    // Whole warps take each turn.
     const int vectors = (row.hi + VEC - 1) / VEC, turns = (vectors + NT - 1) / NT;
     T xl = (T)0, c = (T)0, f = (T)0;
     int l = -1;
     Stat<T> a, st;
-    typename std::conditional<Obj::TARGETS, typename DistillRow<T>::Part, int>::type part{};
-    bool zero = !now.live;
-    if (now.live) {
+    typename std::conditional<Obj::TARGETS, EntriesPart, int>::type part{};
+    bool zero = !now.live();
+    if (now.live()) {
       if constexpr (Obj::TARGETS) {
         if (warp == 0) {
           part = obj.prepare(r, x.row(r), x.v, lane, ti, tq, tx);
@@ -960,7 +1140,7 @@ template <typename T, class Obj> __global__ void __launch_bounds__(LONG_THREADS)
         y[q] = zero ? (T)0 : Num<T>::exps(y[q] - st.m, k) * f;
         if (!zero && i * VEC + q == l) y[q] += c;
       }
-      out.put(row, i, lane, y);
+      store<T, 32, 1, false>(g.row(r), row, i - lane, lane, y);
     }
     __syncthreads();
     if constexpr (Obj::TARGETS) {
@@ -978,12 +1158,12 @@ template <typename T, class Obj> __global__ void __launch_bounds__(LONG_THREADS)
         }
       }
       if (warp == 0 && lane == 0) {
-        if (now.live) obj.report(r, now, part, st);
+        if (now.live()) obj.report(r, now, part, st);
         else obj.skip(r);
       }
       __syncthreads();
     } else if (threadIdx.x == 0) {
-      if (now.live) obj.report(r, now, xl, st);
+      if (now.live()) obj.report(r, now, xl, st);
       else obj.skip(r);
     }
   }
@@ -1045,15 +1225,16 @@ __global__ void __launch_bounds__(PAIR_THREADS) k_pairs(const T* __restrict__ to
 
 // ---- host side ----
 
-template <typename T> View<T> view(const RowView& x) { return {(const T*)x.data, std::max<long long>(x.inner, 1), x.vocab, x.so, x.si}; }
-template <typename T> Out<T> out(const RowView& x, const RowOut& g) { return {(T*)g.data, std::max<long long>(x.inner, 1), g.so, g.si}; }
+template <typename T> View<T> view(const RowView& x) { return {(const T*)x.data, make_fdiv((unsigned long long)std::max<long long>(x.inner, 1)), x.vocab, x.so, x.si}; }
+template <typename T> Out<T> out(const RowView& x, const RowOut& g) { return {(T*)g.data, make_fdiv((unsigned long long)std::max<long long>(x.inner, 1)), g.so, g.si}; }
 
 // Vectors of the longest row, from the alignments that rows have.
-template <typename T> long long most_vectors(const RowView& x) {
+template <typename T> long long most_vectors(const RowView& x, const void* data, long long so, long long si) {
   constexpr long long VEC = Num<T>::VEC;
-  const bool aligned = (uintptr_t)x.data % 16 == 0 && (x.outer <= 1 || x.so % VEC == 0) && (x.inner <= 1 || x.si % VEC == 0);
+  const bool aligned = (uintptr_t)data % 16 == 0 && (x.outer <= 1 || so % VEC == 0) && (x.inner <= 1 || si % VEC == 0);
   return (x.vocab + (aligned ? 0 : VEC - 1) + VEC - 1) / VEC;
 }
+template <typename T> long long most_vectors(const RowView& x) { return most_vectors<T>(x, x.data, x.so, x.si); }
 
 int sm_count() {
   static int n = [] {
@@ -1150,15 +1331,16 @@ template <class Obj> size_t target_bytes(const Obj& obj, size_t es, int halves) 
 template <typename T, int NT, int E, int STAGES, bool CLUSTER, class Obj>
 cudaError_t go_block(const RowView& x, const Obj& obj, T k, const RowOut& g, long long slice, unsigned cluster, cudaStream_t s) {
   auto* kernel = k_block<T, NT, E, STAGES, CLUSTER, Obj>;
-  const size_t smem = (size_t)STAGES * E * NT * 16 + target_bytes(obj, sizeof(T), 2);
+  const size_t smem = (size_t)STAGES * (NT / 32) * (32 * E + 1) * 16 + target_bytes(obj, sizeof(T), 2);
   const long long clusters = std::min(x.rows(), resident(kernel, NT, smem, cluster));
-  return launch(kernel, dim3((unsigned)(clusters * cluster)), dim3(NT), smem, cluster, s, view<T>(x), x.rows(), obj, k, out<T>(x, g), (int)slice);
+  return launch(kernel, dim3((unsigned)(clusters * cluster)), dim3(NT), smem, cluster, s, view<T>(x), x.rows(), obj, k, out<T>(x, g), (int)slice,
+                (int)pieces_of(slice, NT));
 }
 
 // Rows with a gradient that no group holds.
 constexpr long long BLOCK_VECTORS = 4096;
 template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& obj, T k, const RowOut& g, cudaStream_t s) {
-  const long long v = most_vectors<T>(x);
+  const long long v = most_vectors<T>(x, g.data, g.so, g.si);
   const unsigned c = split(x.rows(), v, BLOCK_VECTORS, 512);
   const long long slice = pieces_of(pieces_of(v, c), 32) * 32;
   if (slice > BLOCK_VECTORS) {
@@ -1168,14 +1350,14 @@ template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& 
                   obj, k, out<T>(x, g));
   }
   if (c == 1) {
-    if (slice <= 512) return go_block<T, 128, 4, 3, false>(x, obj, k, g, slice, 1, s);
-    if (slice <= 1024) return go_block<T, 128, 8, 1, false>(x, obj, k, g, slice, 1, s);
-    if (slice <= 2048) return go_block<T, 256, 8, 1, false>(x, obj, k, g, slice, 1, s);
-    return go_block<T, 512, 8, 1, false>(x, obj, k, g, slice, 1, s);
+    if (slice <= 512) return go_block<T, 64, 8, 2, false>(x, obj, k, g, slice, 1, s);
+    if (slice <= 1024) return go_block<T, 64, 16, 1, false>(x, obj, k, g, slice, 1, s);
+    if (slice <= 2048) return go_block<T, 128, 16, 1, false>(x, obj, k, g, slice, 1, s);
+    return go_block<T, 256, 16, 1, false>(x, obj, k, g, slice, 1, s);
   }
-  if (slice <= 1024) return go_block<T, 128, 8, 1, true>(x, obj, k, g, slice, c, s);
-  if (slice <= 2048) return go_block<T, 256, 8, 1, true>(x, obj, k, g, slice, c, s);
-  return go_block<T, 512, 8, 1, true>(x, obj, k, g, slice, c, s);
+  if (slice <= 1024) return go_block<T, 64, 16, 1, true>(x, obj, k, g, slice, c, s);
+  if (slice <= 2048) return go_block<T, 128, 16, 1, true>(x, obj, k, g, slice, c, s);
+  return go_block<T, 256, 16, 1, true>(x, obj, k, g, slice, c, s);
 }
 
 template <typename T, class Obj> cudaError_t stream(const RowView& x, const Obj& obj, T k, cudaStream_t s) {
@@ -1228,7 +1410,7 @@ template <typename T> cudaError_t Objectives<T>::log_prob(const RowView& x, cons
 
 template <typename T>
 cudaError_t Objectives<T>::log_prob_grad(const RowView& x, const int32_t* labels, const void* stats, const void* dlogp, const RowOut& grad, cudaStream_t s) {
-  return given_grad<T>(x, GivenRow<T>{labels, (const T*)stats, (const T*)dlogp, nullptr, nullptr, 1}, grad, s);
+  return given_grad<T>(x, GivenRow<T>{labels, (const T*)stats, (const T*)dlogp, nullptr, nullptr, FDiv{}}, grad, s);
 }
 
 template <typename T>
@@ -1262,7 +1444,7 @@ cudaError_t Objectives<T>::preference(const RowView& x, const int32_t* labels, c
                a.beta, a.smoothing, terms, coef, (T*)margins, (T*)logp);
   if (e == cudaSuccess && loss) e = sum_terms<T>(terms, pairs, loss, pairs ? 1.0 / (double)pairs : 0.0, s);
   if (e == cudaSuccess && g.data)
-    e = given_grad<T>(x, GivenRow<T>{labels, stats, nullptr, coef, (const T*)a.weight, std::max<long long>(x.inner, 1)}, g, s);
+    e = given_grad<T>(x, GivenRow<T>{labels, stats, nullptr, coef, (const T*)a.weight, make_fdiv((unsigned long long)std::max<long long>(x.inner, 1))}, g, s);
   return e;
 }
 

@@ -7,7 +7,7 @@ namespace rg {
 namespace {
 
 constexpr size_t MAX_TEACHER = 1024;  // teacher entries per row the device's kernel holds
-constexpr size_t MAX_VOCAB = size_t(1) << 30;
+constexpr size_t MAX_VOCAB = size_t(1) << 30, MAX_ROWS = 0x7fffffff;
 
 bool attrs_ok(const Op& op, size_t n) {
   if (!op.value || op.value->n() != n) return false;
@@ -40,6 +40,7 @@ bool objective_of(const Op& op, const std::vector<std::vector<size_t>>& s, const
   const std::vector<size_t> lead(s[0].begin(), s[0].end() - 1);
   o.vocab = s[0].back();
   o.rows = o.outer = product(lead);
+  if (o.rows > MAX_ROWS) return no("too_many_rows");
   o.inner = 1;
   auto with = [&](size_t n) {
     auto v = lead;
