@@ -29,6 +29,10 @@ def _native():
     return _rg
 
 
+# The current stream's handle without building a Stream object, where torch has the call.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _rows(x, out=None):
     """The leading axes of `x` as (outer, inner, outer stride, inner stride), and the same strides of `out`:
     axes that chain in both are one."""
@@ -59,54 +63,60 @@ class _Call:
     """The logits of a call, where their gradient goes, and the stream it runs on. `sequences`: the leading
     axes are (sequences, positions) as they are."""
 
+    __slots__ = ("logits", "index", "dtype", "lead", "grad", "args", "grad_args")
+
     def __init__(self, logits, grad=False, out=None, sequences=False):
         if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
             raise TypeError("logits must be a CUDA tensor")
-        dtype = _DTYPES.get(logits.dtype)
+        self.dtype = logits.dtype
+        dtype = _DTYPES.get(self.dtype)
         if dtype is None:
             raise TypeError(f"logits must be float32 or float64, not {logits.dtype}")
-        if sequences and logits.dim() != 3:
+        shape = logits.shape
+        if sequences and len(shape) != 3:
             raise ValueError("logits must be (sequences, positions, vocabulary)")
-        self.logits, self.device, self.lead, self.dtype = logits, logits.device, logits.shape[:-1], dtype
-        if out is None:
-            self.grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
-        elif not grad:
-            raise ValueError("out is given but no gradient is asked for")
-        elif not isinstance(out, torch.Tensor) or out.device != logits.device or out.dtype != logits.dtype or out.shape != logits.shape:
-            raise ValueError("out must have the logits' shape, dtype and device")
-        else:
-            self.grad = out
+        self.logits, self.index, self.lead = logits, logits.get_device(), shape[:-1]
+        if out is not None:
+            if not grad:
+                raise ValueError("out is given but no gradient is asked for")
+            if not isinstance(out, torch.Tensor) or out.get_device() != self.index or out.dtype != self.dtype or out.shape != shape:
+                raise ValueError("out must have the logits' shape, dtype and device")
+        elif len(shape) and logits.is_contiguous() and shape[-1]:
+            # The usual case, in as few steps as there are.
+            v = shape[-1]
+            outer, inner = (shape[0], shape[1]) if sequences else (logits.numel() // v, 1)
+            self.grad = torch.empty_like(logits, memory_format=torch.contiguous_format) if grad else None
+            self.args = (logits.data_ptr(), outer, inner, v, inner * v, v, dtype)
+            self.grad_args = (self.grad.data_ptr(), inner * v, v) if grad else (0, 0, 0)
+            return
+        self.grad = out if out is not None else logits.new_empty(shape) if grad else None
         if sequences:
             strides = [logits.stride()] if self.grad is None else [logits.stride(), self.grad.stride()]
-            if any(s[2] != 1 for s in strides) and logits.shape[2] != 1:
+            if any(s[2] != 1 for s in strides) and shape[2] != 1:
                 raise ValueError("the last axis of the logits and of out must be contiguous")
-            outer, inner = logits.shape[:2]
+            outer, inner = shape[:2]
             so, si = [s[0] for s in strides], [s[1] for s in strides]
         else:
             outer, inner, so, si = _rows(logits, self.grad)
-        self.args = (logits.data_ptr(), outer, inner, logits.shape[-1], so[0], si[0], dtype)
+        self.args = (logits.data_ptr(), outer, inner, shape[-1], so[0], si[0], dtype)
         self.grad_args = (0, 0, 0) if self.grad is None else (self.grad.data_ptr(), so[1], si[1])
 
     def per_row(self, t, what, shape=None, dtype=None):
         """A contiguous operand on the logits' device."""
-        if not isinstance(t, torch.Tensor) or t.device != self.device:
-            raise TypeError(f"{what} must be a tensor on {self.device}")
-        want = self.logits.dtype if dtype is None else dtype
-        if t.dtype != want:
-            raise TypeError(f"{what} must be {want}, not {t.dtype}")
+        if not isinstance(t, torch.Tensor) or t.get_device() != self.index:
+            raise TypeError(f"{what} must be a tensor on the logits' device")
+        if t.dtype != (dtype or self.dtype):
+            raise TypeError(f"{what} must be {dtype or self.dtype}, not {t.dtype}")
         if t.shape != (self.lead if shape is None else shape):
             raise ValueError(f"{what} has shape {tuple(t.shape)}, not {tuple(self.lead if shape is None else shape)}")
         return t if t.is_contiguous() else t.contiguous()
 
-    def new(self, *shape):
-        return torch.empty(shape, dtype=self.logits.dtype, device=self.device)
-
     def run(self, call, *args):
-        if self.device.index == torch.cuda.current_device():
-            call(*args, torch.cuda.current_stream(self.device).cuda_stream)
+        if self.index == torch.cuda.current_device():
+            call(self.args, *args, _stream(self.index))
         else:
-            with torch.cuda.device(self.device):
-                call(*args, torch.cuda.current_stream(self.device).cuda_stream)
+            with torch.cuda.device(self.index):
+                call(self.args, *args, _stream(self.index))
 
 
 def token_log_prob(logits, labels, *, stats=False):
@@ -114,9 +124,9 @@ def token_log_prob(logits, labels, *, stats=False):
     exp(logits - maximum)) that `token_log_prob_grad` takes."""
     c = _Call(logits)
     labels = c.per_row(labels, "labels", dtype=torch.int32)
-    logp = c.new(*c.lead)
-    st = c.new(*c.lead, 2) if stats else None
-    c.run(_native().token_log_prob, c.args, labels.data_ptr(), logp.data_ptr(), st.data_ptr() if stats else 0)
+    logp = logits.new_empty(c.lead)
+    st = logits.new_empty((*c.lead, 2)) if stats else None
+    c.run(_native().token_log_prob, labels.data_ptr(), logp.data_ptr(), st.data_ptr() if stats else 0)
     return (logp, st) if stats else logp
 
 
@@ -126,7 +136,7 @@ def token_log_prob_grad(logits, labels, stats, dlogp, *, out=None):
     labels = c.per_row(labels, "labels", dtype=torch.int32)
     stats = c.per_row(stats, "stats", shape=(*c.lead, 2))
     dlogp = c.per_row(dlogp, "dlogp")
-    c.run(_native().token_log_prob_grad, c.args, labels.data_ptr(), stats.data_ptr(), dlogp.data_ptr(), c.grad_args)
+    c.run(_native().token_log_prob_grad, labels.data_ptr(), stats.data_ptr(), dlogp.data_ptr(), c.grad_args)
     return c.grad
 
 
@@ -149,8 +159,8 @@ def policy_loss(logits, labels, old_logp, advantages, weights, *, ref_logp=None,
     adv = c.per_row(advantages, "advantages")
     w = c.per_row(weights, "weights")
     ref = c.per_row(ref_logp, "ref_logp") if ref_logp is not None else None
-    loss, terms, logp = c.new(), c.new(*c.lead), c.new(*c.lead)
-    c.run(_native().policy_loss, c.args, labels.data_ptr(), old.data_ptr(), adv.data_ptr(), w.data_ptr(), 0 if ref is None else ref.data_ptr(),
+    loss, terms, logp = logits.new_empty(()), torch.empty_like(w), torch.empty_like(w)
+    c.run(_native().policy_loss, labels.data_ptr(), old.data_ptr(), adv.data_ptr(), w.data_ptr(), 0 if ref is None else ref.data_ptr(),
           clip_low, clip_high, kl, loss.data_ptr(), terms.data_ptr(), logp.data_ptr(), c.grad_args)
     return PolicyLoss(loss, terms, logp, c.grad)
 
@@ -174,10 +184,10 @@ def preference_loss(logits, labels, weights, ref_logp, *, beta=0.1, smoothing=0.
     labels = c.per_row(labels, "labels", dtype=torch.int32)
     w = c.per_row(weights, "weights")
     ref = c.per_row(ref_logp, "ref_logp", shape=(n,))
-    nbytes = _native().preference_workspace(n, t, c.dtype)
-    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=c.device)
-    loss, margins, logp = c.new(), c.new(n // 2), c.new(n)
-    c.run(_native().preference_loss, c.args, labels.data_ptr(), w.data_ptr(), ref.data_ptr(), beta, smoothing, loss.data_ptr(), margins.data_ptr(),
+    nbytes = _native().preference_workspace(n, t, _DTYPES[c.dtype])
+    workspace = logits.new_empty((nbytes,), dtype=torch.uint8)
+    loss, margins, logp = logits.new_empty(()), logits.new_empty((n // 2,)), torch.empty_like(ref)
+    c.run(_native().preference_loss, labels.data_ptr(), w.data_ptr(), ref.data_ptr(), beta, smoothing, loss.data_ptr(), margins.data_ptr(),
           logp.data_ptr(), c.grad_args, workspace.data_ptr(), nbytes)
     return PreferenceLoss(loss, margins, logp, c.grad)
 
@@ -200,6 +210,6 @@ def distillation_loss(logits, index, teacher, weights, *, temperature=1.0, grad=
     index = c.per_row(index, "index", shape=(*c.lead, k), dtype=torch.int32)
     teacher = c.per_row(teacher, "teacher", shape=(*c.lead, k))
     w = c.per_row(weights, "weights")
-    loss, terms = c.new(), c.new(*c.lead)
-    c.run(_native().distillation_loss, c.args, index.data_ptr(), teacher.data_ptr(), w.data_ptr(), k, temperature, loss.data_ptr(), terms.data_ptr(), c.grad_args)
+    loss, terms = logits.new_empty(()), torch.empty_like(w)
+    c.run(_native().distillation_loss, index.data_ptr(), teacher.data_ptr(), w.data_ptr(), k, temperature, loss.data_ptr(), terms.data_ptr(), c.grad_args)
     return DistillationLoss(loss, terms, c.grad)

@@ -426,3 +426,26 @@ def test_compiled_checks_and_training(oracle):
         again = F.run(c, state, batch, steps=5)
         assert r.history == again.history
         state = r.state
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_parts_of_a_row_without_any_logit(dtype):
+    # Rows far below zero, with long stretches of -inf: whole lanes, warps and blocks hold nothing finite.
+    for v in (70, 900, 3001, 20000, 70001, 300007):
+        rng = np.random.default_rng(v)
+        x = np.full((4, v), -np.inf, dtype)
+        x[0, v // 2] = -5000.0                       # one logit: p = 1
+        x[1, v - v // 3:] = rng.normal(size=v // 3) - 1000.0
+        x[2, : v // 4] = rng.normal(size=v // 4) + 3000.0
+        x[3, ::max(1, v // 7)] = -30000.0            # equal ones, far apart
+        lab = R.labels(rng, x)
+        old, adv, w, ref = R.policy_inputs(rng, x, lab, dtype)
+        w = np.full(4, 0.25, dtype)
+        check(losses.policy_loss(*put(x, lab, old, adv, w), clip_high=0.28), R.policy(x, lab, old, adv, w, ref, 0.2, 0.28, 0.0, dtype, adds(v)),
+              ("loss", "terms", "logp", "grad"), f"sparse {v}")
+        logp, stats = losses.token_log_prob(*put(x, lab), stats=True)
+        grad = losses.token_log_prob_grad(*put(x, lab), stats, *put(adv))
+        check((logp, grad), R.token_log_prob(x, lab, adv, dtype, adds(v)), ("logp", "grad"), f"sparse {v}")
+        index, teacher = lab[:, None].copy(), np.zeros((4, 1), dtype)
+        d = losses.distillation_loss(*put(x, index, teacher, w))
+        check(d, R.distillation(x, index, teacher, w, 1.0, dtype, adds(v)), d._fields, f"sparse {v}")
