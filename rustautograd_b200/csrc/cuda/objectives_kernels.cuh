@@ -73,6 +73,8 @@ template <> struct Num<float> {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * k));
     return r;
   }
+  static __device__ __forceinline__ float ex(float v) { return expf(v); }
+  static __device__ __forceinline__ float ln(float v) { return logf(v); }
   static __device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }  // a NaN gives the other
   static float factor(double scale) { return (float)(scale * 1.4426950408889634074); }
 };
@@ -80,6 +82,8 @@ template <> struct Num<double> {
   static constexpr int VEC = 2;
   using Vec = double2;
   static __device__ __forceinline__ double exps(double d, double k) { return exp(d * k); }
+  static __device__ __forceinline__ double ex(double v) { return exp(v); }
+  static __device__ __forceinline__ double ln(double v) { return log(v); }
   static __device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
   static double factor(double scale) { return scale; }
 };
@@ -218,10 +222,11 @@ template <typename T, int G, int E, bool INSIDE> __device__ __forceinline__ void
   }
 }
 
-// The same for the groups of a warp, each with a row of its own (and an alignment of its own).
+// The same for the groups of a warp, each with a row of its own (and an alignment of its own); with many vectors a lane
+// the registers do not hold the shifted ones too.
 template <typename T, int G, int E> __device__ __forceinline__ void store_group(T* row, const Span<T>& x, int lane, const T* y) {
   constexpr int VEC = Num<T>::VEC;
-  if constexpr (G == 32) {
+  if constexpr (G == 32 && E <= 8) {
     store<T, G, E, false>(row, x, 0, lane, y);
   } else {
     const int goff = (int)(((unsigned long long)row / sizeof(T)) % VEC), sh = (x.off - goff + VEC) % VEC;
@@ -296,9 +301,9 @@ template <typename T> struct PolicyRow {
     if (logp) logp[r] = (T)0;
   }
   __device__ __forceinline__ T coef(const Meta& m, T xl, Stat<T> st) const {
-    const T lp = (xl - st.m) - ln(st.s), ratio = ex(lp - m.old);
+    const T lp = (xl - st.m) - Num<T>::ln(st.s), ratio = Num<T>::ex(lp - m.old);
     T c = (m.a >= (T)0 ? ratio <= high : ratio >= low) ? -(ratio * m.a) : (T)0;
-    if (kl != (T)0) c += kl * ((T)1 - ex(m.ref - lp));
+    if (kl != (T)0) c += kl * ((T)1 - Num<T>::ex(m.ref - lp));
     return m.w * c;
   }
   __device__ __forceinline__ void report(long long r, const Meta& m, T xl, Stat<T> st) const {
@@ -313,10 +318,6 @@ template <typename T> struct PolicyRow {
     terms[r] = (T)((double)m.w * term);
     if (logp) logp[r] = (T)lp;
   }
-  static __device__ __forceinline__ float ex(float v) { return expf(v); }
-  static __device__ __forceinline__ double ex(double v) { return exp(v); }
-  static __device__ __forceinline__ float ln(float v) { return logf(v); }
-  static __device__ __forceinline__ double ln(double v) { return log(v); }
 };
 
 // Coefficients that need more than the row: the statistics are those of an earlier pass. c = by_row[r], or
@@ -376,7 +377,7 @@ template <typename T> struct DistillRow {
   }
   __device__ void skip(long long r) const { terms[r] = (T)0; }
   __device__ __forceinline__ void report(long long r, const Meta& m, Part p, Stat<T> st) const {
-    const double lse = ((double)st.m - p.from) * inverse + log((double)st.s);
+    const double lse = ((double)st.m - p.from) * inverse + (double)Num<T>::ln(st.s);
     terms[r] = p.some ? (T)((double)m.w * (double)wt * (double)wt * (p.a + lse * p.q)) : (T)0;
   }
   // One warp; x: the row's logits. Keeps q, the index and its logit of each entry when `at` is given.
@@ -398,7 +399,7 @@ template <typename T> struct DistillRow {
     p.from = far > neg_inf<T>() && far < -neg_inf<T>() ? (double)far : 0.0;
     p.some = st.s != (T)0;  // all entries -inf: none
     const T inv = (T)1 / st.s;
-    const double logs = log((double)st.s);
+    const double logs = (double)Num<T>::ln(st.s);
     for (int i = lane; i < (int)k; i += 32) {
       const long long l = clamp_label(ix[i], v);
       const T d = t[i] - base(st.m), qi = p.some ? Num<T>::exps(d, tk) * inv : (T)0, xi = x[l];
@@ -473,21 +474,100 @@ template <typename T> __device__ __forceinline__ T share(T m, Stat<T> st, T k, T
   return (m == neg_inf<T>() ? (T)0 : Num<T>::exps(m - base(st.m), k)) * (scale / st.s);
 }
 
-template <typename T, int G, int E, class Obj, bool GRAD>
-__global__ void __launch_bounds__(GROUP_THREADS) k_group(View<T> x, long long rows, Obj obj, T k, Out<T> g) {
-  constexpr int VEC = Num<T>::VEC, PER_WARP = 32 / G;
+// A warp computes B times 32 / G rows together (G lanes each, E vectors a lane): all loads first, then the sums, then what
+// the rows need once, a lane per row, then the gradients. The label's element is stored a second time by
+// its row's lane, so no lane looks for it.
+// What a row needs once is some 400 instructions: with a lane of every group doing it per row, 131072 x 96 took 62 us.
+template <typename T, int G, int E, int B, class Obj, bool GRAD>
+__global__ void __launch_bounds__(GROUP_THREADS, 2) k_group(const View<T> x, const long long rows, const Obj obj, const T k, const Out<T> g) {
+  constexpr int VEC = Num<T>::VEC, R = 32 / G, ROWS = B * R;
+  static_assert(ROWS <= 32, "a lane per row");
+  pdl_wait();
+  const int lane = threadIdx.x % 32, in_group = lane % G, group = lane / G;
+  const long long warps = (long long)gridDim.x * (GROUP_THREADS / 32);
+  for (long long w = (long long)blockIdx.x * (GROUP_THREADS / 32) + threadIdx.x / 32; w * ROWS < rows; w += warps) {
+    const long long row0 = w * ROWS, mine = row0 + lane;
+    const bool in = lane < ROWS && mine < rows;
+    typename Obj::Meta meta{};
+    if (in) meta = obj.meta(mine);
+    const bool live = in && meta.live();
+    const unsigned lives = __ballot_sync(~0u, live);
+    const T xl = live ? x.row(mine)[clamp_label(meta.label, x.v)] : (T)0;
+    T y[B][E * VEC], most[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int at = b * R + group;
+      if (lives >> at & 1) {
+        const Span<T> row(x.row(row0 + at), x.v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) row.load(in_group + G * e, y[b] + e * VEC);
+      } else {
+#pragma unroll
+        for (int q = 0; q < E * VEC; ++q) y[b][q] = neg_inf<T>();
+      }
+    }
+    Stat<T> st;
+    if constexpr (Obj::GIVEN) {
+      st = {meta.m, meta.s};
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const T m = __shfl_sync(~0u, st.m, (b * R + group) % 32);
+#pragma unroll
+        for (int q = 0; q < E * VEC; ++q) y[b][q] = Num<T>::exps(y[b][q] - m, k);
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const Stat<T> own = exponentials<T, E * VEC>(y[b], k);
+        most[b] = own.m;
+        const Stat<T> all = join<G>(own, k);
+        const T m = __shfl_sync(~0u, all.m, lane % R * G), s = __shfl_sync(~0u, all.s, lane % R * G);
+        if (lane / R == b) st = {m, s};
+      }
+    }
+    T c = (T)0, scale = (T)0;
+    if (live) {
+      c = obj.coef(meta, xl, st);
+      scale = -c / st.s;
+    }
+    if constexpr (GRAD) {
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const int at = (b * R + group) % 32;
+        const T sc = __shfl_sync(~0u, scale, at);
+        T f = sc;
+        if constexpr (!Obj::GIVEN) {
+          const T m = __shfl_sync(~0u, st.m, at);
+          f = most[b] == neg_inf<T>() ? (T)0 * sc : Num<T>::exps(most[b] - base(m), k) * sc;
+        }
+        const bool zero = !(lives >> at & 1), have = row0 + b * R + group < rows;
+#pragma unroll
+        for (int q = 0; q < E * VEC; ++q) y[b][q] = zero ? (T)0 : y[b][q] * f;
+        const long long r = have ? row0 + b * R + group : row0;
+        store_group<T, G, E>(g.row(r), Span<T>(x.row(r), have ? x.v : 0), in_group, y[b]);
+      }
+      __syncwarp();  // the label's element over what its group has stored
+      if (live) g.row(mine)[clamp_label(meta.label, x.v)] = c + Num<T>::exps(xl - st.m, k) * scale;
+    }
+    if (in) {
+      if (live) obj.report(mine, meta, xl, st);
+      else obj.skip(mine);
+    }
+  }
+}
+
+// The distillation: a warp per row.
+template <typename T, int E, class Obj, bool GRAD>
+__global__ void __launch_bounds__(GROUP_THREADS) k_group_targets(const View<T> x, const long long rows, const Obj obj, const T k, const Out<T> g) {
+  constexpr int VEC = Num<T>::VEC, G = 32;
   pdl_wait();
   extern __shared__ __align__(16) unsigned char dyn[];
-  const int lane = threadIdx.x % G;
+  const int lane = threadIdx.x % 32;
   const long long warps = (long long)gridDim.x * (GROUP_THREADS / 32);
-  // All groups of a warp take the same number of turns: shuffles name the whole warp.
-  for (long long w = (long long)blockIdx.x * (GROUP_THREADS / 32) + threadIdx.x / 32; w * PER_WARP < rows; w += warps) {
-    const long long r = w * PER_WARP + (threadIdx.x % 32) / G;
-    const bool in = r < rows;
-    typename Obj::Meta meta{};
-    if (in) meta = obj.meta(r);
-    const bool live = in && meta.live();
-    const Span<T> row(x.row(in ? r : 0), in ? x.v : 0);
+  for (long long r = (long long)blockIdx.x * (GROUP_THREADS / 32) + threadIdx.x / 32; r < rows; r += warps) {
+    const typename Obj::Meta meta = obj.meta(r);
+    const bool live = meta.live();
+    const Span<T> row(x.row(r), x.v);
     T y[E * VEC];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -498,92 +578,48 @@ __global__ void __launch_bounds__(GROUP_THREADS) k_group(View<T> x, long long ro
         for (int c = 0; c < VEC; ++c) y[e * VEC + c] = neg_inf<T>();
       }
     }
-    if constexpr (!Obj::TARGETS) {
-      const int l = live ? (int)clamp_label(meta.label, x.v) + row.off : 0;
-      T xl = (T)0;
+    // Per warp: the targets' total probability at each of the row's elements, and the entries.
+    T* hit = (T*)dyn + (threadIdx.x / 32) * (E * 32 * VEC + 2 * obj.k);
+    T* q = hit + E * 32 * VEC;
+    T* xk = q + obj.k;
+    int* at = (int*)((T*)dyn + (GROUP_THREADS / 32) * (E * 32 * VEC + 2 * obj.k)) + (threadIdx.x / 32) * obj.k;
+    typename Obj::Part part{0, 0, 0, false};
+    if (live) part = obj.prepare(r, x.row(r), x.v, lane, GRAD ? at : nullptr, q, xk);
+    const bool some = live && part.some;
+    if (GRAD && some) {
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (lane + G * e == l / VEC) {
-#pragma unroll
-          for (int c = 0; c < VEC; ++c)
-            if (l % VEC == c) xl = y[e * VEC + c];
+      for (int e = 0; e < E * VEC; ++e) hit[lane + 32 * e] = (T)0;
+      __syncwarp();
+      // 32 entries at a time: the first lane of those with the same index adds them up in order.
+      for (long long i0 = 0; i0 < obj.k; i0 += 32) {
+        const long long i = i0 + lane;
+        const bool on = i < obj.k;
+        const int l = on ? at[i] : -1 - lane;
+        unsigned same = __match_any_sync(~0u, l);
+        const bool first = (same & ((1u << lane) - 1)) == 0;
+        if (on && first) {
+          T sum = hit[l + row.off];
+          for (; same; same &= same - 1) sum += q[i0 + __ffs(same) - 1];
+          hit[l + row.off] = sum;
         }
-      Stat<T> st;
-      T c, f;
-      if constexpr (Obj::GIVEN) {
-        st = {meta.m, meta.s};
-        c = meta.c;
-        f = -c / st.s;
-#pragma unroll
-        for (int q = 0; q < E * VEC; ++q) y[q] = Num<T>::exps(y[q] - st.m, k);
-      } else {
-        xl = __shfl_sync(~0u, xl, (l / VEC) % G, G);
-        const Stat<T> own = exponentials<T, E * VEC>(y, k);
-        st = join<G>(own, k);
-        c = live ? obj.coef(meta, xl, st) : (T)0;
-        f = share(own.m, st, k, -c);
-      }
-      if (GRAD) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-#pragma unroll
-          for (int q = 0; q < VEC; ++q) y[e * VEC + q] = live ? y[e * VEC + q] * f : (T)0;
-          if (live && lane + G * e == l / VEC) {
-#pragma unroll
-            for (int q = 0; q < VEC; ++q)
-              if (l % VEC == q) y[e * VEC + q] += c;
-          }
-        }
-        store_group<T, G, E>(g.row(in ? r : 0), row, lane, y);
-      }
-      if (lane == 0 && in) {
-        if (live) obj.report(r, meta, xl, st);
-        else obj.skip(r);
-      }
-    } else {
-      // Per warp: the targets' total probability at each of the row's elements, and the entries.
-      T* hit = (T*)dyn + (threadIdx.x / 32) * (E * 32 * VEC + 2 * obj.k);
-      T* q = hit + E * 32 * VEC;
-      T* xk = q + obj.k;
-      int* at = (int*)((T*)dyn + (GROUP_THREADS / 32) * (E * 32 * VEC + 2 * obj.k)) + (threadIdx.x / 32) * obj.k;
-      typename Obj::Part part{0, 0, 0, false};
-      if (live) part = obj.prepare(r, x.row(r), x.v, lane, GRAD ? at : nullptr, q, xk);
-      const bool some = live && part.some;
-      if (GRAD && some) {
-#pragma unroll
-        for (int e = 0; e < E * VEC; ++e) hit[lane + 32 * e] = (T)0;
-        __syncwarp();
-        // 32 entries at a time: the first lane of those with the same index adds them up in order.
-        for (long long i0 = 0; i0 < obj.k; i0 += 32) {
-          const long long i = i0 + lane;
-          const bool on = i < obj.k;
-          const int l = on ? at[i] : -1 - lane;
-          unsigned same = __match_any_sync(~0u, l);
-          const bool first = (same & ((1u << lane) - 1)) == 0;
-          if (on && first) {
-            T sum = hit[l + row.off];
-            for (; same; same &= same - 1) sum += q[i0 + __ffs(same) - 1];
-            hit[l + row.off] = sum;
-          }
-          __syncwarp();
-        }
-      }
-      const Stat<T> own = exponentials<T, E * VEC>(y, k);
-      const Stat<T> st = join<G>(own, k);
-      if (GRAD) {
-        const T c = meta.w * obj.wt, f = some ? share(own.m, st, k, c) : (T)0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-#pragma unroll
-          for (int z = 0; z < VEC; ++z) y[e * VEC + z] = some ? y[e * VEC + z] * f - c * hit[(lane + 32 * e) * VEC + z] : (T)0;
-        }
-        store_group<T, G, E>(g.row(in ? r : 0), row, lane, y);
         __syncwarp();
       }
-      if (lane == 0 && in) {
-        if (live) obj.report(r, meta, part, st);
-        else obj.skip(r);
+    }
+    const Stat<T> own = exponentials<T, E * VEC>(y, k);
+    const Stat<T> st = join<G>(own, k);
+    if (GRAD) {
+      const T c = meta.w * obj.wt, f = some ? share(own.m, st, k, c) : (T)0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+#pragma unroll
+        for (int z = 0; z < VEC; ++z) y[e * VEC + z] = some ? y[e * VEC + z] * f - c * hit[(lane + 32 * e) * VEC + z] : (T)0;
       }
+      store_group<T, G, E>(g.row(r), row, lane, y);
+      __syncwarp();
+    }
+    if (lane == 0) {
+      if (live) obj.report(r, meta, part, st);
+      else obj.skip(r);
     }
   }
 }
@@ -922,13 +958,34 @@ __device__ double block_sum(double v, double* sh) {
   return r;
 }
 
-template <typename T> __global__ void __launch_bounds__(1024) k_sum_terms(const T* __restrict__ terms, long long n, T* loss, double scale) {
+// A cluster's blocks, or one block, add up the terms: eight of a thread at a time, then threads, warps and blocks in order.
+constexpr int SUM_THREADS = 512, SUM_CLUSTER = 8;
+template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms(const T* __restrict__ terms, long long n, T* loss, double scale) {
   pdl_wait();
-  __shared__ double sh[32];
+  __shared__ double sh[SUM_THREADS / 32];
+  __shared__ Pair<double> of_block[SUM_CLUSTER];
+  const unsigned rank = cluster_rank(), blocks = cluster_size();
+  if (blocks > 1) cluster_sync();
   double v = 0;
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) v += (double)terms[i];
+  const long long step = (long long)blocks * SUM_THREADS;
+  long long i = (long long)rank * SUM_THREADS + threadIdx.x;
+  for (; i + 7 * step < n; i += 8 * step) {
+    T z[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) z[q] = terms[i + q * step];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += (double)z[q];
+  }
+  for (; i < n; i += step) v += (double)terms[i];
   v = block_sum(v, sh);
-  if (threadIdx.x == 0) *loss = (T)(v * scale);
+  if (blocks > 1) {
+    if (threadIdx.x == 0) put_remote(&of_block[rank], 0u, Pair<double>{v, 0.0});
+    cluster_sync();
+    if (rank != 0) return;
+    v = 0;
+    for (unsigned b = 0; b < blocks; ++b) v += of_block[b].m;
+  }
+  if (rank == 0 && threadIdx.x == 0) *loss = (T)(v * scale);
 }
 
 // Block k: pair k's sequence sums, margin, loss term and the coefficients of its two sequences.
@@ -1035,32 +1092,38 @@ unsigned split(long long rows, long long vectors, long long most, long long leas
   return c;
 }
 
-template <typename T, int G, int E, class Obj, bool GRAD> cudaError_t go_group(const RowView& x, const Obj& obj, T k, const RowOut& g, size_t smem, cudaStream_t s) {
-  auto* kernel = k_group<T, G, E, Obj, GRAD>;
-  const long long warps = pieces_of(x.rows(), 32 / G), blocks = std::min(pieces_of(warps, GROUP_THREADS / 32), resident(kernel, GROUP_THREADS, smem, 1));
+template <typename K, typename T, class Obj>
+cudaError_t go_group(K* kernel, long long rows_per_warp, const RowView& x, const Obj& obj, T k, const RowOut& g, size_t smem, cudaStream_t s) {
+  const long long warps = pieces_of(x.rows(), rows_per_warp), blocks = std::min(pieces_of(warps, GROUP_THREADS / 32), resident(kernel, GROUP_THREADS, smem, 1));
   return launch(kernel, dim3((unsigned)blocks), dim3(GROUP_THREADS), smem, 1, s, view<T>(x), x.rows(), obj, k, out<T>(x, g));
 }
 
-// Rows of at most 256 vectors, by the fewest lanes that hold one in at most 8 vectors each.
-constexpr long long GROUP_VECTORS = 256;
+// Rows of at most 512 vectors, by the fewest lanes that hold one; up to 16 vectors a lane in all.
+constexpr long long GROUP_VECTORS = 512;
 template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, const Obj& obj, T k, const RowOut& g, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
   if constexpr (Obj::TARGETS) {
-    const int e = v <= 32 ? 1 : v <= 64 ? 2 : v <= 128 ? 4 : 8;
+    const int e = v <= 32 ? 1 : v <= 64 ? 2 : v <= 128 ? 4 : v <= 256 ? 8 : 16;
     const size_t smem = (GROUP_THREADS / 32) * ((e * 32 * Num<T>::VEC + 2 * (size_t)obj.k) * sizeof(T) + (size_t)obj.k * sizeof(int));
+    auto go = [&](auto* kernel) { return go_group(kernel, 1, x, obj, k, g, smem, s); };
     switch (e) {
-      case 1: return go_group<T, 32, 1, Obj, GRAD>(x, obj, k, g, smem, s);
-      case 2: return go_group<T, 32, 2, Obj, GRAD>(x, obj, k, g, smem, s);
-      case 4: return go_group<T, 32, 4, Obj, GRAD>(x, obj, k, g, smem, s);
-      default: return go_group<T, 32, 8, Obj, GRAD>(x, obj, k, g, smem, s);
+      case 1: return go(k_group_targets<T, 1, Obj, GRAD>);
+      case 2: return go(k_group_targets<T, 2, Obj, GRAD>);
+      case 4: return go(k_group_targets<T, 4, Obj, GRAD>);
+      case 8: return go(k_group_targets<T, 8, Obj, GRAD>);
+      default: return go(k_group_targets<T, 16, Obj, GRAD>);
     }
   } else {
-    if (v <= 8) return go_group<T, 8, 1, Obj, GRAD>(x, obj, k, g, 0, s);
-    if (v <= 16) return go_group<T, 8, 2, Obj, GRAD>(x, obj, k, g, 0, s);
-    if (v <= 32) return go_group<T, 8, 4, Obj, GRAD>(x, obj, k, g, 0, s);
-    if (v <= 64) return go_group<T, 8, 8, Obj, GRAD>(x, obj, k, g, 0, s);
-    if (v <= 128) return go_group<T, 16, 8, Obj, GRAD>(x, obj, k, g, 0, s);
-    return go_group<T, 32, 8, Obj, GRAD>(x, obj, k, g, 0, s);
+    auto go = [&](auto* kernel, int rows) { return go_group(kernel, rows, x, obj, k, g, 0, s); };
+    if (v <= 8) return go(k_group<T, 8, 1, 8, Obj, GRAD>, 32);
+    if (v <= 16) return go(k_group<T, 8, 2, 8, Obj, GRAD>, 32);
+    if (v <= 24) return go(k_group<T, 8, 3, 5, Obj, GRAD>, 20);
+    if (v <= 32) return go(k_group<T, 8, 4, 4, Obj, GRAD>, 16);
+    if (v <= 64) return go(k_group<T, 16, 4, 4, Obj, GRAD>, 8);
+    if (v <= 128) return go(k_group<T, 32, 4, 4, Obj, GRAD>, 4);
+    if (v <= 256) return go(k_group<T, 32, 8, 2, Obj, GRAD>, 2);
+    if (v <= 384) return go(k_group<T, 32, 12, 1, Obj, GRAD>, 1);
+    return go(k_group<T, 32, 16, 1, Obj, GRAD>, 1);
   }
 }
 
@@ -1077,19 +1140,24 @@ cudaError_t go_rows(const RowView& x, const Obj& obj, T k, const RowOut& g, long
   return launch(kernel, dim3((unsigned)(clusters * cluster)), dim3(NT), smem, cluster, s, view<T>(x), x.rows(), obj, k, out<T>(x, g), (int)slice);
 }
 
+constexpr long long L2_ROWS_BYTES = 64ll << 20;
 // Rows with a gradient that no group holds.
 template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& obj, T k, const RowOut& g, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
   unsigned c = split(x.rows(), v, v, 512);
-  if (getenv("CX")) c = atoi(getenv("CX"));
+  // Rows under way at once that do not fit the L2 (its two halves hold copies of what the other half's SMs read):
+  // fewer, each by a cluster.
+  if (c == 1 && v * 16 * 2 * sm_count() > L2_ROWS_BYTES)
+    for (c = 2; c < MAX_CLUSTER && v * 16 * 4 * sm_count() / c > L2_ROWS_BYTES; c *= 2) {
+    }
   const long long slice = pieces_of(v, c);
-  const char* e = getenv("NTX");
-  int nt = e ? atoi(e) : slice <= 1024 ? 128 : slice <= 4096 ? 256 : slice <= 16384 ? 512 : 1024;
-  if (c > 1) return nt == 512 ? go_rows<T, 512, true>(x, obj, k, g, slice, c, s) : nt == 1024 ? go_rows<T, 1024, true>(x, obj, k, g, slice, c, s) : go_rows<T, 256, true>(x, obj, k, g, slice, c, s);
-  if (nt == 128) return go_rows<T, 128, false>(x, obj, k, g, slice, 1, s);
-  if (nt == 256) return go_rows<T, 256, false>(x, obj, k, g, slice, 1, s);
-  if (nt == 512) return go_rows<T, 512, false>(x, obj, k, g, slice, 1, s);
-  return go_rows<T, 1024, false>(x, obj, k, g, slice, 1, s);
+  if (c > 1) return go_rows<T, 256, true>(x, obj, k, g, slice, c, s);
+  // About four turns of a block over the row: 8192 floats (2048 vectors) at 78, 91, 84 and 65 % of the copy rate with 64, 128,
+  // 256 and 512 threads, 16384 at 68, 78, 90 and 81 %, 4096 at 88, 84, 68 and 33 %.
+  if (v <= 1448) return go_rows<T, 64, false>(x, obj, k, g, slice, 1, s);
+  if (v <= 2896) return go_rows<T, 128, false>(x, obj, k, g, slice, 1, s);
+  if (v <= 5792) return go_rows<T, 256, false>(x, obj, k, g, slice, 1, s);
+  return go_rows<T, 512, false>(x, obj, k, g, slice, 1, s);
 }
 
 template <typename T, class Obj> cudaError_t stream(const RowView& x, const Obj& obj, T k, cudaStream_t s) {
@@ -1128,7 +1196,8 @@ template <typename T> cudaError_t given_grad(const RowView& x, const GivenRow<T>
 }
 
 template <typename T> cudaError_t sum_terms(const void* terms, long long n, void* loss, double scale, cudaStream_t s) {
-  return launch(k_sum_terms<T>, 1, 1024, 0, 1, s, (const T*)terms, n, (T*)loss, scale);
+  const unsigned blocks = n > 8 * SUM_THREADS ? SUM_CLUSTER : 1;
+  return launch(k_sum_terms<T>, dim3(blocks), dim3(SUM_THREADS), 0, blocks, s, (const T*)terms, n, (T*)loss, scale);
 }
 
 }  // namespace
