@@ -13,7 +13,7 @@
 // Numbers. Row statistics are held in the logits' type. For float, exp(x - m) is computed as
 // 2^((x - m) * log2 e) with the hardware's ex2: the difference and the product are rounded, 2.3 u |x - m|
 // relatively (log2 e as a float is 0.22 u off), and ex2 is within 2 ulp; against expf that halves the
-// instructions per logit. What a row reports (its log-probability's terms) is computed from the statistics
+// instructions per logit. For double it is a polynomial (Num<double>). What a row reports (its log-probability's terms) is computed from the statistics
 // in double by one lane, and sums over rows are double: a loss is a sum of terms of both signs.
 // Everything is summed in a fixed order: the same inputs give the same bits on every call. The bits of a row do
 // depend on how it is split over lanes and blocks, which goes by the vocabulary and the row count.
@@ -81,11 +81,26 @@ template <> struct Num<float> {
 template <> struct Num<double> {
   static constexpr int VEC = 2;
   using Vec = double2;
-  static __device__ __forceinline__ double exps(double d, double k) { return exp(d * k); }
+  // exp(d * scale) for d <= 0: 2^t with t = d * scale * log2 e = n + f, n whole and |f| <= 1/2; 2^f by the polynomial of
+  // degree 11 that equals it at 12 Chebyshev nodes (off by 4.3e-18 relatively; 1.2 u with Horner's roundings).
+  // Below 2^-1022 it is 0. 17 double operations, where exp() took twice as long for the whole pass.
+  static __device__ __forceinline__ double exps(double d, double k) {
+    constexpr double C[12] = {0x1.0000000000000p+0,  0x1.62e42fefa39efp-1,  0x1.ebfbdff82c5aep-3,  0x1.c6b08d704a0c6p-5,
+                              0x1.3b2ab6fb9f1a5p-7,  0x1.5d87fe78a3f9cp-10, 0x1.430913112c61bp-13, 0x1.ffcbfc6da6ed1p-17,
+                              0x1.62bfc2c86d700p-20, 0x1.b524ebd13a55fp-24, 0x1.e6228acd1c6e5p-28, 0x1.e9ec1fcb69a7fp-32};
+    constexpr double WHOLE = 6755399441055744.0;  // 3 * 2^51: adding it rounds to a whole number, in the low bits
+    const double t = d * k, w = t + WHOLE, f = t - (w - WHOLE);
+    double r = C[11];
+#pragma unroll
+    for (int i = 10; i >= 0; --i) r = __fma_rn(r, f, C[i]);
+    // Beyond 2^1024, which only wrong statistics of a caller's give, it is infinity; NaN stays NaN in r.
+    const double two_n = __hiloint2double(__double2hiint(t) >= 0x40900000 ? 0x7ff00000 : (__double2loint(w) + 1023) << 20, 0);
+    return t < -1022.0 ? 0.0 : r * two_n;
+  }
   static __device__ __forceinline__ double ex(double v) { return exp(v); }
   static __device__ __forceinline__ double ln(double v) { return log(v); }
   static __device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
-  static double factor(double scale) { return scale; }
+  static double factor(double scale) { return scale * 1.4426950408889634074; }
 };
 
 template <typename T> __device__ __forceinline__ T neg_inf() { return -(T)INFINITY; }
@@ -258,13 +273,14 @@ __device__ __forceinline__ long long clamp_label(int l, long long v) { return l 
 template <typename T> struct LogProbRow {
   static constexpr bool TARGETS = false, GIVEN = false;
   const int32_t* labels;
+  const T* weight;  // null: every row counts
   T *logp, *stats;
   struct Meta {
     int label;
     T w;
     __device__ __forceinline__ bool live() const { return w != (T)0; }
   };
-  __device__ __forceinline__ Meta meta(long long r) const { return {labels[r], (T)1}; }
+  __device__ __forceinline__ Meta meta(long long r) const { return {labels[r], weight ? weight[r] : (T)1}; }
   __device__ void skip(long long) const {}
   __device__ __forceinline__ T coef(const Meta&, T, Stat<T>) const { return (T)0; }
   __device__ __forceinline__ void report(long long r, const Meta&, T xl, Stat<T> st) const {
@@ -380,19 +396,48 @@ template <typename T> struct DistillRow {
     const double lse = ((double)st.m - p.from) * inverse + (double)Num<T>::ln(st.s);
     terms[r] = p.some ? (T)((double)m.w * (double)wt * (double)wt * (p.a + lse * p.q)) : (T)0;
   }
-  // One warp; x: the row's logits. Keeps q, the index and its logit of each entry when `at` is given.
-  __device__ Part prepare(long long r, const T* x, long long v, int lane, int* at, T* q, T* xk) const {
-    const T* t = teacher + r * k;
-    const int32_t* ix = index + r * k;
+  struct Entry {
+    T t, x;
+    int at;
+  };
+  // Entry i of row r, whose logits are at x.
+  __device__ __forceinline__ Entry entry(long long r, const T* x, long long v, int i) const {
+    Entry e;
+    e.t = teacher[r * k + i];
+    e.at = (int)clamp_label(index[r * k + i], v);
+    e.x = x[e.at];
+    return e;
+  }
+  // The entries' loads, two of each lane, before the row's: what they are needed for comes after it.
+  struct Ahead {
+    T t[2], x[2];
+    int at[2];
+  };
+  __device__ __forceinline__ Ahead ahead(long long r, const T* x, long long v, int lane) const {
+    Ahead h;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = lane + 32 * e;
+      const bool on = i < (int)k;
+      h.t[e] = on ? teacher[r * k + i] : neg_inf<T>();
+      h.at[e] = on ? (int)clamp_label(index[r * k + i], v) : 0;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) h.x[e] = lane + 32 * e < (int)k ? x[h.at[e]] : (T)0;
+    return h;
+  }
+  // One warp; x: the row's logits, h: ahead(). Keeps q, the index and its logit of each entry when `at` is given.
+  __device__ Part prepare(long long r, const T* x, long long v, int lane, const Ahead& h, int* at, T* q, T* xk) const {
+    auto get = [&](int i) { return i < 32 ? Entry{h.t[0], h.x[0], h.at[0]} : i < 64 ? Entry{h.t[1], h.x[1], h.at[1]} : entry(r, x, v, i); };
     Stat<T> st;
     Part p{0, 0, 0, false};
     T far = neg_inf<T>();  // the largest logit of the entries
-#pragma unroll 2
     for (int i = lane; i < (int)k; i += 32) {
-      const T z = t[i], xi = x[clamp_label(ix[i], v)], m = z > st.m ? z : st.m;
-      st.s = st.s * Num<T>::exps(st.m - base(m), tk) + Num<T>::exps(z - base(m), tk);
+      const Entry n = get(i);
+      const T m = n.t > st.m ? n.t : st.m;
+      st.s = st.s * Num<T>::exps(st.m - base(m), tk) + Num<T>::exps(n.t - base(m), tk);
       st.m = m;
-      if (z != neg_inf<T>()) far = Num<T>::most(far, xi);
+      if (n.t != neg_inf<T>()) far = Num<T>::most(far, n.x);
     }
     st = join<32>(st, tk);
     for (int d = 16; d; d >>= 1) far = Num<T>::most(far, __shfl_xor_sync(~0u, far, d));
@@ -401,15 +446,15 @@ template <typename T> struct DistillRow {
     const T inv = (T)1 / st.s;
     const double logs = (double)Num<T>::ln(st.s);
     for (int i = lane; i < (int)k; i += 32) {
-      const long long l = clamp_label(ix[i], v);
-      const T d = t[i] - base(st.m), qi = p.some ? Num<T>::exps(d, tk) * inv : (T)0, xi = x[l];
+      const Entry n = get(i);
+      const T d = n.t - base(st.m), qi = p.some ? Num<T>::exps(d, tk) * inv : (T)0;
       if (at) {
-        at[i] = (int)l;
+        at[i] = n.at;
         q[i] = qi;
-        xk[i] = xi;
+        xk[i] = n.x;
       }
       if (qi != (T)0) {
-        p.a += (double)qi * (((double)d - ((double)xi - p.from)) * inverse - logs);
+        p.a += (double)qi * (((double)d - ((double)n.x - p.from)) * inverse - logs);
         p.q += (double)qi;
       }
     }
@@ -420,6 +465,46 @@ template <typename T> struct DistillRow {
     return p;
   }
 };
+
+// A row's entries in shared memory: the indices (whole vectors of four, the rest -1), the probabilities, the logits.
+template <typename T> struct Kept {
+  int* at;
+  T *q, *x;
+  __device__ __forceinline__ Kept(unsigned char* p, int k) {
+    at = (int*)p;
+    q = (T*)(p + (k + 3) / 4 * 16);
+    x = q + k;
+  }
+  __device__ __forceinline__ void fill(int k, int lane) {
+    if (lane < (k + 3) / 4 * 4 - k) at[k + lane] = -1;
+  }
+  // Whether entry i is the first with its index; *sum: the probabilities of all of them, in order. Most are alone.
+  __device__ __forceinline__ bool leads(int i, int k, T* sum) const {
+    const int mine = at[i];
+    int n = 0;
+    for (int o = 0; o < k; o += 4) {
+      const int4 z = *reinterpret_cast<const int4*>(at + o);
+      n += (z.x == mine) + (z.y == mine) + (z.z == mine) + (z.w == mine);
+    }
+    *sum = q[i];
+    if (n == 1) return true;
+    *sum = (T)0;
+    for (int o = 0; o < k; ++o) {
+      if (at[o] != mine) continue;
+      if (o < i) return false;
+      *sum += q[o];
+    }
+    return true;
+  }
+};
+struct NoKept {
+  __device__ __forceinline__ NoKept(unsigned char*, int) {}
+};
+template <class Obj> __device__ __forceinline__ int entries_per_row(const Obj& obj) {
+  if constexpr (Obj::TARGETS) return (int)obj.k;
+  else return 0;
+}
+template <typename T> size_t kept_bytes(size_t k) { return (k + 3) / 4 * 16 + (2 * k * sizeof(T) + 15) / 16 * 16; }
 
 // ---- short rows: a group of G lanes per row ----
 
@@ -441,37 +526,6 @@ template <typename T, int N> __device__ __forceinline__ Stat<T> exponentials(T* 
   }
   a.s = s0 + s1;
   return a;
-}
-
-// The same of the first `turns` of E vectors.
-template <typename T, int E, int VEC> __device__ __forceinline__ Stat<T> exponentials(T* x, T k, int turns) {
-  Stat<T> a;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e < turns) {
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) a.m = Num<T>::most(x[e * VEC + c], a.m);
-    }
-  const T b = base(a.m);
-  T s0 = (T)0, s1 = (T)0;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e < turns) {
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) {
-        T& z = x[e * VEC + c];
-        z = Num<T>::exps(z - b, k);
-        if (c % 2) s1 += z;
-        else s0 += z;
-      }
-    }
-  a.s = s0 + s1;
-  return a;
-}
-
-// What this thread's exponentials are multiplied by to give scale * p.
-template <typename T> __device__ __forceinline__ T share(T m, Stat<T> st, T k, T scale) {
-  return (m == neg_inf<T>() ? (T)0 : Num<T>::exps(m - base(st.m), k)) * (scale / st.s);
 }
 
 // A warp computes B times 32 / G rows together (G lanes each, E vectors a lane): all loads first, then the sums, then what
@@ -556,70 +610,131 @@ __global__ void __launch_bounds__(GROUP_THREADS, 2) k_group(const View<T> x, con
   }
 }
 
-// The distillation: a warp per row.
-template <typename T, int E, class Obj, bool GRAD>
-__global__ void __launch_bounds__(GROUP_THREADS) k_group_targets(const View<T> x, const long long rows, const Obj obj, const T k, const Out<T> g) {
-  constexpr int VEC = Num<T>::VEC, G = 32;
-  pdl_wait();
+// The same for the distillation. `gk` lanes take a row's entries, 32 / gk rows at a time, and what they come to goes
+// to the row's lane; with MANY, more than 32 entries, a warp has one row. The gradients at the entries are written a second time, over what the row's
+// lanes have stored; the first entry of an index writes its element, with the probabilities of all of that index.
+template <typename T, int G, int E, int B, bool MANY, class Obj, bool GRAD>
+__global__ void __launch_bounds__(GROUP_THREADS, 2) k_group_targets(const View<T> x, const long long rows, const Obj obj, const T k, const Out<T> g, const int gk) {
+  constexpr int VEC = Num<T>::VEC, R = 32 / G, ROWS = B * R, KEEP = GRAD && !MANY ? ROWS * 32 : 1;
+  static_assert(ROWS <= 32 && (!MANY || ROWS == 1), "a lane per row");
+  __shared__ T keep_q[GROUP_THREADS / 32][KEEP], keep_x[GROUP_THREADS / 32][KEEP];
+  __shared__ int keep_at[GROUP_THREADS / 32][KEEP];
   extern __shared__ __align__(16) unsigned char dyn[];
-  const int lane = threadIdx.x % 32;
+  pdl_wait();
+  const int lane = threadIdx.x % 32, in_group = lane % G, group = lane / G, i = lane % gk, of = lane / gk, at_once = 32 / gk;
+  T *kq = keep_q[threadIdx.x / 32], *kx = keep_x[threadIdx.x / 32];
+  int* ka = keep_at[threadIdx.x / 32];
+  Kept<T> kept(dyn + (MANY && GRAD ? threadIdx.x / 32 * ((obj.k + 3) / 4 * 16 + (2 * obj.k * sizeof(T) + 15) / 16 * 16) : 0), (int)obj.k);
   const long long warps = (long long)gridDim.x * (GROUP_THREADS / 32);
-  for (long long r = (long long)blockIdx.x * (GROUP_THREADS / 32) + threadIdx.x / 32; r < rows; r += warps) {
-    const typename Obj::Meta meta = obj.meta(r);
-    const bool live = meta.live();
-    const Span<T> row(x.row(r), x.v);
-    T y[E * VEC];
+  for (long long w = (long long)blockIdx.x * (GROUP_THREADS / 32) + threadIdx.x / 32; w * ROWS < rows; w += warps) {
+    const long long row0 = w * ROWS, mine = row0 + lane;
+    const bool in = lane < ROWS && mine < rows;
+    typename Obj::Meta meta{};
+    if (in) meta = obj.meta(mine);
+    const bool live = in && meta.live();
+    const unsigned lives = __ballot_sync(~0u, live);
+    auto fetch = [&](int j) {  // this lane's entry of row j of the warp's
+      if (j < ROWS && i < (int)obj.k && (lives >> j & 1)) return obj.entry(row0 + j, x.row(row0 + j), x.v, i);
+      return typename Obj::Entry{neg_inf<T>(), (T)0, -1 - lane};
+    };
+    typename Obj::Entry next;
+    typename Obj::Ahead ahead;
+    if constexpr (!MANY) next = fetch(of);
+    else if (lives) ahead = obj.ahead(row0, x.row(row0), x.v, lane);
+    T y[B][E * VEC], most[B];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (live) {
-        row.load(lane + G * e, y + e * VEC);
+    for (int b = 0; b < B; ++b) {
+      const int at = b * R + group;
+      if (lives >> at & 1) {
+        const Span<T> row(x.row(row0 + at), x.v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) row.load(in_group + G * e, y[b] + e * VEC);
       } else {
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) y[e * VEC + c] = neg_inf<T>();
+        for (int q = 0; q < E * VEC; ++q) y[b][q] = neg_inf<T>();
       }
     }
-    // Per warp: the targets' total probability at each of the row's elements, and the entries.
-    T* hit = (T*)dyn + (threadIdx.x / 32) * (E * 32 * VEC + 2 * obj.k);
-    T* q = hit + E * 32 * VEC;
-    T* xk = q + obj.k;
-    int* at = (int*)((T*)dyn + (GROUP_THREADS / 32) * (E * 32 * VEC + 2 * obj.k)) + (threadIdx.x / 32) * obj.k;
     typename Obj::Part part{0, 0, 0, false};
-    if (live) part = obj.prepare(r, x.row(r), x.v, lane, GRAD ? at : nullptr, q, xk);
+    if constexpr (MANY) {
+      if (lives) part = obj.prepare(row0, x.row(row0), x.v, lane, ahead, GRAD ? kept.at : nullptr, kept.q, kept.x);
+      if (GRAD) kept.fill((int)obj.k, lane);
+    }
+    for (int j0 = 0; !MANY && j0 < ROWS; j0 += at_once) {
+      const typename Obj::Entry now = next;
+      next = fetch(j0 + at_once + of);
+      T top = now.t != now.t ? neg_inf<T>() : now.t, far = now.t != neg_inf<T>() ? Num<T>::most(now.x, neg_inf<T>()) : neg_inf<T>();
+      for (int d = gk / 2; d; d >>= 1) {
+        top = Num<T>::most(top, __shfl_xor_sync(~0u, top, d));
+        far = Num<T>::most(far, __shfl_xor_sync(~0u, far, d));
+      }
+      const T from = far > neg_inf<T>() && far < -neg_inf<T>() ? far : (T)0, dt = now.t - base(top), e = Num<T>::exps(dt, obj.tk);
+      T s = e;
+      for (int d = gk / 2; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+      const T q = s != (T)0 ? e * ((T)1 / s) : (T)0;  // all entries -inf: none
+      double a = q != (T)0 ? (double)q * (((double)dt - ((double)now.x - (double)from)) * obj.inverse - (double)Num<T>::ln(s)) : 0.0, total = (double)q;
+      for (int d = gk / 2; d; d >>= 1) {
+        a += __shfl_xor_sync(~0u, a, d);
+        total += __shfl_xor_sync(~0u, total, d);
+      }
+      const int src = lane % at_once * gk;
+      a = __shfl_sync(~0u, a, src);
+      total = __shfl_sync(~0u, total, src);
+      const T z = __shfl_sync(~0u, from, src);
+      if (lane / at_once == j0 / at_once) part = {a, total, (double)z, total != 0};
+      if constexpr (GRAD) {
+        kq[j0 * gk + lane] = q;
+        kx[j0 * gk + lane] = now.x;
+        ka[j0 * gk + lane] = now.at;
+      }
+    }
+    Stat<T> st;
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const Stat<T> own = exponentials<T, E * VEC>(y[b], k);
+      most[b] = own.m;
+      const Stat<T> all = join<G>(own, k);
+      const T m = __shfl_sync(~0u, all.m, lane % R * G), s = __shfl_sync(~0u, all.s, lane % R * G);
+      if (lane / R == b) st = {m, s};
+    }
     const bool some = live && part.some;
-    if (GRAD && some) {
+    if constexpr (GRAD) {
+      const unsigned somes = __ballot_sync(~0u, some);
+      const T c = some ? meta.w * obj.wt : (T)0, scale = some ? c / st.s : (T)0;
 #pragma unroll
-      for (int e = 0; e < E * VEC; ++e) hit[lane + 32 * e] = (T)0;
+      for (int b = 0; b < B; ++b) {
+        const int at = (b * R + group) % 32;
+        const T sc = __shfl_sync(~0u, scale, at), m = __shfl_sync(~0u, st.m, at);
+        const T f = most[b] == neg_inf<T>() ? (T)0 * sc : Num<T>::exps(most[b] - base(m), k) * sc;
+        const bool zero = !(somes >> at & 1), have = row0 + b * R + group < rows;
+#pragma unroll
+        for (int q = 0; q < E * VEC; ++q) y[b][q] = zero ? (T)0 : y[b][q] * f;
+        const long long r = have ? row0 + b * R + group : row0;
+        store_group<T, G, E>(g.row(r), Span<T>(x.row(r), have ? x.v : 0), in_group, y[b]);
+      }
       __syncwarp();
-      // 32 entries at a time: the first lane of those with the same index adds them up in order.
-      for (long long i0 = 0; i0 < obj.k; i0 += 32) {
-        const long long i = i0 + lane;
-        const bool on = i < obj.k;
-        const int l = on ? at[i] : -1 - lane;
-        unsigned same = __match_any_sync(~0u, l);
-        const bool first = (same & ((1u << lane) - 1)) == 0;
-        if (on && first) {
-          T sum = hit[l + row.off];
-          for (; same; same &= same - 1) sum += q[i0 + __ffs(same) - 1];
-          hit[l + row.off] = sum;
+      const unsigned ours = (gk == 32 ? ~0u : (1u << gk) - 1) << (of * gk);
+      if constexpr (MANY) {
+        const T sc = __shfl_sync(~0u, scale, 0), cj = __shfl_sync(~0u, c, 0), m = __shfl_sync(~0u, st.m, 0);
+        for (int e = lane; somes && e < (int)obj.k; e += 32) {
+          T sum;
+          if (kept.leads(e, (int)obj.k, &sum)) g.row(row0)[kept.at[e]] = Num<T>::exps(kept.x[e] - m, k) * sc - cj * sum;
         }
-        __syncwarp();
       }
-    }
-    const Stat<T> own = exponentials<T, E * VEC>(y, k);
-    const Stat<T> st = join<G>(own, k);
-    if (GRAD) {
-      const T c = meta.w * obj.wt, f = some ? share(own.m, st, k, c) : (T)0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-#pragma unroll
-        for (int z = 0; z < VEC; ++z) y[e * VEC + z] = some ? y[e * VEC + z] * f - c * hit[(lane + 32 * e) * VEC + z] : (T)0;
+      for (int j0 = 0; !MANY && j0 < ROWS; j0 += at_once) {
+        const int j = j0 + of, at = ka[j0 * gk + lane];
+        unsigned same = __match_any_sync(~0u, at) & ours;
+        const T sc = __shfl_sync(~0u, scale, j % 32), cj = __shfl_sync(~0u, c, j % 32), m = __shfl_sync(~0u, st.m, j % 32);
+        if (j < ROWS && i < (int)obj.k && (somes >> j & 1) && (same & ((1u << lane) - 1)) == 0) {
+          T sum = (T)0;
+          for (; same; same &= same - 1) sum += kq[j0 * gk + __ffs(same) - 1];
+          g.row(row0 + j)[at] = Num<T>::exps(kx[j0 * gk + lane] - m, k) * sc - cj * sum;
+        }
       }
-      store_group<T, G, E>(g.row(r), row, lane, y);
-      __syncwarp();
+      __syncwarp();  // the kept entries are read before the next rows'
     }
-    if (lane == 0) {
-      if (live) obj.report(r, meta, part, st);
-      else obj.skip(r);
+    if (in) {
+      if (live) obj.report(mine, meta, part, st);
+      else obj.skip(mine);
     }
   }
 }
@@ -671,6 +786,13 @@ template <typename T, int N> struct Table {
 };
 template <typename T> __device__ __forceinline__ Pair<T> pair(Stat<T> a) { return {a.m, a.s}; }
 
+template <class Obj, bool TARGETS = Obj::TARGETS> struct AheadOf {
+  struct type {};
+};
+template <class Obj> struct AheadOf<Obj, true> {
+  using type = typename Obj::Ahead;
+};
+
 // ---- longer rows without a gradient ----
 
 constexpr int STREAM_THREADS = 256, STREAM_UNROLL = 4;
@@ -701,9 +823,9 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
     Span<T> row(x.row(r), x.v);
     row.clip(begin, begin + slice);
     T xl = (T)0;
-    typename std::conditional<Obj::TARGETS, EntriesPart, int>::type part{};
+    typename AheadOf<Obj>::type ahead{};
     if constexpr (Obj::TARGETS) {
-      if (reports) part = obj.prepare(r, x.row(r), x.v, lane, nullptr, nullptr, nullptr);
+      if (reports) ahead = obj.ahead(r, x.row(r), x.v, lane);
     } else {
       if (reports && lane == 0) xl = x.row(r)[clamp_label(now.label, x.v)];
     }
@@ -732,9 +854,11 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
     }
     if (reports) {
       const Stat<T> st = CLUSTER ? shares.read(half, (int)blocks, k) : table.read(half, NT / 32, k);
-      if (lane == 0) {
-        if constexpr (Obj::TARGETS) obj.report(r, now, part, st);
-        else obj.report(r, now, xl, st);
+      if constexpr (Obj::TARGETS) {
+        const EntriesPart part = obj.prepare(r, x.row(r), x.v, lane, ahead, nullptr, nullptr, nullptr);
+        if (lane == 0) obj.report(r, now, part, st);
+      } else {
+        if (lane == 0) obj.report(r, now, xl, st);
       }
     }
     half ^= 1;
@@ -794,17 +918,6 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_grad(View<T> x, long long rows
 
 // ---- longer rows with a gradient ----
 
-// Calls, not inlined: registers are for the rows.
-template <typename T, class Obj> __device__ __noinline__ T coef_of(const Obj& obj, typename Obj::Meta m, T xl, Stat<T> st) { return obj.coef(m, xl, st); }
-template <typename T, class Obj> __device__ __noinline__ void report_of(const Obj& obj, long long r, typename Obj::Meta m, T xl, Stat<T> st) { obj.report(r, m, xl, st); }
-template <typename T, class Obj> __device__ __noinline__ void report_entries(const Obj& obj, long long r, typename Obj::Meta m, EntriesPart part, Stat<T> st) {
-  obj.report(r, m, part, st);
-}
-template <typename T, class Obj>
-__device__ __noinline__ EntriesPart entries_of(const Obj& obj, long long r, const T* x, long long v, int lane, int* at, T* q, T* xk) {
-  return obj.prepare(r, x, v, lane, at, q, xk);
-}
-
 // A block of NT threads, or a cluster of such blocks (`slice` vectors each), per row: one pass for the statistics and
 // one, backwards, that reads the logits again and writes the gradient. The second pass finds them in the L2 (or the
 // L1), as long as the rows under way fit there, so memory sees each logit once.
@@ -821,12 +934,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
   __shared__ int entries;
   const unsigned rank = CLUSTER ? cluster_rank() : 0, blocks = CLUSTER ? cluster_size() : 1;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, begin = (int)rank * slice, first = begin + warp * 32 * U;
-  T *tq = (T*)dyn, *tx = nullptr;
-  int* ti = nullptr;
-  if constexpr (Obj::TARGETS) {
-    tx = tq + obj.k;
-    ti = (int*)(tx + obj.k);
-  }
+  typename std::conditional<Obj::TARGETS, Kept<T>, NoKept>::type kept(dyn, entries_per_row(obj));
   pdl_wait();
   if constexpr (CLUSTER) cluster_sync();  // every block's shared memory is there before another writes to it
   const long long step = gridDim.x / blocks;
@@ -857,14 +965,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
     int l = -1;
     Stat<T> st;
     typename std::conditional<Obj::TARGETS, EntriesPart, int>::type part{};
+    typename AheadOf<Obj>::type ahead{};
     bool zero = !now.live();
     if (now.live()) {
       if constexpr (Obj::TARGETS) {
-        // Before any of the gradient is written, which may be in the logits' place.
-        if (warp == 0) {
-          part = obj.prepare(r, xr, x.v, lane, ti, tq, tx);
-          if (lane == 0) entries = part.some;
-        }
+        if (warp == 0) ahead = obj.ahead(r, xr, x.v, lane);
       } else {
         l = (int)clamp_label(now.label, x.v);
         xl = xr[l];
@@ -878,6 +983,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
         const T m = Num<T>::most(a.m, b.m);
         a.s = a.s * Num<T>::exps(a.m - base(m), k) + b.s * Num<T>::exps(b.m - base(m), k);
         a.m = m;
+      }
+      if constexpr (Obj::TARGETS) {
+        // Before any of the gradient is written, which may be in the logits' place.
+        if (warp == 0) {
+          part = obj.prepare(r, xr, x.v, lane, ahead, kept.at, kept.q, kept.x);
+          kept.fill((int)obj.k, lane);
+          if (lane == 0) entries = part.some;
+        }
       }
       const Stat<T> of_warp = join<32>(a, k);
       if (lane == 0) table.slot[half][warp] = pair(of_warp);
@@ -921,16 +1034,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
       if (!zero) {
         const int lo = begin * VEC - row.off, hi = (begin + slice) * VEC - row.off;
         for (int i = threadIdx.x; i < (int)obj.k; i += NT) {
-          const int at = ti[i];
-          if (at < lo || at >= hi) continue;
-          T sum = (T)0;
-          bool leads = true;
-          for (int o = 0; o < (int)obj.k; ++o) {
-            const bool same = ti[o] == at;
-            leads = leads && !(same && o < i);
-            sum += same ? tq[o] : (T)0;
-          }
-          if (leads) gr[at] = Num<T>::exps(tx[i] - m_all, k) * f - c * sum;
+          const int at = kept.at[i];
+          T sum;
+          if (at >= lo && at < hi && kept.leads(i, (int)obj.k, &sum)) gr[at] = Num<T>::exps(kept.x[i] - m_all, k) * f - c * sum;
         }
       }
       if (rank == 0 && warp == 0 && lane == 0) {
@@ -948,18 +1054,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
 
 // ---- sums in a fixed order ----
 
+// sh: one of each of the block's warps.
 __device__ double block_sum(double v, double* sh) {
+  const int lane = threadIdx.x % 32;
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
   __syncthreads();
-  if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = v;
+  if (lane == 0) sh[threadIdx.x / 32] = v;
   __syncthreads();
-  double r = 0;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) r += sh[w];
-  return r;
+  v = lane < (int)blockDim.x / 32 ? sh[lane] : 0.0;
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  return v;
 }
 
-// A cluster's blocks, or one block, add up the terms: eight of a thread at a time, then threads, warps and blocks in order.
-constexpr int SUM_THREADS = 512, SUM_CLUSTER = 8;
+// A cluster's blocks, or one block, add up the terms: sixteen of a thread at a time, then threads, warps and blocks in order.
+constexpr int SUM_THREADS = 1024, SUM_CLUSTER = 8, SUM_AHEAD = 16;
 template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms(const T* __restrict__ terms, long long n, T* loss, double scale) {
   pdl_wait();
   __shared__ double sh[SUM_THREADS / 32];
@@ -969,14 +1077,15 @@ template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms
   double v = 0;
   const long long step = (long long)blocks * SUM_THREADS;
   long long i = (long long)rank * SUM_THREADS + threadIdx.x;
-  for (; i + 7 * step < n; i += 8 * step) {
-    T z[8];
+  for (; i < n; i += SUM_AHEAD * step) {
+    T z[SUM_AHEAD];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) z[q] = terms[i + q * step];
+    for (int q = 0; q < SUM_AHEAD; ++q) z[q] = i + q * step < n ? terms[i + q * step] : (T)0;
+    double part[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v += (double)z[q];
+    for (int q = 0; q < SUM_AHEAD; ++q) part[q % 4] += (double)z[q];
+    v += (part[0] + part[1]) + (part[2] + part[3]);
   }
-  for (; i < n; i += step) v += (double)terms[i];
   v = block_sum(v, sh);
   if (blocks > 1) {
     if (threadIdx.x == 0) put_remote(&of_block[rank], 0u, Pair<double>{v, 0.0});
@@ -988,37 +1097,58 @@ template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms
   if (rank == 0 && threadIdx.x == 0) *loss = (T)(v * scale);
 }
 
-// Block k: pair k's sequence sums, margin, loss term and the coefficients of its two sequences.
-constexpr int PAIR_THREADS = 256;
-template <typename T>
+// The pairs, a warp for each (or a block, LONG), over the warps (blocks) of a cluster or one block: both sequences' sums, the margin, the
+// loss term and the coefficients of the two sequences; then the mean of the terms.
+constexpr int PAIR_THREADS = 512;
+template <typename T, bool LONG>
 __global__ void __launch_bounds__(PAIR_THREADS) k_pairs(const T* __restrict__ token_logp, const T* __restrict__ weight, const T* __restrict__ ref,
-                                                        long long pairs, long long length, double beta, double smoothing, T* terms, T* coef, T* margins,
-                                                        T* logp) {
+                                                        long long pairs, long long length, double beta, double smoothing, T* coef, T* margins, T* logp,
+                                                        T* loss) {
   pdl_wait();
   __shared__ double sh[PAIR_THREADS / 32];
-  const long long k = blockIdx.x;
-  double total[2];
-  for (int side = 0; side < 2; ++side) {
-    const long long at = (k + side * pairs) * length;
-    double v = 0;
-    for (long long t = threadIdx.x; t < length; t += PAIR_THREADS)
-      if (weight[at + t] != (T)0) v += (double)weight[at + t] * (double)token_logp[at + t];
-    total[side] = block_sum(v, sh);
+  __shared__ Pair<double> of_block[SUM_CLUSTER];
+  const unsigned rank = cluster_rank(), blocks = cluster_size();
+  if (blocks > 1) cluster_sync();
+  constexpr int TEAM = LONG ? PAIR_THREADS : 32, TEAMS = PAIR_THREADS / TEAM;
+  const int lane = threadIdx.x % TEAM;
+  double terms = 0;
+  for (long long k = (long long)rank * TEAMS + threadIdx.x / TEAM; k < pairs; k += (long long)blocks * TEAMS) {
+    double total[2] = {0, 0};
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const long long at = (k + side * pairs) * length;
+#pragma unroll 4
+      for (long long t = lane; t < length; t += TEAM) {
+        const T w = weight[at + t], lp = w != (T)0 ? token_logp[at + t] : (T)0;
+        total[side] += (double)w * (double)lp;
+      }
+      if constexpr (LONG) {
+        total[side] = block_sum(total[side], sh);
+      } else {
+        for (int d = 16; d; d >>= 1) total[side] += __shfl_xor_sync(~0u, total[side], d);
+      }
+    }
+    const double h = beta * ((total[0] - (double)ref[k]) - (total[1] - (double)ref[pairs + k]));
+    const double e = exp(-fabs(h)), up = h >= 0 ? 1 / (1 + e) : e / (1 + e), down = h >= 0 ? e / (1 + e) : 1 / (1 + e);
+    const double tail = log1p(e);
+    // -log sigma(h) = tail + max(-h, 0), -log sigma(-h) = tail + max(h, 0)
+    if (lane == 0) terms += h != h ? h : (1 - smoothing) * (tail + (h < 0 ? -h : 0)) + smoothing * (tail + (h > 0 ? h : 0));
+    const double dh = beta * (smoothing * up - (1 - smoothing) * down) / (double)pairs;
+    if (lane < 2) {
+      coef[k + lane * pairs] = (T)(lane ? -dh : dh);
+      if (logp) logp[k + lane * pairs] = (T)total[lane];
+      if (margins && lane == 0) margins[k] = (T)h;
+    }
   }
-  if (threadIdx.x) return;
-  const double h = beta * ((total[0] - (double)ref[k]) - (total[1] - (double)ref[pairs + k]));
-  const double e = exp(-fabs(h)), up = h >= 0 ? 1 / (1 + e) : e / (1 + e), down = h >= 0 ? e / (1 + e) : 1 / (1 + e);
-  const double tail = log1p(e);
-  // -log sigma(h) = tail + max(-h, 0), -log sigma(-h) = tail + max(h, 0)
-  terms[k] = h != h ? (T)h : (T)((1 - smoothing) * (tail + (h < 0 ? -h : 0)) + smoothing * (tail + (h > 0 ? h : 0)));
-  const double dh = beta * (smoothing * up - (1 - smoothing) * down) / (double)pairs;
-  coef[k] = (T)dh;
-  coef[pairs + k] = (T)-dh;
-  if (margins) margins[k] = (T)h;
-  if (logp) {
-    logp[k] = (T)total[0];
-    logp[pairs + k] = (T)total[1];
+  terms = block_sum(terms, sh);
+  if (blocks > 1) {
+    if (threadIdx.x == 0) put_remote(&of_block[rank], 0u, Pair<double>{terms, 0.0});
+    cluster_sync();
+    if (rank != 0) return;
+    terms = 0;
+    for (unsigned b = 0; b < blocks; ++b) terms += of_block[b].m;
   }
+  if (loss && rank == 0 && threadIdx.x == 0) *loss = (T)(terms / (double)pairs);
 }
 
 // ---- host side ----
@@ -1083,19 +1213,16 @@ template <typename K> long long resident(K* kernel, int threads, size_t smem, un
 
 long long pieces_of(long long n, long long of) { return (n + of - 1) / of; }
 
-// Blocks per row: the fewest that hold it (`most` vectors each), and more when the rows alone would
-// leave SMs without work, down to `least` vectors each.
-unsigned split(long long rows, long long vectors, long long most, long long least) {
+// Blocks per row: more than one when the rows alone would leave SMs without work, down to 512 vectors each.
+unsigned split(long long rows, long long vectors) {
   unsigned c = 1;
-  while (c < MAX_CLUSTER && pieces_of(vectors, c) > most) c *= 2;
-  while (c < MAX_CLUSTER && rows * c * 2 <= sm_count() && vectors / (2 * c) >= least) c *= 2;
+  while (c < MAX_CLUSTER && rows * c * 2 <= 4 * sm_count() && vectors / (2 * c) >= 512) c *= 2;
   return c;
 }
 
-template <typename K, typename T, class Obj>
-cudaError_t go_group(K* kernel, long long rows_per_warp, const RowView& x, const Obj& obj, T k, const RowOut& g, size_t smem, cudaStream_t s) {
+template <typename K, typename... A> cudaError_t go_group(K* kernel, long long rows_per_warp, size_t smem, const RowView& x, cudaStream_t s, A... args) {
   const long long warps = pieces_of(x.rows(), rows_per_warp), blocks = std::min(pieces_of(warps, GROUP_THREADS / 32), resident(kernel, GROUP_THREADS, smem, 1));
-  return launch(kernel, dim3((unsigned)blocks), dim3(GROUP_THREADS), smem, 1, s, view<T>(x), x.rows(), obj, k, out<T>(x, g));
+  return launch(kernel, dim3((unsigned)blocks), dim3(GROUP_THREADS), smem, 1, s, args...);
 }
 
 // Rows of at most 512 vectors, by the fewest lanes that hold one; up to 16 vectors a lane in all.
@@ -1103,18 +1230,25 @@ constexpr long long GROUP_VECTORS = 512;
 template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, const Obj& obj, T k, const RowOut& g, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
   if constexpr (Obj::TARGETS) {
-    const int e = v <= 32 ? 1 : v <= 64 ? 2 : v <= 128 ? 4 : v <= 256 ? 8 : 16;
-    const size_t smem = (GROUP_THREADS / 32) * ((e * 32 * Num<T>::VEC + 2 * (size_t)obj.k) * sizeof(T) + (size_t)obj.k * sizeof(int));
-    auto go = [&](auto* kernel) { return go_group(kernel, 1, x, obj, k, g, smem, s); };
-    switch (e) {
-      case 1: return go(k_group_targets<T, 1, Obj, GRAD>);
-      case 2: return go(k_group_targets<T, 2, Obj, GRAD>);
-      case 4: return go(k_group_targets<T, 4, Obj, GRAD>);
-      case 8: return go(k_group_targets<T, 8, Obj, GRAD>);
-      default: return go(k_group_targets<T, 16, Obj, GRAD>);
+    int gk = 1;
+    while (gk < 32 && gk < (int)obj.k) gk *= 2;
+    const bool many = obj.k > 32;
+    const size_t smem = many && GRAD ? GROUP_THREADS / 32 * kept_bytes<T>((size_t)obj.k) : 0;
+    auto go = [&](auto* kernel, int rows) { return go_group(kernel, rows, smem, x, s, view<T>(x), x.rows(), obj, k, out<T>(x, g), gk); };
+    if (many) {
+      if (v <= 32) return go(k_group_targets<T, 32, 1, 1, true, Obj, GRAD>, 1);
+      if (v <= 128) return go(k_group_targets<T, 32, 4, 1, true, Obj, GRAD>, 1);
+      return go(k_group_targets<T, 32, 16, 1, true, Obj, GRAD>, 1);
     }
+    if (v <= 8) return go(k_group_targets<T, 8, 1, 2, false, Obj, GRAD>, 8);
+    if (v <= 16) return go(k_group_targets<T, 8, 2, 2, false, Obj, GRAD>, 8);
+    if (v <= 32) return go(k_group_targets<T, 8, 4, 2, false, Obj, GRAD>, 8);
+    if (v <= 64) return go(k_group_targets<T, 16, 4, 2, false, Obj, GRAD>, 4);
+    if (v <= 128) return go(k_group_targets<T, 32, 4, 2, false, Obj, GRAD>, 2);
+    if (v <= 256) return go(k_group_targets<T, 32, 8, 1, false, Obj, GRAD>, 1);
+    return go(k_group_targets<T, 32, 16, 1, false, Obj, GRAD>, 1);
   } else {
-    auto go = [&](auto* kernel, int rows) { return go_group(kernel, rows, x, obj, k, g, 0, s); };
+    auto go = [&](auto* kernel, int rows) { return go_group(kernel, rows, 0, x, s, view<T>(x), x.rows(), obj, k, out<T>(x, g)); };
     if (v <= 8) return go(k_group<T, 8, 1, 8, Obj, GRAD>, 32);
     if (v <= 16) return go(k_group<T, 8, 2, 8, Obj, GRAD>, 32);
     if (v <= 24) return go(k_group<T, 8, 3, 5, Obj, GRAD>, 20);
@@ -1127,15 +1261,15 @@ template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, 
   }
 }
 
-template <class Obj> size_t target_bytes(const Obj& obj, size_t es, int halves) {
-  if constexpr (Obj::TARGETS) return halves * (size_t)obj.k * (2 * es + sizeof(int));
+template <typename T, class Obj> size_t target_bytes(const Obj& obj) {
+  if constexpr (Obj::TARGETS) return kept_bytes<T>((size_t)obj.k);
   else return 0;
 }
 
 template <typename T, int NT, bool CLUSTER, class Obj>
 cudaError_t go_rows(const RowView& x, const Obj& obj, T k, const RowOut& g, long long slice, unsigned cluster, cudaStream_t s) {
   auto* kernel = k_rows<T, NT, CLUSTER, Obj>;
-  const size_t smem = target_bytes(obj, sizeof(T), 1);
+  const size_t smem = target_bytes<T>(obj);
   const long long clusters = std::min(x.rows(), resident(kernel, NT, smem, cluster));
   return launch(kernel, dim3((unsigned)(clusters * cluster)), dim3(NT), smem, cluster, s, view<T>(x), x.rows(), obj, k, out<T>(x, g), (int)slice);
 }
@@ -1144,7 +1278,7 @@ constexpr long long L2_ROWS_BYTES = 64ll << 20;
 // Rows with a gradient that no group holds.
 template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& obj, T k, const RowOut& g, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
-  unsigned c = split(x.rows(), v, v, 512);
+  unsigned c = split(x.rows(), v);
   // Rows under way at once that do not fit the L2 (its two halves hold copies of what the other half's SMs read):
   // fewer, each by a cluster.
   if (c == 1 && v * 16 * 2 * sm_count() > L2_ROWS_BYTES)
@@ -1162,7 +1296,7 @@ template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& 
 
 template <typename T, class Obj> cudaError_t stream(const RowView& x, const Obj& obj, T k, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
-  const unsigned c = split(x.rows(), v, v, 512);
+  const unsigned c = split(x.rows(), v);
   const long long slice = pieces_of(v, c);
   if (c == 1) {
     auto* kernel = k_stream<T, false, Obj>;
@@ -1196,17 +1330,22 @@ template <typename T> cudaError_t given_grad(const RowView& x, const GivenRow<T>
 }
 
 template <typename T> cudaError_t sum_terms(const void* terms, long long n, void* loss, double scale, cudaStream_t s) {
-  const unsigned blocks = n > 8 * SUM_THREADS ? SUM_CLUSTER : 1;
+  const unsigned blocks = n > SUM_AHEAD * SUM_THREADS ? SUM_CLUSTER : 1;
   return launch(k_sum_terms<T>, dim3(blocks), dim3(SUM_THREADS), 0, blocks, s, (const T*)terms, n, (T*)loss, scale);
+}
+
+// weight: null, or rows with weight 0 are not read and give nothing.
+template <typename T> cudaError_t log_prob_rows(const RowView& x, const int32_t* labels, const T* weight, T* logp, T* stats, cudaStream_t s) {
+  const LogProbRow<T> obj{labels, weight, logp, stats};
+  if (x.rows() == 0) return cudaSuccess;
+  const T k = Num<T>::factor(1.0);
+  return most_vectors<T>(x) <= GROUP_VECTORS ? group<T, LogProbRow<T>, false>(x, obj, k, RowOut{}, s) : stream<T, LogProbRow<T>>(x, obj, k, s);
 }
 
 }  // namespace
 
 template <typename T> cudaError_t Objectives<T>::log_prob(const RowView& x, const int32_t* labels, void* logp, void* stats, cudaStream_t s) {
-  const LogProbRow<T> obj{labels, (T*)logp, (T*)stats};
-  if (x.rows() == 0) return cudaSuccess;
-  const T k = Num<T>::factor(1.0);
-  return most_vectors<T>(x) <= GROUP_VECTORS ? group<T, LogProbRow<T>, false>(x, obj, k, RowOut{}, s) : stream<T, LogProbRow<T>>(x, obj, k, s);
+  return log_prob_rows<T>(x, labels, nullptr, (T*)logp, (T*)stats, s);
 }
 
 template <typename T>
@@ -1235,17 +1374,21 @@ template <typename T>
 cudaError_t Objectives<T>::preference(const RowView& x, const int32_t* labels, const PreferenceArgs& a, void* loss, void* margins, void* logp, const RowOut& g,
                          void* workspace, cudaStream_t s) {
   const long long rows = x.rows(), pairs = x.outer / 2;
-  T* token = (T*)workspace;     // rows
-  T* stats = token + rows;      // 2 * rows
-  T* terms = stats + 2 * rows;  // pairs
-  T* coef = terms + pairs;      // 2 * pairs
-  cudaError_t e = log_prob(x, labels, token, stats, s);
-  if (e == cudaSuccess && pairs > 0)
-    e = launch(k_pairs<T>, dim3((unsigned)pairs), dim3(PAIR_THREADS), 0, 1, s, (const T*)token, (const T*)a.weight, (const T*)a.ref_logp, pairs, x.inner,
-               a.beta, a.smoothing, terms, coef, (T*)margins, (T*)logp);
-  if (e == cudaSuccess && loss) e = sum_terms<T>(terms, pairs, loss, pairs ? 1.0 / (double)pairs : 0.0, s);
+  T* token = (T*)workspace;    // rows
+  T* stats = token + rows;     // 2 * rows
+  T* coef = stats + 2 * rows;  // 2 * pairs
+  const T* weight = (const T*)a.weight;
+  cudaError_t e = log_prob_rows<T>(x, labels, weight, token, stats, s);
+  if (e == cudaSuccess) {
+    auto go = [&](auto* kernel, long long at_once) {
+      return launch(kernel, dim3(pairs > at_once ? SUM_CLUSTER : 1), dim3(PAIR_THREADS), 0, pairs > at_once ? SUM_CLUSTER : 1, s, (const T*)token, weight,
+                    (const T*)a.ref_logp, pairs, x.inner, a.beta, a.smoothing, coef, (T*)margins, (T*)logp, (T*)loss);
+    };
+    // A warp's loads under way hold 128 tokens of a sequence.
+    e = x.inner > 256 ? go(k_pairs<T, true>, 1) : go(k_pairs<T, false>, PAIR_THREADS / 32);
+  }
   if (e == cudaSuccess && g.data)
-    e = given_grad<T>(x, GivenRow<T>{labels, stats, nullptr, coef, (const T*)a.weight, make_fdiv((unsigned long long)std::max<long long>(x.inner, 1))}, g, s);
+    e = given_grad<T>(x, GivenRow<T>{labels, stats, nullptr, coef, weight, make_fdiv((unsigned long long)std::max<long long>(x.inner, 1))}, g, s);
   return e;
 }
 
