@@ -354,7 +354,8 @@ template <typename T> struct GivenRow {
       q.w = q.c = by_row[r];
     } else {
       q.w = weight[r];
-      q.c = q.live() ? by_sequence[quotient((unsigned)r, length)] * q.w : (T)0;
+      const T c = by_sequence[quotient((unsigned)r, length)];
+      q.c = q.live() ? c * q.w : (T)0;
     }
     q.label = labels[r];
     q.m = stats[2 * r];
@@ -366,14 +367,16 @@ template <typename T> struct GivenRow {
   __device__ __forceinline__ void report(long long, const Meta&, T, Stat<T>) const {}
 };
 
-struct EntriesPart {
-  double a, q, from;
-  bool some;  // the row has entries
+// Some of a row's teacher entries: the largest teacher logit m and the largest logit `from` of the row at them, with
+// e = exp((t - m) / T) the sum s of e and the sum a of e ((t - m) - (x - from)). Without any entry s is 0.
+template <typename T> struct EntriesPart {
+  T m = -(T)INFINITY, from = (T)0;
+  double s = 0, a = 0;
 };
 
-// The distillation: a row's targets are its teacher entries. `prepare` (one warp) gives q at shared arrays
-// and the part of the term that does not need the row's statistics: with z the largest logit of the entries,
-// sum q (log q - log p_i) = sum q (log q - (x_i - z) / T) + ((m - z) / T + log s) sum q.
+// The distillation: a row's targets are its teacher entries. With q = e / s the term is
+// sum q (log q - log p_i) = a / (s T) - log s + (row's m - from) / T + log(row's s).
+// Taken relative to `from`, the logits' own size does not count in the difference of the two sums.
 template <typename T> struct DistillRow {
   static constexpr bool TARGETS = true, GIVEN = false;
   const int32_t* index;
@@ -387,124 +390,102 @@ template <typename T> struct DistillRow {
     T w;
     __device__ __forceinline__ bool live() const { return w != (T)0; }
   };
-  using Part = EntriesPart;
-  __device__ __forceinline__ Meta meta(long long r) const {
-    return {weight[r]};
-  }
+  using Part = EntriesPart<T>;
+  __device__ __forceinline__ Meta meta(long long r) const { return {weight[r]}; }
   __device__ void skip(long long r) const { terms[r] = (T)0; }
-  __device__ __forceinline__ void report(long long r, const Meta& m, Part p, Stat<T> st) const {
-    const double lse = ((double)st.m - p.from) * inverse + (double)Num<T>::ln(st.s);
-    terms[r] = p.some ? (T)((double)m.w * (double)wt * (double)wt * (p.a + lse * p.q)) : (T)0;
-  }
   struct Entry {
     T t, x;
     int at;
+    __device__ __forceinline__ Part part() const {
+      Part p;
+      if (t != neg_inf<T>()) p.m = t, p.from = x, p.s = 1;
+      return p;
+    }
   };
-  // Entry i of row r, whose logits are at x.
-  __device__ __forceinline__ Entry entry(long long r, const T* x, long long v, int i) const {
+  // Entry i of row r, without its logit: that is element `at` of the row.
+  __device__ __forceinline__ Entry entry(long long r, long long v, int i) const {
     Entry e;
     e.t = teacher[r * k + i];
     e.at = (int)clamp_label(index[r * k + i], v);
-    e.x = x[e.at];
     return e;
   }
-  // The entries' loads, two of each lane, before the row's: what they are needed for comes after it.
-  struct Ahead {
-    T t[2], x[2];
-    int at[2];
-  };
-  __device__ __forceinline__ Ahead ahead(long long r, const T* x, long long v, int lane) const {
-    Ahead h;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = lane + 32 * e;
-      const bool on = i < (int)k;
-      h.t[e] = on ? teacher[r * k + i] : neg_inf<T>();
-      h.at[e] = on ? (int)clamp_label(index[r * k + i], v) : 0;
+  // What the n parts of WIDTH neighbouring lanes are together, each lane's own every WIDTH-th of them from `first` on.
+  template <int WIDTH, typename F> __device__ __forceinline__ Part join(int first, int n, F part) const {
+    T top = neg_inf<T>(), far = neg_inf<T>();
+    for (int i = first; i < n; i += WIDTH) {
+      const Part p = part(i);
+      if (p.s == 0) continue;
+      top = Num<T>::most(top, p.m);
+      far = Num<T>::most(far, p.from);
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) h.x[e] = lane + 32 * e < (int)k ? x[h.at[e]] : (T)0;
-    return h;
+    for (int d = WIDTH / 2; d; d >>= 1) {
+      top = Num<T>::most(top, __shfl_xor_sync(~0u, top, d));
+      far = Num<T>::most(far, __shfl_xor_sync(~0u, far, d));
+    }
+    if (!(far > neg_inf<T>() && far < -neg_inf<T>())) far = (T)0;
+    Part all{top, far, 0, 0};
+    for (int i = first; i < n; i += WIDTH) {
+      const Part p = part(i);
+      const T f = Num<T>::exps(p.m - base(top), tk);
+      if (p.s != p.s || (p.s != 0 && f != (T)0)) {  // a NaN stays, whatever its weight
+        all.s += (double)f * p.s;
+        all.a += (double)f * (p.a + p.s * (((double)p.m - (double)top) - ((double)p.from - (double)far)));
+      }
+    }
+#pragma unroll
+    for (int d = WIDTH / 2; d; d >>= 1) {
+      all.s += __shfl_xor_sync(~0u, all.s, d);
+      all.a += __shfl_xor_sync(~0u, all.a, d);
+    }
+    return all;
   }
-  // One warp; x: the row's logits, h: ahead(). Keeps q, the index and its logit of each entry when `at` is given.
-  __device__ Part prepare(long long r, const T* x, long long v, int lane, const Ahead& h, int* at, T* q, T* xk) const {
-    auto get = [&](int i) { return i < 32 ? Entry{h.t[0], h.x[0], h.at[0]} : i < 64 ? Entry{h.t[1], h.x[1], h.at[1]} : entry(r, x, v, i); };
-    Stat<T> st;
-    Part p{0, 0, 0, false};
-    T far = neg_inf<T>();  // the largest logit of the entries
-    for (int i = lane; i < (int)k; i += 32) {
-      const Entry n = get(i);
-      const T m = n.t > st.m ? n.t : st.m;
-      st.s = st.s * Num<T>::exps(st.m - base(m), tk) + Num<T>::exps(n.t - base(m), tk);
-      st.m = m;
-      if (n.t != neg_inf<T>()) far = Num<T>::most(far, n.x);
-    }
-    st = join<32>(st, tk);
-    for (int d = 16; d; d >>= 1) far = Num<T>::most(far, __shfl_xor_sync(~0u, far, d));
-    p.from = far > neg_inf<T>() && far < -neg_inf<T>() ? (double)far : 0.0;
-    p.some = st.s != (T)0;  // all entries -inf: none
-    const T inv = (T)1 / st.s;
-    const double logs = (double)Num<T>::ln(st.s);
-    for (int i = lane; i < (int)k; i += 32) {
-      const Entry n = get(i);
-      const T d = n.t - base(st.m), qi = p.some ? Num<T>::exps(d, tk) * inv : (T)0;
-      if (at) {
-        at[i] = n.at;
-        q[i] = qi;
-        xk[i] = n.x;
-      }
-      if (qi != (T)0) {
-        p.a += (double)qi * (((double)d - ((double)n.x - p.from)) * inverse - logs);
-        p.q += (double)qi;
-      }
-    }
-    for (int d = 16; d; d >>= 1) {
-      p.a += __shfl_xor_sync(~0u, p.a, d);
-      p.q += __shfl_xor_sync(~0u, p.q, d);
-    }
-    return p;
+  // q of an entry with teacher logit t, of all entries' part.
+  __device__ __forceinline__ T share(T t, T m, T inverse_s) const { return Num<T>::exps(t - base(m), tk) * inverse_s; }
+  __device__ __forceinline__ void report(long long r, const Meta& m, const Part& p, Stat<T> st) const {
+    const double term = (p.a / p.s + ((double)st.m - (double)p.from)) * inverse + (double)Num<T>::ln(st.s) - (double)Num<T>::ln((T)p.s);
+    terms[r] = p.s != 0 ? (T)((double)m.w * (double)wt * (double)wt * term) : (T)0;
   }
 };
+constexpr int DISTILL_CHUNKS = DISTILL_MAX_K / 32;  // of 32 entries
+static_assert(DISTILL_CHUNKS <= 32, "a lane per chunk");
 
-// A row's entries in shared memory: the indices (whole vectors of four, the rest -1), the probabilities, the logits.
+// A row's entries in shared memory: the indices (whole vectors of four, what is not an entry negative), the teacher's
+// logits, the row's.
 template <typename T> struct Kept {
   int* at;
-  T *q, *x;
-  __device__ __forceinline__ Kept(unsigned char* p, int k) {
+  T *t, *x;
+  __device__ __forceinline__ Kept(unsigned char* p, int slots) {  // slots: a multiple of four
     at = (int*)p;
-    q = (T*)(p + (k + 3) / 4 * 16);
-    x = q + k;
+    t = (T*)(p + slots * sizeof(int));
+    x = t + slots;
   }
-  __device__ __forceinline__ void fill(int k, int lane) {
-    if (lane < (k + 3) / 4 * 4 - k) at[k + lane] = -1;
-  }
-  // Whether entry i is the first with its index; *sum: the probabilities of all of them, in order. Most are alone.
-  __device__ __forceinline__ bool leads(int i, int k, T* sum) const {
+  // Whether entry i of k is the first with its index; *sum: share(t) of all of them, in order.
+  template <typename F> __device__ __forceinline__ bool leads(int i, int k, T* sum, F share) const {
     const int mine = at[i];
-    int n = 0;
+    *sum = (T)0;
+#pragma unroll 4
     for (int o = 0; o < k; o += 4) {
       const int4 z = *reinterpret_cast<const int4*>(at + o);
-      n += (z.x == mine) + (z.y == mine) + (z.z == mine) + (z.w == mine);
-    }
-    *sum = q[i];
-    if (n == 1) return true;
-    *sum = (T)0;
-    for (int o = 0; o < k; ++o) {
-      if (at[o] != mine) continue;
-      if (o < i) return false;
-      *sum += q[o];
+      if (z.x != mine && z.y != mine && z.z != mine && z.w != mine) continue;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if ((c == 0 ? z.x : c == 1 ? z.y : c == 2 ? z.z : z.w) != mine) continue;
+        if (o + c < i) return false;
+        *sum += share(t[o + c]);
+      }
     }
     return true;
   }
 };
-struct NoKept {
-  __device__ __forceinline__ NoKept(unsigned char*, int) {}
-};
-template <class Obj> __device__ __forceinline__ int entries_per_row(const Obj& obj) {
-  if constexpr (Obj::TARGETS) return (int)obj.k;
-  else return 0;
+template <typename T> size_t kept_bytes(size_t slots) { return slots * (sizeof(int) + 2 * sizeof(T)); }
+
+__device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+// One number from global to shared memory, there for this thread after copies_wait().
+template <typename T> __device__ __forceinline__ void copy_ahead(T* to, const T* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(to)), "l"(from), "n"((int)sizeof(T)) : "memory");
 }
-template <typename T> size_t kept_bytes(size_t k) { return (k + 3) / 4 * 16 + (2 * k * sizeof(T) + 15) / 16 * 16; }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---- short rows: a group of G lanes per row ----
 
@@ -610,21 +591,22 @@ __global__ void __launch_bounds__(GROUP_THREADS, 2) k_group(const View<T> x, con
   }
 }
 
-// The same for the distillation. `gk` lanes take a row's entries, 32 / gk rows at a time, and what they come to goes
-// to the row's lane; with MANY, more than 32 entries, a warp has one row. The gradients at the entries are written a second time, over what the row's
-// lanes have stored; the first entry of an index writes its element, with the probabilities of all of that index.
-template <typename T, int G, int E, int B, bool MANY, class Obj, bool GRAD>
-__global__ void __launch_bounds__(GROUP_THREADS, 2) k_group_targets(const View<T> x, const long long rows, const Obj obj, const T k, const Out<T> g, const int gk) {
-  constexpr int VEC = Num<T>::VEC, R = 32 / G, ROWS = B * R, KEEP = GRAD && !MANY ? ROWS * 32 : 1;
-  static_assert(ROWS <= 32 && (!MANY || ROWS == 1), "a lane per row");
-  __shared__ T keep_q[GROUP_THREADS / 32][KEEP], keep_x[GROUP_THREADS / 32][KEEP];
-  __shared__ int keep_at[GROUP_THREADS / 32][KEEP];
+// The same for the distillation: 32 / ROWS lanes take a row's entries, one after the other, and what they come to goes to the
+// row's lane. The entries reach shared memory while the logits are under way. (With a lane for every entry and 5 steps
+// between lanes for each row, 131072 x 96 with 32 entries took 142 us.)
+// The gradients at the entries are written a second time, over what the row's lanes have stored; the first entry of an
+// index writes its element, with the probabilities of all of that index.
+template <typename T, int G, int E, int B, class Obj, bool GRAD>
+__global__ void __launch_bounds__(GROUP_THREADS, 2) k_group_targets(const View<T> x, const long long rows, const Obj obj, const T k, const Out<T> g, const int slots) {
+  constexpr int VEC = Num<T>::VEC, R = 32 / G, ROWS = B * R, TEAM = 32 / ROWS;
+  static_assert(ROWS <= 32, "a lane per row");
   extern __shared__ __align__(16) unsigned char dyn[];
   pdl_wait();
-  const int lane = threadIdx.x % 32, in_group = lane % G, group = lane / G, i = lane % gk, of = lane / gk, at_once = 32 / gk;
-  T *kq = keep_q[threadIdx.x / 32], *kx = keep_x[threadIdx.x / 32];
-  int* ka = keep_at[threadIdx.x / 32];
-  Kept<T> kept(dyn + (MANY && GRAD ? threadIdx.x / 32 * ((obj.k + 3) / 4 * 16 + (2 * obj.k * sizeof(T) + 15) / 16 * 16) : 0), (int)obj.k);
+  const int lane = threadIdx.x % 32, in_group = lane % G, group = lane / G, mate = lane % TEAM, of = lane / TEAM, entries = (int)obj.k;
+  // Of this lane's row of entries.
+  const Kept<T> kept(dyn + (threadIdx.x / 32 * ROWS + of) * slots * (sizeof(int) + 2 * sizeof(T)), slots);
+  if (mate == 0) *reinterpret_cast<int4*>(kept.at + (entries - 1) / 4 * 4) = make_int4(-1, -1, -1, -1);  // behind the entries
+  __syncwarp();
   const long long warps = (long long)gridDim.x * (GROUP_THREADS / 32);
   for (long long w = (long long)blockIdx.x * (GROUP_THREADS / 32) + threadIdx.x / 32; w * ROWS < rows; w += warps) {
     const long long row0 = w * ROWS, mine = row0 + lane;
@@ -633,14 +615,11 @@ __global__ void __launch_bounds__(GROUP_THREADS, 2) k_group_targets(const View<T
     if (in) meta = obj.meta(mine);
     const bool live = in && meta.live();
     const unsigned lives = __ballot_sync(~0u, live);
-    auto fetch = [&](int j) {  // this lane's entry of row j of the warp's
-      if (j < ROWS && i < (int)obj.k && (lives >> j & 1)) return obj.entry(row0 + j, x.row(row0 + j), x.v, i);
-      return typename Obj::Entry{neg_inf<T>(), (T)0, -1 - lane};
-    };
-    typename Obj::Entry next;
-    typename Obj::Ahead ahead;
-    if constexpr (!MANY) next = fetch(of);
-    else if (lives) ahead = obj.ahead(row0, x.row(row0), x.v, lane);
+    const bool fed = lives >> of & 1;
+    for (int i = mate; fed && i < entries; i += TEAM) {
+      copy_ahead(kept.t + i, obj.teacher + (row0 + of) * obj.k + i);
+      copy_ahead(kept.at + i, obj.index + (row0 + of) * obj.k + i);
+    }
     T y[B][E * VEC], most[B];
 #pragma unroll
     for (int b = 0; b < B; ++b) {
@@ -654,38 +633,11 @@ __global__ void __launch_bounds__(GROUP_THREADS, 2) k_group_targets(const View<T
         for (int q = 0; q < E * VEC; ++q) y[b][q] = neg_inf<T>();
       }
     }
-    typename Obj::Part part{0, 0, 0, false};
-    if constexpr (MANY) {
-      if (lives) part = obj.prepare(row0, x.row(row0), x.v, lane, ahead, GRAD ? kept.at : nullptr, kept.q, kept.x);
-      if (GRAD) kept.fill((int)obj.k, lane);
-    }
-    for (int j0 = 0; !MANY && j0 < ROWS; j0 += at_once) {
-      const typename Obj::Entry now = next;
-      next = fetch(j0 + at_once + of);
-      T top = now.t != now.t ? neg_inf<T>() : now.t, far = now.t != neg_inf<T>() ? Num<T>::most(now.x, neg_inf<T>()) : neg_inf<T>();
-      for (int d = gk / 2; d; d >>= 1) {
-        top = Num<T>::most(top, __shfl_xor_sync(~0u, top, d));
-        far = Num<T>::most(far, __shfl_xor_sync(~0u, far, d));
-      }
-      const T from = far > neg_inf<T>() && far < -neg_inf<T>() ? far : (T)0, dt = now.t - base(top), e = Num<T>::exps(dt, obj.tk);
-      T s = e;
-      for (int d = gk / 2; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-      const T q = s != (T)0 ? e * ((T)1 / s) : (T)0;  // all entries -inf: none
-      double a = q != (T)0 ? (double)q * (((double)dt - ((double)now.x - (double)from)) * obj.inverse - (double)Num<T>::ln(s)) : 0.0, total = (double)q;
-      for (int d = gk / 2; d; d >>= 1) {
-        a += __shfl_xor_sync(~0u, a, d);
-        total += __shfl_xor_sync(~0u, total, d);
-      }
-      const int src = lane % at_once * gk;
-      a = __shfl_sync(~0u, a, src);
-      total = __shfl_sync(~0u, total, src);
-      const T z = __shfl_sync(~0u, from, src);
-      if (lane / at_once == j0 / at_once) part = {a, total, (double)z, total != 0};
-      if constexpr (GRAD) {
-        kq[j0 * gk + lane] = q;
-        kx[j0 * gk + lane] = now.x;
-        ka[j0 * gk + lane] = now.at;
-      }
+    copies_wait();
+    for (int i = mate; fed && i < entries; i += TEAM) {
+      const int at = (int)clamp_label(kept.at[i], x.v);
+      kept.at[i] = at;
+      copy_ahead(kept.x + i, x.row(row0 + of) + at);
     }
     Stat<T> st;
 #pragma unroll
@@ -696,10 +648,14 @@ __global__ void __launch_bounds__(GROUP_THREADS, 2) k_group_targets(const View<T
       const T m = __shfl_sync(~0u, all.m, lane % R * G), s = __shfl_sync(~0u, all.s, lane % R * G);
       if (lane / R == b) st = {m, s};
     }
-    const bool some = live && part.some;
+    copies_wait();
+    typename Obj::Part part = obj.template join<TEAM>(mate, fed ? entries : 0, [&](int i) { return typename Obj::Entry{kept.t[i], kept.x[i], 0}.part(); });
+    const int src = lane % ROWS * TEAM;
+    part = {__shfl_sync(~0u, part.m, src), __shfl_sync(~0u, part.from, src), __shfl_sync(~0u, part.s, src), __shfl_sync(~0u, part.a, src)};
+    const bool some = live && part.s != 0;
     if constexpr (GRAD) {
       const unsigned somes = __ballot_sync(~0u, some);
-      const T c = some ? meta.w * obj.wt : (T)0, scale = some ? c / st.s : (T)0;
+      const T c = some ? meta.w * obj.wt : (T)0, scale = some ? c / st.s : (T)0, inverse_s = (T)1 / (T)part.s;
 #pragma unroll
       for (int b = 0; b < B; ++b) {
         const int at = (b * R + group) % 32;
@@ -712,26 +668,17 @@ __global__ void __launch_bounds__(GROUP_THREADS, 2) k_group_targets(const View<T
         store_group<T, G, E>(g.row(r), Span<T>(x.row(r), have ? x.v : 0), in_group, y[b]);
       }
       __syncwarp();
-      const unsigned ours = (gk == 32 ? ~0u : (1u << gk) - 1) << (of * gk);
-      if constexpr (MANY) {
-        const T sc = __shfl_sync(~0u, scale, 0), cj = __shfl_sync(~0u, c, 0), m = __shfl_sync(~0u, st.m, 0);
-        for (int e = lane; somes && e < (int)obj.k; e += 32) {
+      const T sc = __shfl_sync(~0u, scale, of), cj = __shfl_sync(~0u, c, of), m = __shfl_sync(~0u, st.m, of);
+      const T top = __shfl_sync(~0u, part.m, of), inv = __shfl_sync(~0u, inverse_s, of);
+      if (somes >> of & 1) {
+        T* gr = g.row(row0 + of);
+        for (int i = mate; i < entries; i += TEAM) {
           T sum;
-          if (kept.leads(e, (int)obj.k, &sum)) g.row(row0)[kept.at[e]] = Num<T>::exps(kept.x[e] - m, k) * sc - cj * sum;
+          if (kept.leads(i, entries, &sum, [&](T z) { return obj.share(z, top, inv); })) gr[kept.at[i]] = Num<T>::exps(kept.x[i] - m, k) * sc - cj * sum;
         }
       }
-      for (int j0 = 0; !MANY && j0 < ROWS; j0 += at_once) {
-        const int j = j0 + of, at = ka[j0 * gk + lane];
-        unsigned same = __match_any_sync(~0u, at) & ours;
-        const T sc = __shfl_sync(~0u, scale, j % 32), cj = __shfl_sync(~0u, c, j % 32), m = __shfl_sync(~0u, st.m, j % 32);
-        if (j < ROWS && i < (int)obj.k && (somes >> j & 1) && (same & ((1u << lane) - 1)) == 0) {
-          T sum = (T)0;
-          for (; same; same &= same - 1) sum += kq[j0 * gk + __ffs(same) - 1];
-          g.row(row0 + j)[at] = Num<T>::exps(kx[j0 * gk + lane] - m, k) * sc - cj * sum;
-        }
-      }
-      __syncwarp();  // the kept entries are read before the next rows'
     }
+    __syncwarp();  // the kept entries are read before the next rows'
     if (in) {
       if (live) obj.report(mine, meta, part, st);
       else obj.skip(mine);
@@ -741,7 +688,6 @@ __global__ void __launch_bounds__(GROUP_THREADS, 2) k_group_targets(const View<T
 
 // ---- longer rows: a block, or a cluster of blocks, per row ----
 
-__device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ unsigned cluster_rank() {
   unsigned r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -786,11 +732,56 @@ template <typename T, int N> struct Table {
 };
 template <typename T> __device__ __forceinline__ Pair<T> pair(Stat<T> a) { return {a.m, a.s}; }
 
-template <class Obj, bool TARGETS = Obj::TARGETS> struct AheadOf {
-  struct type {};
+// What a block's threads do with a row's entries, if the objective has any: entry threadIdx.x of the first NT is loaded before
+// the row's logits (its own logit between them, when the index is there), the others after them.
+template <typename T, int NT, class Obj, bool TARGETS = Obj::TARGETS> struct Entries {
+  struct Slots {};
+  __device__ __forceinline__ Entries(const Obj&, long long, const T*, long long, bool) {}
+  __device__ __forceinline__ void gather() {}
 };
-template <class Obj> struct AheadOf<Obj, true> {
-  using type = typename Obj::Ahead;
+template <typename T, int NT, class Obj> struct Entries<T, NT, Obj, true> {
+  using Part = typename Obj::Part;
+  struct Slots {
+    Part of[2][DISTILL_CHUNKS];  // of 32 entries each
+    // By a warp: all entries.
+    __device__ __forceinline__ Part read(const Obj& obj, int half) const {
+      return obj.template join<32>((int)threadIdx.x % 32, ((int)obj.k + 31) / 32, [&](int i) { return of[half][i]; });
+    }
+  };
+  const Obj& obj;
+  const long long r, v;
+  const T* x;
+  bool on;
+  typename Obj::Entry first{neg_inf<T>(), (T)0, -1};
+  __device__ __forceinline__ Entries(const Obj& o, long long row, const T* logits, long long vocab, bool live) : obj(o), r(row), v(vocab), x(logits), on(live) {
+    if (on && (int)threadIdx.x < (int)obj.k) first = obj.entry(r, v, (int)threadIdx.x);
+  }
+  __device__ __forceinline__ void gather() {
+    if (on && (int)threadIdx.x < (int)obj.k) first.x = x[first.at];
+  }
+  // Leaves the parts in `slots` and, if kept, the entries there. Whether this thread has any.
+  __device__ __forceinline__ bool finish(Slots& slots, int half, const Kept<T>* kept) {
+    bool some = false;
+    for (int i = (int)threadIdx.x; i / 32 * 32 < (int)obj.k; i += NT) {
+      typename Obj::Entry n{neg_inf<T>(), (T)0, -1};
+      if (i < NT) {
+        n = first;
+      } else if (i < (int)obj.k) {
+        n = obj.entry(r, v, i);
+        n.x = x[n.at];
+      }
+      if (kept && i < ((int)obj.k + 3) / 4 * 4) {
+        kept->at[i] = n.at;
+        kept->t[i] = n.t;
+        kept->x[i] = n.x;
+      }
+      const int lane = (int)threadIdx.x % 32;
+      const Part p = obj.template join<32>(lane, lane + 1, [&](int) { return n.part(); });
+      if (lane == 0) slots.of[half][i / 32] = p;
+      some = some || p.s != 0;
+    }
+    return some;
+  }
 };
 
 // ---- longer rows without a gradient ----
@@ -803,6 +794,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
   constexpr int VEC = Num<T>::VEC, NT = STREAM_THREADS, U = STREAM_UNROLL;
   __shared__ Table<T, NT / 32> table;
   __shared__ Table<T, CLUSTER ? MAX_CLUSTER : 1> shares;
+  __shared__ typename Entries<T, NT, Obj>::Slots slots;
   const unsigned rank = CLUSTER ? cluster_rank() : 0, blocks = CLUSTER ? cluster_size() : 1;
   const long long step = gridDim.x / blocks;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, begin = (int)rank * slice;
@@ -823,10 +815,8 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
     Span<T> row(x.row(r), x.v);
     row.clip(begin, begin + slice);
     T xl = (T)0;
-    typename AheadOf<Obj>::type ahead{};
-    if constexpr (Obj::TARGETS) {
-      if (reports) ahead = obj.ahead(r, x.row(r), x.v, lane);
-    } else {
+    Entries<T, NT, Obj> entries(obj, r, x.row(r), x.v, rank == 0);
+    if constexpr (!Obj::TARGETS) {
       if (reports && lane == 0) xl = x.row(r)[clamp_label(now.label, x.v)];
     }
     Stat<T> a;
@@ -834,10 +824,17 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
       T y[U * VEC];
 #pragma unroll
       for (int u = 0; u < U; ++u) row.load(i + NT * u, y + u * VEC);
+      if (i < begin + NT * U) entries.gather();
       const Stat<T> b = exponentials<T, U * VEC>(y, k);
-      const T m = b.m > a.m ? b.m : a.m;
+      const T m = Num<T>::most(a.m, b.m);
       a.s = a.s * Num<T>::exps(a.m - base(m), k) + b.s * Num<T>::exps(b.m - base(m), k);
       a.m = m;
+    }
+    if constexpr (Obj::TARGETS) {
+      if (rank == 0) {
+        if ((begin + (int)threadIdx.x) * VEC >= row.hi) entries.gather();  // no logits for this thread
+        entries.finish(slots, half, nullptr);
+      }
     }
     const Stat<T> of_warp = join<32>(a, k);
     if (lane == 0) table.slot[half][warp] = pair(of_warp);
@@ -855,7 +852,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
     if (reports) {
       const Stat<T> st = CLUSTER ? shares.read(half, (int)blocks, k) : table.read(half, NT / 32, k);
       if constexpr (Obj::TARGETS) {
-        const EntriesPart part = obj.prepare(r, x.row(r), x.v, lane, ahead, nullptr, nullptr, nullptr);
+        const auto part = slots.read(obj, half);
         if (lane == 0) obj.report(r, now, part, st);
       } else {
         if (lane == 0) obj.report(r, now, xl, st);
@@ -868,23 +865,24 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
 
 // ---- gradients from the statistics of an earlier pass ----
 
-// A block computes a piece of NT * U vectors of a row.
-constexpr int GRAD_THREADS = 256;
-template <typename T, int U>
-__global__ void __launch_bounds__(GRAD_THREADS) k_grad(View<T> x, long long rows, GivenRow<T> obj, T k, Out<T> g, int pieces) {
-  constexpr int VEC = Num<T>::VEC, NT = GRAD_THREADS;
+// A warp computes a piece of 64 vectors of a row at a time. Many warps with two vectors a lane under way: with four, 32 instead
+// of 48 warps fit an SM, and 8192 x 8192 took 100 instead of 83 us.
+constexpr int GRAD_THREADS = 256, GRAD_UNROLL = 2, GRAD_VECTORS = 32 * GRAD_UNROLL;
+template <typename T>
+__global__ void __launch_bounds__(GRAD_THREADS, 6) k_grad(View<T> x, long long rows, GivenRow<T> obj, T k, Out<T> g, int pieces) {
+  constexpr int VEC = Num<T>::VEC, U = GRAD_UNROLL;
   pdl_wait();
   const int lane = threadIdx.x % 32;
-  // Piece p of row r; then gridDim.x pieces on.
-  const long long step_r = gridDim.x / (unsigned)pieces;
-  const int step_p = (int)(gridDim.x % (unsigned)pieces);
-  long long r = blockIdx.x / (unsigned)pieces;
-  for (int p = (int)(blockIdx.x % (unsigned)pieces); r < rows; r += step_r + (p + step_p >= pieces), p = p + step_p >= pieces ? p + step_p - pieces : p + step_p) {
-    const int first = p * NT * U;
+  // Piece p of row r; then as many pieces on as there are warps.
+  const unsigned warps = gridDim.x * (GRAD_THREADS / 32), warp = blockIdx.x * (GRAD_THREADS / 32) + threadIdx.x / 32;
+  const long long step_r = warps / (unsigned)pieces;
+  const int step_p = (int)(warps % (unsigned)pieces);
+  long long r = warp / (unsigned)pieces;
+  for (int p = (int)(warp % (unsigned)pieces); r < rows; r += step_r + (p + step_p >= pieces), p = p + step_p >= pieces ? p + step_p - pieces : p + step_p) {
+    const int warp0 = p * GRAD_VECTORS;  // this warp's vectors: warp0 + lane + 32 * u
     const typename GivenRow<T>::Meta q = obj.meta(r);
     Span<T> row(x.row(r), x.v);
-    row.clip(first, first + NT * U);
-    const int warp0 = first + (int)threadIdx.x / 32 * 32 * U;  // this warp's vectors: warp0 + lane + 32 * u
+    row.clip(warp0, warp0 + GRAD_VECTORS);
     T y[U * VEC];
     const bool inside = warp0 * VEC >= row.lo && (warp0 + 32 * U) * VEC <= row.hi;
     if (q.live()) {
@@ -931,10 +929,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Table<T, NW> table;                          // of the block's warps
   __shared__ Table<T, CLUSTER ? MAX_CLUSTER : 1> shares;  // of the cluster's blocks
-  __shared__ int entries;
+  __shared__ typename Entries<T, NT, Obj>::Slots slots;
   const unsigned rank = CLUSTER ? cluster_rank() : 0, blocks = CLUSTER ? cluster_size() : 1;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, begin = (int)rank * slice, first = begin + warp * 32 * U;
-  typename std::conditional<Obj::TARGETS, Kept<T>, NoKept>::type kept(dyn, entries_per_row(obj));
+  int entry_slots = 0;
+  if constexpr (Obj::TARGETS) entry_slots = ((int)obj.k + 3) / 4 * 4;
+  const Kept<T> kept(dyn, entry_slots);
   pdl_wait();
   if constexpr (CLUSTER) cluster_sync();  // every block's shared memory is there before another writes to it
   const long long step = gridDim.x / blocks;
@@ -964,13 +964,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
     T xl = (T)0, c = (T)0, f = (T)0, m_all = (T)0;
     int l = -1;
     Stat<T> st;
-    typename std::conditional<Obj::TARGETS, EntriesPart, int>::type part{};
-    typename AheadOf<Obj>::type ahead{};
     bool zero = !now.live();
     if (now.live()) {
-      if constexpr (Obj::TARGETS) {
-        if (warp == 0) ahead = obj.ahead(r, xr, x.v, lane);
-      } else {
+      Entries<T, NT, Obj> entries(obj, r, xr, x.v, true);
+      if constexpr (!Obj::TARGETS) {
         l = (int)clamp_label(now.label, x.v);
         xl = xr[l];
         l += row.off;
@@ -979,22 +976,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
       for (int e = 0; e < turns; ++e) {
         T y[U * VEC];
         load(first + NT * U * e, y, std::false_type{});
+        if (e == 0) entries.gather();
         const Stat<T> b = exponentials<T, U * VEC>(y, k);
         const T m = Num<T>::most(a.m, b.m);
         a.s = a.s * Num<T>::exps(a.m - base(m), k) + b.s * Num<T>::exps(b.m - base(m), k);
         a.m = m;
       }
+      bool some = false;
       if constexpr (Obj::TARGETS) {
         // Before any of the gradient is written, which may be in the logits' place.
-        if (warp == 0) {
-          part = obj.prepare(r, xr, x.v, lane, ahead, kept.at, kept.q, kept.x);
-          kept.fill((int)obj.k, lane);
-          if (lane == 0) entries = part.some;
-        }
+        if (turns == 0) entries.gather();
+        some = entries.finish(slots, 0, &kept);
       }
       const Stat<T> of_warp = join<32>(a, k);
       if (lane == 0) table.slot[half][warp] = pair(of_warp);
-      __syncthreads();
+      if constexpr (Obj::TARGETS) zero = !__syncthreads_or(some);  // a row without entries counts nothing
+      else __syncthreads();
       st = table.read(half, NW, k);
       if constexpr (CLUSTER) {
         if (warp == 0 && lane < (int)blocks) put_remote(&shares.slot[half][rank], (unsigned)lane, pair(st));
@@ -1002,7 +999,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
         st = shares.read(half, (int)blocks, k);
       }
       if constexpr (Obj::TARGETS) {
-        zero = !entries;  // a row without entries counts nothing
         c = now.w * obj.wt;
         f = c / st.s;
       } else {
@@ -1031,15 +1027,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
       // The entries in this block's slice, over what the block has stored. The first entry of an index writes its
       // element, with the probabilities of all entries of that index in order.
       __syncthreads();
-      if (!zero) {
+      typename Obj::Part part;
+      if (!zero && (warp == 0 || warp * 32 < (int)obj.k)) {
+        part = slots.read(obj, 0);
+        const T inverse_s = (T)1 / (T)part.s;
         const int lo = begin * VEC - row.off, hi = (begin + slice) * VEC - row.off;
         for (int i = threadIdx.x; i < (int)obj.k; i += NT) {
           const int at = kept.at[i];
           T sum;
-          if (at >= lo && at < hi && kept.leads(i, (int)obj.k, &sum)) gr[at] = Num<T>::exps(kept.x[i] - m_all, k) * f - c * sum;
+          if (at >= lo && at < hi && kept.leads(i, (int)obj.k, &sum, [&](T t) { return obj.share(t, part.m, inverse_s); }))
+            gr[at] = Num<T>::exps(kept.x[i] - m_all, k) * f - c * sum;
         }
       }
-      if (rank == 0 && warp == 0 && lane == 0) {
+      if (rank == 0 && threadIdx.x == 0) {
         if (now.live()) obj.report(r, now, part, st);
         else obj.skip(r);
       }
@@ -1230,23 +1230,22 @@ constexpr long long GROUP_VECTORS = 512;
 template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, const Obj& obj, T k, const RowOut& g, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
   if constexpr (Obj::TARGETS) {
-    int gk = 1;
-    while (gk < 32 && gk < (int)obj.k) gk *= 2;
-    const bool many = obj.k > 32;
-    const size_t smem = many && GRAD ? GROUP_THREADS / 32 * kept_bytes<T>((size_t)obj.k) : 0;
-    auto go = [&](auto* kernel, int rows) { return go_group(kernel, rows, smem, x, s, view<T>(x), x.rows(), obj, k, out<T>(x, g), gk); };
-    if (many) {
-      if (v <= 32) return go(k_group_targets<T, 32, 1, 1, true, Obj, GRAD>, 1);
-      if (v <= 128) return go(k_group_targets<T, 32, 4, 1, true, Obj, GRAD>, 1);
-      return go(k_group_targets<T, 32, 16, 1, true, Obj, GRAD>, 1);
+    // Slots for a row's entries: vectors of four, an odd number of them, so that rows begin in different banks.
+    const int slots = ((int)pieces_of(obj.k, 4) | 1) * 4;
+    auto go = [&](auto* kernel, int rows) {
+      return go_group(kernel, rows, GROUP_THREADS / 32 * rows * kept_bytes<T>((size_t)slots), x, s, view<T>(x), x.rows(), obj, k, out<T>(x, g), slots);
+    };
+    if (obj.k <= 64) {  // the entries of several rows to a warp leave room for two blocks to an SM
+      if (v <= 8) return go(k_group_targets<T, 8, 1, 2, Obj, GRAD>, 8);
+      if (v <= 16) return go(k_group_targets<T, 8, 2, 2, Obj, GRAD>, 8);
+      if (v <= 32) return go(k_group_targets<T, 8, 4, 2, Obj, GRAD>, 8);
+      if (v <= 64) return go(k_group_targets<T, 16, 4, 2, Obj, GRAD>, 4);
+      if (v <= 128) return go(k_group_targets<T, 32, 4, 2, Obj, GRAD>, 2);
     }
-    if (v <= 8) return go(k_group_targets<T, 8, 1, 2, false, Obj, GRAD>, 8);
-    if (v <= 16) return go(k_group_targets<T, 8, 2, 2, false, Obj, GRAD>, 8);
-    if (v <= 32) return go(k_group_targets<T, 8, 4, 2, false, Obj, GRAD>, 8);
-    if (v <= 64) return go(k_group_targets<T, 16, 4, 2, false, Obj, GRAD>, 4);
-    if (v <= 128) return go(k_group_targets<T, 32, 4, 2, false, Obj, GRAD>, 2);
-    if (v <= 256) return go(k_group_targets<T, 32, 8, 1, false, Obj, GRAD>, 1);
-    return go(k_group_targets<T, 32, 16, 1, false, Obj, GRAD>, 1);
+    if (v <= 32) return go(k_group_targets<T, 32, 1, 1, Obj, GRAD>, 1);
+    if (v <= 128) return go(k_group_targets<T, 32, 4, 1, Obj, GRAD>, 1);
+    if (v <= 256) return go(k_group_targets<T, 32, 8, 1, Obj, GRAD>, 1);
+    return go(k_group_targets<T, 32, 16, 1, Obj, GRAD>, 1);
   } else {
     auto go = [&](auto* kernel, int rows) { return go_group(kernel, rows, 0, x, s, view<T>(x), x.rows(), obj, k, out<T>(x, g)); };
     if (v <= 8) return go(k_group<T, 8, 1, 8, Obj, GRAD>, 32);
@@ -1262,7 +1261,7 @@ template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, 
 }
 
 template <typename T, class Obj> size_t target_bytes(const Obj& obj) {
-  if constexpr (Obj::TARGETS) return kept_bytes<T>((size_t)obj.k);
+  if constexpr (Obj::TARGETS) return kept_bytes<T>(((size_t)obj.k + 3) / 4 * 4);
   else return 0;
 }
 
@@ -1321,12 +1320,9 @@ template <typename T> cudaError_t given_grad(const RowView& x, const GivenRow<T>
   const T k = Num<T>::factor(1.0);
   const long long v = most_vectors<T>(x);
   if (v <= GROUP_VECTORS) return group<T, GivenRow<T>, true>(x, obj, k, g, s);
-  auto go = [&](auto* kernel, int u) {
-    const long long pieces = pieces_of(v, GRAD_THREADS * u);
-    return launch(kernel, dim3((unsigned)std::min(x.rows() * pieces, resident(kernel, GRAD_THREADS, 0, 1))), dim3(GRAD_THREADS), 0, 1, s, view<T>(x), x.rows(),
-                  obj, k, out<T>(x, g), (int)pieces);
-  };
-  return v <= 2 * GRAD_THREADS ? go(k_grad<T, 2>, 2) : go(k_grad<T, 4>, 4);
+  const long long pieces = pieces_of(v, GRAD_VECTORS), blocks = pieces_of(x.rows() * pieces, GRAD_THREADS / 32);
+  return launch(k_grad<T>, dim3((unsigned)std::min(blocks, resident(k_grad<T>, GRAD_THREADS, 0, 1))), dim3(GRAD_THREADS), 0, 1, s, view<T>(x), x.rows(), obj, k,
+                out<T>(x, g), (int)pieces);
 }
 
 template <typename T> cudaError_t sum_terms(const void* terms, long long n, void* loss, double scale, cudaStream_t s) {
