@@ -447,8 +447,6 @@ template <typename T> struct DistillRow {
     terms[r] = p.s != 0 ? (T)((double)m.w * (double)wt * (double)wt * term) : (T)0;
   }
 };
-constexpr int DISTILL_CHUNKS = DISTILL_MAX_K / 32;  // of 32 entries
-static_assert(DISTILL_CHUNKS <= 32, "a lane per chunk");
 
 // A row's entries in shared memory: the indices (whole vectors of four, what is not an entry negative), the teacher's
 // logits, the row's.
@@ -732,26 +730,18 @@ template <typename T, int N> struct Table {
 };
 template <typename T> __device__ __forceinline__ Pair<T> pair(Stat<T> a) { return {a.m, a.s}; }
 
-// What a block's threads do with a row's entries, if the objective has any: entry threadIdx.x of the first NT is loaded before
-// the row's logits (its own logit between them, when the index is there), the others after them.
+// A row's entries, if the objective has any, by the threads of a block: entry threadIdx.x of the first NT is loaded before the
+// row's logits, and its own logit after the first of them, when the index is there.
 template <typename T, int NT, class Obj, bool TARGETS = Obj::TARGETS> struct Entries {
-  struct Slots {};
   __device__ __forceinline__ Entries(const Obj&, long long, const T*, long long, bool) {}
   __device__ __forceinline__ void gather() {}
+  static __device__ __forceinline__ int slots(const Obj&) { return 0; }
 };
 template <typename T, int NT, class Obj> struct Entries<T, NT, Obj, true> {
-  using Part = typename Obj::Part;
-  struct Slots {
-    Part of[2][DISTILL_CHUNKS];  // of 32 entries each
-    // By a warp: all entries.
-    __device__ __forceinline__ Part read(const Obj& obj, int half) const {
-      return obj.template join<32>((int)threadIdx.x % 32, ((int)obj.k + 31) / 32, [&](int i) { return of[half][i]; });
-    }
-  };
   const Obj& obj;
   const long long r, v;
   const T* x;
-  bool on;
+  const bool on;
   typename Obj::Entry first{neg_inf<T>(), (T)0, -1};
   __device__ __forceinline__ Entries(const Obj& o, long long row, const T* logits, long long vocab, bool live) : obj(o), r(row), v(vocab), x(logits), on(live) {
     if (on && (int)threadIdx.x < (int)obj.k) first = obj.entry(r, v, (int)threadIdx.x);
@@ -759,10 +749,11 @@ template <typename T, int NT, class Obj> struct Entries<T, NT, Obj, true> {
   __device__ __forceinline__ void gather() {
     if (on && (int)threadIdx.x < (int)obj.k) first.x = x[first.at];
   }
-  // Leaves the parts in `slots` and, if kept, the entries there. Whether this thread has any.
-  __device__ __forceinline__ bool finish(Slots& slots, int half, const Kept<T>* kept) {
+  static __device__ __forceinline__ int slots(const Obj& obj) { return ((int)obj.k + 3) / 4 * 4; }
+  // Leaves the entries in `kept`. Whether this thread has any that is not absent.
+  __device__ __forceinline__ bool keep(const Kept<T>& kept) {
     bool some = false;
-    for (int i = (int)threadIdx.x; i / 32 * 32 < (int)obj.k; i += NT) {
+    for (int i = (int)threadIdx.x; i < slots(obj); i += NT) {
       typename Obj::Entry n{neg_inf<T>(), (T)0, -1};
       if (i < NT) {
         n = first;
@@ -770,31 +761,30 @@ template <typename T, int NT, class Obj> struct Entries<T, NT, Obj, true> {
         n = obj.entry(r, v, i);
         n.x = x[n.at];
       }
-      if (kept && i < ((int)obj.k + 3) / 4 * 4) {
-        kept->at[i] = n.at;
-        kept->t[i] = n.t;
-        kept->x[i] = n.x;
-      }
-      const int lane = (int)threadIdx.x % 32;
-      const Part p = obj.template join<32>(lane, lane + 1, [&](int) { return n.part(); });
-      if (lane == 0) slots.of[half][i / 32] = p;
-      some = some || p.s != 0;
+      kept.at[i] = n.at;
+      kept.t[i] = n.t;
+      kept.x[i] = n.x;
+      some = some || n.t != neg_inf<T>();
     }
     return some;
   }
 };
+// By a warp: what the kept entries are together.
+template <typename T, class Obj> __device__ __forceinline__ typename Obj::Part together(const Obj& obj, const Kept<T>& kept) {
+  return obj.template join<32>((int)threadIdx.x % 32, (int)obj.k, [&](int i) { return typename Obj::Entry{kept.t[i], kept.x[i], 0}.part(); });
+}
 
 // ---- longer rows without a gradient ----
 
-constexpr int STREAM_THREADS = 256, STREAM_UNROLL = 4;
+constexpr int STREAM_UNROLL = 4;
 
 // A block, or a cluster of blocks, per row: a running maximum and sum per thread, four vectors at a time.
-template <typename T, bool CLUSTER, class Obj>
-__global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long rows, Obj obj, T k, int slice) {
-  constexpr int VEC = Num<T>::VEC, NT = STREAM_THREADS, U = STREAM_UNROLL;
+template <typename T, int NT, bool CLUSTER, class Obj>
+__global__ void __launch_bounds__(NT) k_stream(View<T> x, long long rows, Obj obj, T k, int slice) {
+  constexpr int VEC = Num<T>::VEC, U = STREAM_UNROLL;
+  extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Table<T, NT / 32> table;
   __shared__ Table<T, CLUSTER ? MAX_CLUSTER : 1> shares;
-  __shared__ typename Entries<T, NT, Obj>::Slots slots;
   const unsigned rank = CLUSTER ? cluster_rank() : 0, blocks = CLUSTER ? cluster_size() : 1;
   const long long step = gridDim.x / blocks;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, begin = (int)rank * slice;
@@ -830,10 +820,11 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
       a.s = a.s * Num<T>::exps(a.m - base(m), k) + b.s * Num<T>::exps(b.m - base(m), k);
       a.m = m;
     }
+    const Kept<T> kept(dyn + half * Entries<T, NT, Obj>::slots(obj) * (sizeof(int) + 2 * sizeof(T)), Entries<T, NT, Obj>::slots(obj));
     if constexpr (Obj::TARGETS) {
       if (rank == 0) {
         if ((begin + (int)threadIdx.x) * VEC >= row.hi) entries.gather();  // no logits for this thread
-        entries.finish(slots, half, nullptr);
+        entries.keep(kept);
       }
     }
     const Stat<T> of_warp = join<32>(a, k);
@@ -852,7 +843,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) k_stream(View<T> x, long long 
     if (reports) {
       const Stat<T> st = CLUSTER ? shares.read(half, (int)blocks, k) : table.read(half, NT / 32, k);
       if constexpr (Obj::TARGETS) {
-        const auto part = slots.read(obj, half);
+        const auto part = together(obj, kept);
         if (lane == 0) obj.report(r, now, part, st);
       } else {
         if (lane == 0) obj.report(r, now, xl, st);
@@ -940,12 +931,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Table<T, NW> table;                          // of the block's warps
   __shared__ Table<T, CLUSTER ? MAX_CLUSTER : 1> shares;  // of the cluster's blocks
-  __shared__ typename Entries<T, NT, Obj>::Slots slots;
   const unsigned rank = CLUSTER ? cluster_rank() : 0, blocks = CLUSTER ? cluster_size() : 1;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, begin = (int)rank * slice, first = begin + warp * 32 * U;
-  int entry_slots = 0;
-  if constexpr (Obj::TARGETS) entry_slots = ((int)obj.k + 3) / 4 * 4;
-  const Kept<T> kept(dyn, entry_slots);
+  const int slots = Entries<T, NT, Obj>::slots(obj);
   pdl_wait();
   if constexpr (CLUSTER) cluster_sync();  // every block's shared memory is there before another writes to it
   unsigned long long policy;
@@ -974,6 +962,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
         for (int u = 0; u < U; ++u) row.load(i + lane + 32 * u, y + u * VEC);
       }
     };
+    // Two rows' entries: the block's other warps are in the next row when the entries' gradients are written.
+    const Kept<T> kept(dyn + half * slots * (sizeof(int) + 2 * sizeof(T)), slots);
     T xl = (T)0, c = (T)0, f = (T)0, m_all = (T)0;
     int l = -1;
     Stat<T> st;
@@ -987,10 +977,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
       }
       Stat<T> a;
       for (int e = 0; e < turns; ++e) {
-        if (e == 0) entries.gather();
         if ((first + NT * U * e) * VEC >= row.hi) break;  // nothing of the row for this warp
         T y[U * VEC];
         load(first + NT * U * e, y, std::false_type{});
+        if (e == 0) entries.gather();
         const Stat<T> b = exponentials<T, U * VEC>(y, k);
         const T m = Num<T>::most(a.m, b.m);
         a.s = a.s * Num<T>::exps(a.m - base(m), k) + b.s * Num<T>::exps(b.m - base(m), k);
@@ -999,8 +989,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
       bool some = false;
       if constexpr (Obj::TARGETS) {
         // Before any of the gradient is written, which may be in the logits' place.
-        if (turns == 0) entries.gather();
-        some = entries.finish(slots, 0, &kept);
+        if (first * VEC >= row.hi) entries.gather();
+        some = entries.keep(kept);
       }
       const Stat<T> of_warp = join<32>(a, k);
       if (lane == 0) table.slot[half][warp] = pair(of_warp);
@@ -1048,8 +1038,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
       // element, with the probabilities of all entries of that index in order.
       __syncthreads();
       typename Obj::Part part;
-      if (!zero && (warp == 0 || warp * 32 < (int)obj.k)) {
-        part = slots.read(obj, 0);
+      if (!zero && warp * 32 < (int)obj.k) {
+        part = together(obj, kept);
         const T inverse_s = (T)1 / (T)part.s;
         const int lo = begin * VEC - row.off, hi = (begin + slice) * VEC - row.off;
         for (int i = threadIdx.x; i < (int)obj.k; i += NT) {
@@ -1063,7 +1053,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
         if (now.live()) obj.report(r, now, part, st);
         else obj.skip(r);
       }
-      __syncthreads();
     } else if (rank == 0 && threadIdx.x == 0) {
       if (now.live()) obj.report(r, now, xl, st);
       else obj.skip(r);
@@ -1286,7 +1275,7 @@ template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, 
 }
 
 template <typename T, class Obj> size_t target_bytes(const Obj& obj) {
-  if constexpr (Obj::TARGETS) return kept_bytes<T>(((size_t)obj.k + 3) / 4 * 4);
+  if constexpr (Obj::TARGETS) return 2 * kept_bytes<T>(((size_t)obj.k + 3) / 4 * 4);
   else return 0;
 }
 
@@ -1318,18 +1307,22 @@ template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& 
   return go_rows<T, 512, false>(x, obj, k, g, slice, 1, s);
 }
 
+template <typename T, int NT, bool CLUSTER, class Obj>
+cudaError_t go_stream(const RowView& x, const Obj& obj, T k, long long slice, unsigned cluster, cudaStream_t s) {
+  auto* kernel = k_stream<T, NT, CLUSTER, Obj>;
+  const size_t smem = target_bytes<T>(obj);
+  const long long clusters = std::min(x.rows(), resident(kernel, NT, smem, cluster));
+  return launch(kernel, dim3((unsigned)(clusters * cluster)), dim3(NT), smem, cluster, s, view<T>(x), x.rows(), obj, k, (int)slice);
+}
+
+// Rows without a gradient that no group holds.
 template <typename T, class Obj> cudaError_t stream(const RowView& x, const Obj& obj, T k, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
   const unsigned c = split(x.rows(), v);
-  const long long slice = pieces_of(v, c);
-  if (c == 1) {
-    auto* kernel = k_stream<T, false, Obj>;
-    return launch(kernel, dim3((unsigned)std::min(x.rows(), resident(kernel, STREAM_THREADS, 0, 1))), dim3(STREAM_THREADS), 0, 1, s, view<T>(x), x.rows(), obj,
-                  k, (int)slice);
-  }
-  auto* kernel = k_stream<T, true, Obj>;
-  return launch(kernel, dim3((unsigned)(std::min(x.rows(), resident(kernel, STREAM_THREADS, 0, c)) * c)), dim3(STREAM_THREADS), 0, c, s, view<T>(x), x.rows(),
-                obj, k, (int)slice);
+  if (c > 1) return go_stream<T, 256, true>(x, obj, k, pieces_of(v, c), c, s);
+  if (v <= 1024) return go_stream<T, 64, false>(x, obj, k, v, 1, s);
+  if (v <= 2048) return go_stream<T, 128, false>(x, obj, k, v, 1, s);
+  return go_stream<T, 256, false>(x, obj, k, v, 1, s);
 }
 
 // An objective's rows, with or without their gradient. scale: what the logits are multiplied by.
