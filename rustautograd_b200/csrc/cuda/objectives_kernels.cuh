@@ -440,6 +440,18 @@ template <typename T> struct DistillRow {
     }
     return all;
   }
+  // By a warp: the largest of the k teacher logits at t and the sum of their exponentials.
+  __device__ __forceinline__ Stat<T> total(const T* t) const {
+    const int lane = (int)threadIdx.x % 32;
+    Stat<T> st;
+    for (int i = lane; i < (int)k; i += 32) st.m = Num<T>::most(st.m, t[i]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) st.m = Num<T>::most(st.m, __shfl_xor_sync(~0u, st.m, d));
+    for (int i = lane; i < (int)k; i += 32) st.s += Num<T>::exps(t[i] - base(st.m), tk);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) st.s += __shfl_xor_sync(~0u, st.s, d);
+    return st;
+  }
   // q of an entry with teacher logit t, of all entries' part.
   __device__ __forceinline__ T share(T t, T m, T inverse_s) const { return Num<T>::exps(t - base(m), tk) * inverse_s; }
   __device__ __forceinline__ void report(long long r, const Meta& m, const Part& p, Stat<T> st) const {
@@ -729,6 +741,8 @@ template <typename T, int N> struct Table {
   }
 };
 template <typename T> __device__ __forceinline__ Pair<T> pair(Stat<T> a) { return {a.m, a.s}; }
+
+constexpr int MANY_ENTRIES = 64;
 
 // A row's entries, if the objective has any, by the threads of a block: entry threadIdx.x of the first NT is loaded before the
 // row's logits, and its own logit after the first of them, when the index is there.
@@ -1034,24 +1048,28 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
       else store<T, 32, U, false>(gr, row, i, lane, y);
     }
     if constexpr (Obj::TARGETS) {
-      // The entries in this block's slice, over what the block has stored. The first entry of an index writes its
-      // element, with the probabilities of all entries of that index in order.
-      __syncthreads();
-      typename Obj::Part part;
-      if (!zero && warp * 32 < (int)obj.k) {
-        part = together(obj, kept);
-        const T inverse_s = (T)1 / (T)part.s;
+      // The entries' elements, over what has been stored. Few entries: every warp those among its own vectors, so no warp waits
+      // for another and the next row's loads begin (a barrier here: 32000 logits with 32 entries 224 us). Many: a thread
+      // each, after a barrier.
+      if (!zero) {
+        const bool many = obj.k > MANY_ENTRIES;
+        if (many) __syncthreads();
+        else __syncwarp();
+        const Stat<T> all = obj.total(kept.t);
+        const T inverse_s = (T)1 / all.s;
         const int lo = begin * VEC - row.off, hi = (begin + slice) * VEC - row.off;
-        for (int i = threadIdx.x; i < (int)obj.k; i += NT) {
+        for (int i = many ? (int)threadIdx.x : lane; i < (int)obj.k; i += many ? NT : 32) {
           const int at = kept.at[i];
           T sum;
-          if (at >= lo && at < hi && kept.leads(i, (int)obj.k, &sum, [&](T t) { return obj.share(t, part.m, inverse_s); }))
-            gr[at] = Num<T>::exps(kept.x[i] - m_all, k) * f - c * sum;
+          if (at < lo || at >= hi || !(many || ((at + row.off) / VEC - begin) / (32 * U) % NW == warp)) continue;
+          if (kept.leads(i, (int)obj.k, &sum, [&](T t) { return obj.share(t, all.m, inverse_s); })) gr[at] = Num<T>::exps(kept.x[i] - m_all, k) * f - c * sum;
         }
-      }
-      if (rank == 0 && threadIdx.x == 0) {
-        if (now.live()) obj.report(r, now, part, st);
-        else obj.skip(r);
+        if (rank == 0 && warp == NW - 1) {
+          const auto part = together(obj, kept);
+          if (lane == 0) obj.report(r, now, part, st);
+        }
+      } else if (rank == 0 && threadIdx.x == 0) {
+        obj.skip(r);
       }
     } else if (rank == 0 && threadIdx.x == 0) {
       if (now.live()) obj.report(r, now, xl, st);
