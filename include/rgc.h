@@ -204,7 +204,7 @@ int rgc_preference_loss(const rgc_logits* logits, const int32_t* labels, const r
 
 /* A row's `entries` (1 to 1024) teacher logits at `index`: q = softmax(teacher / T), p = softmax(x / T),
  * terms = weight T^2 sum q (log q - log p[index]), loss = their sum. Entries of -inf are absent; an index
- * given twice counts twice; a row without entries counts nothing. */
+ * given twice counts twice; a row without entries counts nothing. T is between 2^-60 and 2^60. */
 typedef struct {
   const int32_t* index;
   const void *teacher, *weight;

@@ -227,7 +227,7 @@ RGC_EXPORT int rgc_distillation_loss(const rgc_logits* logits, const rgc_distill
     const Rows r = check_logits(logits);
     if (!p) refuse("null argument");
     if (p->entries < 1 || p->entries > DISTILL_MAX_K) refuse("teacher entries per row must be between 1 and " + std::to_string(DISTILL_MAX_K));
-    if (!(p->temperature > 0) || !std::isfinite(p->temperature)) refuse("temperature must be positive");
+    if (!(p->temperature >= 0x1p-60 && p->temperature <= 0x1p60)) refuse("temperature must be between 2^-60 and 2^60");  // 1 / T and T^2 in a float
     const RowOut g = check_gradient(*logits, r, grad);
     const int dev = current_device();
     check_pointer("loss", loss, r.es, dev);

@@ -1,20 +1,23 @@
 // Kernels of the objectives over logits (objectives.cuh has the formulas).
 //
 // All of them are bound by memory: a row is V logits to read and, with a gradient, V values to write, against
-// one exponential per logit. So each row is read from memory once and kept on chip until its gradient is
-// written:
-//  - k_group (rows up to 1024 floats): a group of 8, 16 or 32 lanes holds a row in registers;
-//  - k_block (longer rows, with a gradient): a block, or the blocks of a cluster, hold a row in registers,
-//    16-byte pieces arriving through shared memory (cp.async) while the row before is computed;
+// one exponential per logit (two with a gradient).
+//  - k_group, k_group_targets (rows up to 640 vectors of 16 bytes): groups of 8, 16 or 32 lanes hold rows in registers
+//    from the loads to the gradient;
+//  - k_rows (longer rows, with a gradient): a block, or a cluster of blocks, reads a row twice, the second time from
+//    the L2;
 //  - k_stream (longer rows, no gradient): a running maximum and sum, nothing is held;
-//  - k_two_pass (rows longer than a cluster holds): reads the row twice;
-//  - k_grad: gradients whose coefficients need more than their row (token_log_prob_grad, preferences).
+//  - k_grad (longer rows): gradients whose coefficients need more than their row (token_log_prob_grad, preferences).
+// Of the rate of a plain copy they reach, in floats: k_stream 99 % (8192 to 131072 logits), k_grad 97 %, k_rows 91 %
+// (4096 to 16384), 88 % (32000), 83 % (50257) and 78 % (131072), k_group 88 to 95 % where its vectors are full and there are
+// 1000 logits, 61 % at 96.
 //
 // Numbers. Row statistics are held in the logits' type. For float, exp(x - m) is computed as
 // 2^((x - m) * log2 e) with the hardware's ex2: the difference and the product are rounded, 2.3 u |x - m|
 // relatively (log2 e as a float is 0.22 u off), and ex2 is within 2 ulp; against expf that halves the
-// instructions per logit. For double it is a polynomial (Num<double>). What a row reports (its log-probability's terms) is computed from the statistics
-// in double by one lane, and sums over rows are double: a loss is a sum of terms of both signs.
+// instructions per logit. For double it is a polynomial (Num<double>). What a row reports (its log-probability's
+// terms) is computed from the statistics in double by one lane, and sums over rows are double: a loss is a sum of
+// terms of both signs.
 // Everything is summed in a fixed order: the same inputs give the same bits on every call. The bits of a row do
 // depend on how it is split over lanes and blocks, which goes by the vocabulary and the row count.
 #pragma once
@@ -83,7 +86,7 @@ template <> struct Num<double> {
   using Vec = double2;
   // exp(d * scale) for d <= 0: 2^t with t = d * scale * log2 e = n + f, n whole and |f| <= 1/2; 2^f by the polynomial of
   // degree 11 that equals it at 12 Chebyshev nodes (off by 4.3e-18 relatively; 1.2 u with Horner's roundings).
-  // Below 2^-1022 it is 0. 17 double operations, where exp() took twice as long for the whole pass.
+  // Below 2^-1022 it is 0. (7 x 129 x 10007 without gradient: 28.6 us, with exp() 32.6.)
   static __device__ __forceinline__ double exps(double d, double k) {
     constexpr double C[12] = {0x1.0000000000000p+0,  0x1.62e42fefa39efp-1,  0x1.ebfbdff82c5aep-3,  0x1.c6b08d704a0c6p-5,
                               0x1.3b2ab6fb9f1a5p-7,  0x1.5d87fe78a3f9cp-10, 0x1.430913112c61bp-13, 0x1.ffcbfc6da6ed1p-17,
@@ -711,8 +714,7 @@ __device__ __forceinline__ unsigned cluster_size() {
 // The cluster's barrier, by whole warps.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// Without ordering: for warps whose stores no other block reads (a release waits for the gradient's stores to
-// reach the L2: 16 x 1024 x 50257 at 55 instead of X % of the copy rate).
+// Without ordering: for warps that have written nothing another block reads.
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
   cluster_arrive();
@@ -742,7 +744,7 @@ template <typename T, int N> struct Table {
 };
 template <typename T> __device__ __forceinline__ Pair<T> pair(Stat<T> a) { return {a.m, a.s}; }
 
-constexpr int MANY_ENTRIES = 64;
+constexpr int MANY_ENTRIES = 64;  // 4096 x 50257: 338 us with 64, a barrier a row (65) 349
 
 // A row's entries, if the objective has any, by the threads of a block: entry threadIdx.x of the first NT is loaded before the
 // row's logits, and its own logit after the first of them, when the index is there.
@@ -936,8 +938,9 @@ __device__ __forceinline__ double2 load_keep(const double2* p, unsigned long lon
 // one, backwards, that reads the logits again and writes the gradient. The second pass finds them in the L2 (or the
 // L1), as long as the rows under way fit there, so memory sees each logit once.
 // Measured against keeping a row on chip between the passes (in registers and shared memory, copies of the next row under
-// way): 76 against 57 % of the copy rate at 50257 logits and 84 against 69 % at 32000, where a row needs a cluster of
-// blocks and each waits for the slowest; 80 against 85 % at 16384, where one block holds it.
+// way): 83 against 57 % of the copy rate at 50257 logits and 88 against 69 % at 32000, where a row needs a cluster of
+// blocks and each waits for the slowest; 91 against 85 % at 16384, where one block holds it.
+// 32 warps to an SM with 4 vectors a lane under way: with 48 and 2 16384 logits run at 75 %, with 24 and 8 at 84 %.
 template <typename T, int NT, bool CLUSTER, class Obj>
 __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const long long rows, const __grid_constant__ Obj obj, const T k, const Out<T> g, const int slice) {
   constexpr int VEC = Num<T>::VEC, NW = NT / 32, U = 16 / sizeof(T);
@@ -1093,7 +1096,8 @@ __device__ double block_sum(double v, double* sh) {
   return v;
 }
 
-// A cluster's blocks, or one block, add up the terms: sixteen of a thread at a time, then threads, warps and blocks in order.
+// A cluster's blocks, or one block, add up the terms: sixteen of a thread at a time, then threads, warps and blocks in
+// order. (131072 x 96 logits and their sum: 27 us; with 512 threads, eight at a time, 35.)
 constexpr int SUM_THREADS = 1024, SUM_CLUSTER = 8, SUM_AHEAD = 16;
 template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms(const T* __restrict__ terms, long long n, T* loss, double scale) {
   pdl_wait();
@@ -1240,7 +1244,8 @@ template <typename K> long long resident(K* kernel, int threads, size_t smem, un
 
 long long pieces_of(long long n, long long of) { return (n + of - 1) / of; }
 
-// Blocks per row: more than one when the rows alone would leave SMs without work, down to 512 vectors each.
+// Blocks per row: more than one when the rows alone would leave SMs without work, down to 512 vectors each. (48 rows of
+// 50257: 11.5 us with 8 blocks each, 17.3 with 2.)
 unsigned split(long long rows, long long vectors) {
   unsigned c = 1;
   while (c < MAX_CLUSTER && rows * c * 2 <= 4 * sm_count() && vectors / (2 * c) >= 512) c *= 2;
@@ -1252,7 +1257,8 @@ template <typename K, typename... A> cudaError_t go_group(K* kernel, long long r
   return launch(kernel, dim3((unsigned)blocks), dim3(GROUP_THREADS), smem, 1, s, args...);
 }
 
-// Rows of at most 512 vectors, by the fewest lanes that hold one; up to 16 vectors a lane in all.
+// Rows of at most 640 vectors, by the fewest lanes that hold one; some 16 vectors a lane in all, or one row. (516 vectors,
+// 65536 x 2064: 184 us here, 260 by a block per row; with 24 vectors a lane for 750, 65536 x 3000: 273 us here, 269.)
 constexpr long long GROUP_VECTORS = 640;
 template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, const Obj& obj, T k, const RowOut& g, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
@@ -1311,7 +1317,8 @@ template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& 
   const long long v = most_vectors<T>(x);
   unsigned c = split(x.rows(), v);
   // Rows under way at once that do not fit the L2 (its two halves hold copies of what the other half's SMs read):
-  // fewer, each by a cluster.
+  // fewer, each by a cluster. (4096 x 50257, 60 MB under way: 300 us, by clusters of two 385. 4096 x 65536: clusters
+  // of two, 78 MB, 396 us, of four 409.)
   if (c == 1 && v * 16 * 2 * sm_count() > L2_ROWS_BYTES)
     for (c = 2; c < MAX_CLUSTER && v * 16 * 4 * sm_count() / c > L2_ROWS_BYTES; c *= 2) {
     }
@@ -1338,8 +1345,10 @@ template <typename T, class Obj> cudaError_t stream(const RowView& x, const Obj&
   const long long v = most_vectors<T>(x);
   const unsigned c = split(x.rows(), v);
   if (c > 1) return go_stream<T, 256, true>(x, obj, k, pieces_of(v, c), c, s);
+  // Two to four turns of a block over the row: 2800 floats (700 vectors, 64 threads) 121 us against 226 with 256, 5400 (1350)
+  // 62 and 60 with 64 and 128 threads, 11000 (2750) 110 and 115 with 128 and 256.
   if (v <= 1024) return go_stream<T, 64, false>(x, obj, k, v, 1, s);
-  if (v <= 2048) return go_stream<T, 128, false>(x, obj, k, v, 1, s);
+  if (v <= 2896) return go_stream<T, 128, false>(x, obj, k, v, 1, s);
   return go_stream<T, 256, false>(x, obj, k, v, 1, s);
 }
 

@@ -79,7 +79,8 @@ bool objective_of(const Op& op, const std::vector<std::vector<size_t>>& s, const
       if (s[1].empty() || s[1].back() == 0 || s[1].back() > MAX_TEACHER) return no("teacher_needs_between_1_and_1024_entries_per_row");
       o.k = s[1].back();
       if (s[1] != with(o.k) || s[2] != s[1] || s[3] != lead) return no("operands_do_not_fit_the_logits");
-      if (!attrs_ok(op, 1) || !(objective_attr(op, 0) > 0)) return no("temperature_must_be_positive");
+      // Beyond these bounds 1 / T or T^2 leaves the range of a float.
+      if (!attrs_ok(op, 1) || !(objective_attr(op, 0) >= 0x1p-60 && objective_attr(op, 0) <= 0x1p60)) return no("temperature_must_be_between_2^-60_and_2^60");
       o.outs = {{}, lead, s[0]};
       o.grad_out = 2;
   }

@@ -202,7 +202,7 @@ def distillation_loss(logits, index, teacher, weights, *, temperature=1.0, grad=
     """Distillation from a teacher's top logits: `teacher` (..., k) at the vocabulary positions `index` (..., k).
     With q = softmax(teacher / T) and p = softmax(logits / T), the sum over positions of
     weights * T^2 * sum_k q (log q - log p). Entries of -inf are absent (rows may hold fewer than k), an
-    index given twice counts twice, and k is at most 1024."""
+    index given twice counts twice, and k is at most 1024. T is between 2^-60 and 2^60."""
     c = _Call(logits, grad, out)
     if not isinstance(index, torch.Tensor) or index.dim() < 1:
         raise TypeError("index must be a tensor with a last axis of teacher entries")

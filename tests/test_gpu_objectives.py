@@ -449,3 +449,86 @@ def test_parts_of_a_row_without_any_logit(dtype):
         index, teacher = lab[:, None].copy(), np.zeros((4, 1), dtype)
         d = losses.distillation_loss(*put(x, index, teacher, w))
         check(d, R.distillation(x, index, teacher, w, 1.0, dtype, adds(v)), d._fields, f"sparse {v}")
+
+
+# Vectors of 16 bytes to a row, around the numbers that the kernels for short rows and the blocks' sizes change at.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vectors", [8, 9, 16, 24, 25, 32, 50, 64, 100, 128, 150, 192, 193, 256, 300, 320, 321, 384, 385, 512, 513, 640, 641, 1025, 1449, 2049, 2897, 5793])
+def test_widths_between_the_variants(vectors, dtype):
+    v, rows = vectors * 16 // np.dtype(dtype).itemsize, 11
+    rng = np.random.default_rng([vectors, len(dtype)])
+    x = R.logits(rng, rows, v, "normal", dtype)
+    lab = R.labels(rng, x)
+    old, adv, w, ref = R.policy_inputs(rng, x, lab, dtype)
+    w[3] = 0
+    bad = x.copy()
+    bad[w == 0] = np.nan
+    want = R.policy(x, lab, old, adv, w, ref, 0.2, 0.28, 0.05, dtype, adds(v))
+    r = losses.policy_loss(*put(bad, lab, old, adv, w), ref_logp=put(ref)[0], clip_low=0.2, clip_high=0.28, kl=0.05)
+    check(r, want, r._fields, f"policy {rows} x {vectors} vectors")
+    k = min(v, 13)
+    index, teacher, w = R.teacher_inputs(rng, x, k, dtype)
+    bad = x.copy()
+    bad[w == 0] = np.nan
+    want = R.distillation(x, index, teacher, w, 1.5, dtype, adds(v))
+    r = losses.distillation_loss(*put(bad, index, teacher, w), temperature=1.5)
+    check(r, want, r._fields, f"distillation {rows} x {vectors} vectors")
+    logp, stats = losses.token_log_prob(*put(x, lab), stats=True)
+    grad = losses.token_log_prob_grad(*put(x, lab), stats, *put(adv))
+    check((logp, grad), R.token_log_prob(x, lab, adv, dtype, adds(v)), ("logp", "gradient"), f"{rows} x {vectors} vectors")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [3, 96, 700, 2051, 5001, 20000])
+@pytest.mark.parametrize("k", [2, 5, 16, 32, 33, 64, 65, 257, 1024])
+def test_numbers_of_teacher_entries(k, v, dtype):
+    rng = np.random.default_rng([k, v])
+    rows = 9
+    x = R.logits(rng, rows, v, "normal", dtype)
+    index, teacher, w = R.teacher_inputs(rng, x, k, dtype)
+    w[:3] = 0.5
+    index[0] = rng.integers(0, 2, k)          # the same index many times
+    index[1, -1] = index[1, 0]                # the first and the last entry
+    index[2] = 2 * v                          # past the vocabulary: its last element
+    want = R.distillation(x, index, teacher, w, 0.7, dtype, adds(v))
+    args = put(x, index, teacher, w)
+    r = losses.distillation_loss(*args, temperature=0.7)
+    check(r, want, r._fields, f"distillation {rows}x{v} k {k}")
+    alone = losses.distillation_loss(*args, temperature=0.7, grad=False)
+    check(alone[:2], want, r._fields, f"distillation without gradient {rows}x{v} k {k}")
+    within = losses.distillation_loss(*args, temperature=0.7, out=args[0])
+    assert torch.equal(args[0], r.grad) and torch.equal(within.terms, r.terms)
+
+
+@pytest.mark.parametrize("b,t,v", [(40, 3, 5), (34, 1, 33), (6, 700, 9), (2, 257, 40), (70, 300, 3)])
+def test_preferences_of_many_pairs_and_long_sequences(b, t, v):
+    rng = np.random.default_rng([b, t, v])
+    x = R.logits(rng, b * t, v, "normal", "float32")
+    lab = R.labels(rng, x).reshape(b, t)
+    x = x.reshape(b, t, v)
+    w = ((rng.random((b, t)) < 0.7) / t).astype("float32")
+    ref = (-rng.random(b) * 3).astype("float32")
+    want = R.preference(x, lab, w, ref, 0.3, 0.1, "float32", adds(v))
+    args = put(x, lab, w, ref)
+    r = losses.preference_loss(*args, beta=0.3, smoothing=0.1)
+    check(r, want, r._fields, f"preference {b}x{t}x{v}")
+    again = losses.preference_loss(*args, beta=0.3, smoothing=0.1)
+    assert all(torch.equal(p, q) for p, q in zip(r, again))
+
+
+@pytest.mark.parametrize("v", [96, 5000])
+def test_wide_and_tiny_doubles(v):
+    """Doubles whose exponentials leave the normal range, and rows a constant apart: the polynomial's ends."""
+    rng = np.random.default_rng(v)
+    x = rng.normal(size=(6, v))
+    x[0] *= 400
+    x[1] = -rng.random(v) * 745
+    x[2] = np.where(rng.random(v) < 0.5, -1e308, 0)
+    x[3] = 1e15 + rng.integers(0, 64, v)
+    x[4, 1:] = -709.0 + rng.random(v - 1)
+    x[5] = np.linspace(-708, 0, v)
+    lab, ct = np.argmax(x, 1).astype("int32"), np.ones(6)
+    lab[5] = 0
+    logp, stats = losses.token_log_prob(*put(x, lab), stats=True)
+    grad = losses.token_log_prob_grad(*put(x, lab), stats, *put(ct))
+    check((logp, grad), R.token_log_prob(x, lab, ct, "float64", adds(v)), ("logp", "gradient"), f"doubles {v}")

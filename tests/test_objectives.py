@@ -324,3 +324,10 @@ def test_call_refusals_without_a_gpu(product):
         rows(x[:, :, :-1], torch.zeros(4, 6, 5, 8)[:, :-1])
     with pytest.raises(ValueError, match="contiguous"):
         rows(x.transpose(2, 3))
+
+
+def test_temperature_bounds(cpu):
+    for temp in (2.0 ** -61, 2.0 ** 61, 1e-300, float("nan")):
+        with pytest.raises(Exception) as e:
+            F.nn.distillation_loss(F.zeros((4, 3, 8)), F.zeros((4, 3, 2), "int32"), F.zeros((4, 3, 2)), F.zeros((4, 3)), temperature=temp)
+        assert e.value.diagnostic["code"] == "OBJECTIVE_OPERANDS"
