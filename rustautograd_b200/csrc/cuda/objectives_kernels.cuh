@@ -86,7 +86,8 @@ template <> struct Num<double> {
   using Vec = double2;
   // exp(d * scale) for d <= 0: 2^t with t = d * scale * log2 e = n + f, n whole and |f| <= 1/2; 2^f by the polynomial of
   // degree 11 that equals it at 12 Chebyshev nodes (off by 4.3e-18 relatively; 1.2 u with Horner's roundings).
-  // Below 2^-1022 it is 0. (7 x 129 x 10007 without gradient: 28.6 us, with exp() 32.6.)
+  // Below 2^-1022 it is 0. (7 x 129 x 10007 without gradient: 28.6 us, with exp() 32.6. The power of two put in by integer
+  // operations, 14 instead of 17 double ones: 8192 x 8192 in 190 instead of 165 us, so not those alone bound it.)
   static __device__ __forceinline__ double exps(double d, double k) {
     constexpr double C[12] = {0x1.0000000000000p+0,  0x1.62e42fefa39efp-1,  0x1.ebfbdff82c5aep-3,  0x1.c6b08d704a0c6p-5,
                               0x1.3b2ab6fb9f1a5p-7,  0x1.5d87fe78a3f9cp-10, 0x1.430913112c61bp-13, 0x1.ffcbfc6da6ed1p-17,
@@ -522,6 +523,24 @@ template <typename T, int N> __device__ __forceinline__ Stat<T> exponentials(T* 
   return a;
 }
 
+// The same for N more logits of a thread's running maximum and sum: relative to the maximum of both, so one of the two sums
+// needs no factor. (8192 x 8192 doubles 165 us, 180 with two sums joined.)
+template <typename T, int N> __device__ __forceinline__ void extend(Stat<T>& a, T* x, T k) {
+  T m = a.m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = Num<T>::most(x[i], m);
+  const T b = base(m);
+  T s0 = (T)0, s1 = (T)0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const T e = Num<T>::exps(x[i] - b, k);
+    if (i % 2) s1 += e;
+    else s0 += e;
+  }
+  a.s = a.s * Num<T>::exps(a.m - b, k) + (s0 + s1);
+  a.m = m;
+}
+
 // A warp computes B times 32 / G rows together (G lanes each, E vectors a lane): all loads first, then the sums, then what
 // the rows need once, a lane per row, then the gradients. The label's element is stored a second time by
 // its row's lane, so no lane looks for it.
@@ -792,12 +811,13 @@ template <typename T, class Obj> __device__ __forceinline__ typename Obj::Part t
 
 // ---- longer rows without a gradient ----
 
-constexpr int STREAM_UNROLL = 4;
+// Sixteen logits a thread at a time. (8192 x 8192 doubles: 153 us, with eight 165.)
+template <typename T> constexpr int STREAM_UNROLL = 16 / Num<T>::VEC;
 
-// A block, or a cluster of blocks, per row: a running maximum and sum per thread, four vectors at a time.
+// A block, or a cluster of blocks, per row: a running maximum and sum per thread.
 template <typename T, int NT, bool CLUSTER, class Obj>
 __global__ void __launch_bounds__(NT) k_stream(View<T> x, long long rows, Obj obj, T k, int slice) {
-  constexpr int VEC = Num<T>::VEC, U = STREAM_UNROLL;
+  constexpr int VEC = Num<T>::VEC, U = STREAM_UNROLL<T>;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Table<T, NT / 32> table;
   __shared__ Table<T, CLUSTER ? MAX_CLUSTER : 1> shares;
@@ -831,10 +851,7 @@ __global__ void __launch_bounds__(NT) k_stream(View<T> x, long long rows, Obj ob
 #pragma unroll
       for (int u = 0; u < U; ++u) row.load(i + NT * u, y + u * VEC);
       if (i < begin + NT * U) entries.gather();
-      const Stat<T> b = exponentials<T, U * VEC>(y, k);
-      const T m = Num<T>::most(a.m, b.m);
-      a.s = a.s * Num<T>::exps(a.m - base(m), k) + b.s * Num<T>::exps(b.m - base(m), k);
-      a.m = m;
+      extend<T, U * VEC>(a, y, k);
     }
     const Kept<T> kept(dyn + half * Entries<T, NT, Obj>::slots(obj) * (sizeof(int) + 2 * sizeof(T)), Entries<T, NT, Obj>::slots(obj));
     if constexpr (Obj::TARGETS) {
@@ -940,10 +957,11 @@ __device__ __forceinline__ double2 load_keep(const double2* p, unsigned long lon
 // Measured against keeping a row on chip between the passes (in registers and shared memory, copies of the next row under
 // way): 83 against 57 % of the copy rate at 50257 logits and 88 against 69 % at 32000, where a row needs a cluster of
 // blocks and each waits for the slowest; 91 against 85 % at 16384, where one block holds it.
-// 32 warps to an SM with 4 vectors a lane under way: with 48 and 2 16384 logits run at 75 %, with 24 and 8 at 84 %.
+// 32 warps to an SM with 4 vectors a lane under way: with 48 and 2 16384 logits run at 75 %, with 24 and 8 at 84 %. Doubles:
+// 24 warps and 4 vectors, 8192 x 8192 in 290 us; with 32 and 2 341.
 template <typename T, int NT, bool CLUSTER, class Obj>
-__global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const long long rows, const __grid_constant__ Obj obj, const T k, const Out<T> g, const int slice) {
-  constexpr int VEC = Num<T>::VEC, NW = NT / 32, U = 16 / sizeof(T);
+__global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 768) / NT) k_rows(const View<T> x, const long long rows, const __grid_constant__ Obj obj, const T k, const Out<T> g, const int slice) {
+  constexpr int VEC = Num<T>::VEC, NW = NT / 32, U = 4;
   using Vec = typename Num<T>::Vec;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Table<T, NW> table;                          // of the block's warps
@@ -998,10 +1016,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_rows(const View<T> x, const l
         T y[U * VEC];
         load(first + NT * U * e, y, std::false_type{});
         if (e == 0) entries.gather();
-        const Stat<T> b = exponentials<T, U * VEC>(y, k);
-        const T m = Num<T>::most(a.m, b.m);
-        a.s = a.s * Num<T>::exps(a.m - base(m), k) + b.s * Num<T>::exps(b.m - base(m), k);
-        a.m = m;
+        extend<T, U * VEC>(a, y, k);
       }
       bool some = false;
       if constexpr (Obj::TARGETS) {
@@ -1096,9 +1111,9 @@ __device__ double block_sum(double v, double* sh) {
   return v;
 }
 
-// A cluster's blocks, or one block, add up the terms: sixteen of a thread at a time, then threads, warps and blocks in
-// order. (131072 x 96 logits and their sum: 27 us; with 512 threads, eight at a time, 35.)
-constexpr int SUM_THREADS = 1024, SUM_CLUSTER = 8, SUM_AHEAD = 16;
+// A cluster's blocks, or one block, add up the terms: eight of a thread at a time, then threads, warps and blocks in order.
+// (131072 terms: 6 us; sixteen at a time with a bound on each load 11.)
+constexpr int SUM_THREADS = 512, SUM_CLUSTER = 8, SUM_AHEAD = 8;
 template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms(const T* __restrict__ terms, long long n, T* loss, double scale) {
   pdl_wait();
   __shared__ double sh[SUM_THREADS / 32];
@@ -1108,15 +1123,16 @@ template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms
   double v = 0;
   const long long step = (long long)blocks * SUM_THREADS;
   long long i = (long long)rank * SUM_THREADS + threadIdx.x;
-  for (; i < n; i += SUM_AHEAD * step) {
+  for (; i + (SUM_AHEAD - 1) * step < n; i += SUM_AHEAD * step) {
     T z[SUM_AHEAD];
 #pragma unroll
-    for (int q = 0; q < SUM_AHEAD; ++q) z[q] = i + q * step < n ? terms[i + q * step] : (T)0;
+    for (int q = 0; q < SUM_AHEAD; ++q) z[q] = terms[i + q * step];
     double part[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int q = 0; q < SUM_AHEAD; ++q) part[q % 4] += (double)z[q];
     v += (part[0] + part[1]) + (part[2] + part[3]);
   }
+  for (; i < n; i += step) v += (double)terms[i];
   v = block_sum(v, sh);
   if (blocks > 1) {
     if (threadIdx.x == 0) put_remote(&of_block[rank], 0u, Pair<double>{v, 0.0});
@@ -1345,10 +1361,10 @@ template <typename T, class Obj> cudaError_t stream(const RowView& x, const Obj&
   const long long v = most_vectors<T>(x);
   const unsigned c = split(x.rows(), v);
   if (c > 1) return go_stream<T, 256, true>(x, obj, k, pieces_of(v, c), c, s);
-  // Two to four turns of a block over the row: 2800 floats (700 vectors, 64 threads) 121 us against 226 with 256, 5400 (1350)
-  // 62 and 60 with 64 and 128 threads, 11000 (2750) 110 and 115 with 128 and 256.
-  if (v <= 1024) return go_stream<T, 64, false>(x, obj, k, v, 1, s);
-  if (v <= 2896) return go_stream<T, 128, false>(x, obj, k, v, 1, s);
+  // Some three turns of a block over the row: 2800 floats (700 vectors, 64 threads) 121 us against 226 with 256; 5400 (1350) 62
+  // and 60 with 64 and 128; 11000 (2750) 110 and 115 with 128 and 256; 32000 (8000) 325 and 301.
+  if (v <= 1024 / 4 * STREAM_UNROLL<T>) return go_stream<T, 64, false>(x, obj, k, v, 1, s);
+  if (v <= 2896 / 4 * STREAM_UNROLL<T>) return go_stream<T, 128, false>(x, obj, k, v, 1, s);
   return go_stream<T, 256, false>(x, obj, k, v, 1, s);
 }
 

@@ -92,5 +92,5 @@ def distillation_loss(logits, index, teacher, weights, temperature=1.0):
     """`(loss, terms)` of the distillation from a teacher's k top logits, `teacher` (..., k) at vocabulary
     positions `index` (..., k): with q = softmax(teacher / T) and p = softmax(logits / T), terms =
     weights * T^2 * sum q (log q - log p) and loss their sum. Teacher entries of -inf are absent, an index
-    given twice counts twice, k is at most 1024."""
+    given twice counts twice, k is at most 1024. T is between 2^-60 and 2^60."""
     return objective("distillation_loss", logits, index, teacher, weights, temperature=float(temperature))[:2]
