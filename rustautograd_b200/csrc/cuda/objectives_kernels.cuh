@@ -30,6 +30,7 @@
 #include <mutex>
 #include <tuple>
 #include <type_traits>
+#include <utility>
 
 namespace rgc {
 
@@ -1221,17 +1222,24 @@ int sm_count() {
 }
 
 // Clusters of `cluster` blocks of a kernel that the GPU holds at once (1: blocks), looked up once per kernel,
-// shared memory and cluster. Also lets the kernel have that much dynamic shared memory, on each device.
+// shared memory and cluster. Also lets the kernel have that much dynamic shared memory, on each device: never less than it has
+// been given before, which another call may be counting on.
 template <typename K> long long resident(K* kernel, int threads, size_t smem, unsigned cluster) {
   static std::mutex mu;
   static std::map<std::tuple<const void*, size_t, unsigned, int>, long long> known;
+  static std::map<std::pair<const void*, int>, size_t> given;
   int dev = 0;
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lk(mu);
   const auto key = std::make_tuple((const void*)kernel, smem, cluster, dev);
   const auto it = known.find(key);
   if (it != known.end()) return it->second;
-  if (smem > 48 * 1024) cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  size_t& most = given[{(const void*)kernel, dev}];
+  if (smem > 48 * 1024 && smem > most) {
+    const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) most = smem;
+    else cudaGetLastError();  // the launch says so
+  }
   int n = 0;
   if (cluster > 1) {
     cudaLaunchConfig_t cfg = {};

@@ -532,3 +532,13 @@ def test_wide_and_tiny_doubles(v):
     logp, stats = losses.token_log_prob(*put(x, lab), stats=True)
     grad = losses.token_log_prob_grad(*put(x, lab), stats, *put(ct))
     check((logp, grad), R.token_log_prob(x, lab, ct, "float64", adds(v)), ("logp", "gradient"), f"doubles {v}")
+
+
+def test_entry_counts_in_turn():
+    """More entries, fewer, and more again: the shared memory of the first call is still there for the third."""
+    rng = np.random.default_rng(9)
+    x, w = rng.normal(size=(9, 96)), np.full(9, 0.5)
+    for k in (1024, 600, 1024, 7, 700):
+        index, teacher = rng.integers(0, 96, (9, k)).astype("int32"), rng.random((9, k)) * 3
+        r = losses.distillation_loss(*put(x, index, teacher, w))
+        check(r, R.distillation(x, index, teacher, w, 1.0, "float64", adds(96)), r._fields, f"{k} entries")
