@@ -160,7 +160,10 @@ int rgc_sum_noalloc(const void* src, int64_t n, int dtype, void* dst, void* stre
  * [0, vocab). For a row x: m = max x, s = sum exp(x - m), p = exp(x - m) / s, lp = x[label] - m - log s.
  * A gradient goes to outer x inner rows of its own strides; it may be the logits themselves (same
  * data and strides), and must not overlap them otherwise. Rows with weight 0 are not read: they count
- * nothing, whatever they hold, and their gradient is 0. */
+ * nothing, whatever they hold, and their gradient is 0.
+ * With RGC_VOUCHED added to dtype the caller vouches that every pointer is the current device's memory; otherwise each is
+ * looked up first, some 0.3 us a pointer. */
+#define RGC_VOUCHED 256
 typedef struct {
   const void* data;
   int64_t outer, inner, vocab;

