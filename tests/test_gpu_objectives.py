@@ -542,3 +542,35 @@ def test_entry_counts_in_turn():
         index, teacher = rng.integers(0, 96, (9, k)).astype("int32"), rng.random((9, k)) * 3
         r = losses.distillation_loss(*put(x, index, teacher, w))
         check(r, R.distillation(x, index, teacher, w, 1.0, "float64", adds(96)), r._fields, f"{k} entries")
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose very first calls are captured: nothing they look up or load ends the capture."""
+    import subprocess
+    import sys
+
+    script = """
+import torch
+from rustautograd_b200 import losses
+x = torch.randn(6, 40, 2500, device="cuda")
+y = torch.randn(6, 40, 200, device="cuda", dtype=torch.float64)
+lab = torch.randint(0, 200, (6, 40), device="cuda", dtype=torch.int32)
+w = torch.rand(6, 40, device="cuda")
+seq = torch.rand(6, device="cuda", dtype=torch.float64)
+index = torch.randint(0, 2500, (6, 40, 70), device="cuda", dtype=torch.int32)
+teacher = torch.rand(6, 40, 70, device="cuda")
+torch.cuda.synchronize()
+calls = lambda: (losses.policy_loss(x, lab, -w, w, w), losses.preference_loss(y, lab, w.double(), seq), losses.distillation_loss(x, index, teacher, w),
+                 losses.token_log_prob(y, lab, stats=True))
+s = torch.cuda.Stream()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    got = calls()
+g.replay()
+torch.cuda.synchronize()
+for a, b in zip(got, calls()):
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr[-2000:]
