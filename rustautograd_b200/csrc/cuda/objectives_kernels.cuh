@@ -13,11 +13,15 @@
 // 1000 logits, 61 % at 96.
 //
 // Numbers. Row statistics are held in the logits' type. For float, exp(x - m) is computed as
-// 2^((x - m) * log2 e) with the hardware's ex2: the difference and the product are rounded, 2.3 u |x - m|
-// relatively (log2 e as a float is 0.22 u off), and ex2 is within 2 ulp; against expf that halves the
-// instructions per logit. For double it is a polynomial (Num<double>). What a row reports (its log-probability's
-// terms) is computed from the statistics in double by one lane, and sums over rows are double: a loss is a sum of
-// terms of both signs.
+// 2^((x - m) * log2 e) with the hardware's ex2: the difference and the product are rounded, 2 u |x - m|
+// relatively, and ex2 is within 2 ulp; against expf that halves the instructions per logit. What does not average out over
+// a row's logits is taken out, since it is the same in every row of a batch and a loss is a sum of terms of both
+// signs: log2 e has two parts (as one float it is 1.3e-8 too small), ex2's mean error is put into its argument, and
+// the factors between parts of a row are a polynomial's (Num<float>::share). Row sums of normal logits, deviation 1 and 2.5, are then
+// off by 3e-9 to 9e-9 on average (8192 to 50257 logits; 7e-9 at 96; before, -2e-8 to -9e-8), with a spread of 4.5e-8. Two
+// floats to an instruction, so all this costs 2.8 % of k_stream's time at 50257 logits, 1 % of k_group's at 96, nothing of k_rows',
+// and k_grad gains 6 %. For double it is a polynomial (Num<double>). What a row reports (its log-probability's
+// terms) is computed from the statistics in double by one lane, and sums over rows are double.
 // Everything is summed in a fixed order: the same inputs give the same bits on every call. The bits of a row do
 // depend on how it is split over lanes and blocks, which goes by the vocabulary and the row count.
 #pragma once
@@ -71,16 +75,94 @@ template <typename T> struct Num;
 template <> struct Num<float> {
   static constexpr int VEC = 4;  // elements of a 16-byte vector
   using Vec = float4;
-  // exp(d * scale), given scale * log2 e
-  static __device__ __forceinline__ float exps(float d, float k) {
+  // scale * log2 e in two parts. hi is rounded towards 0 and lo is above 0, so both products have d's sign (-inf stays -inf).
+  struct Scale {
+    float hi, lo;
+    float far;  // the difference at which the exponent is -126
+  };
+  // ex2 is on average 5.0e-8 too small (measured: 5.0e-8 to 5.2e-8 for t from -1 to -120, 2e-8 to 3e-8 above -1): t is raised
+  // by log2(1 + 5.0e-8), before it is rounded. At d = 0 the result is 1.
+  static constexpr float RAISE = 7.2e-8f;
+  static __device__ __forceinline__ float ex2(float t) {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * k));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
     return r;
+  }
+  // exp(d * scale)
+  static __device__ __forceinline__ float exps(float d, Scale k) { return ex2(__fmaf_rn(d, k.hi, __fmaf_rn(d, k.lo, RAISE))); }
+  // The same for differences of about 1, with half the raise: 2e-8 too small on average below -1 / log2 e, 1e-8 too large above.
+  static __device__ __forceinline__ float near(float d, Scale k) { return ex2(__fmaf_rn(d, k.hi, RAISE / 2)); }
+  // The same for d <= 0 without ex2's share, for the factors between parts of a row (each element meets several): 2^t with
+  // t = n + f, n whole and |f| <= 1/2; 2^f by the polynomial of degree 6 that equals it at 7 Chebyshev nodes (with Horner's
+  // roundings off by 1.4 u at most, 1e-9 on average). At d = 0 it is 1; below 2^-126 it is 2^-126.
+  static __device__ __forceinline__ float share(float d, Scale k) {
+    constexpr float C[7] = {0x1.0p+0f, 0x1.62e43p-1f, 0x1.ebfbep-3f, 0x1.c6aeccp-5f, 0x1.3b2a1cp-7f, 0x1.5f48cp-10f, 0x1.444p-13f};
+    constexpr float WHOLE = 12582912.0f;  // 3 * 2^22: adding it rounds to a whole number, in the low bits
+    d = fmaxf(d, k.far);
+    const float w = __fmaf_rn(d, k.hi, WHOLE), f = __fmaf_rn(d, k.lo, __fmaf_rn(d, k.hi, WHOLE - w));
+    float r = C[6];
+#pragma unroll
+    for (int i = 5; i >= 0; --i) r = __fmaf_rn(r, f, C[i]);
+    return r * __int_as_float((__float_as_int(w) + 127) << 23);
+  }
+  // Two floats to an instruction: three additions and products for two logits' exponentials and one for their sum.
+  using Two = unsigned long long;
+  static __device__ __forceinline__ Two two(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+  }
+  static __device__ __forceinline__ void split(Two t, float* a, float* b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(t)); }
+  static __device__ __forceinline__ Two add(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+  }
+  static __device__ __forceinline__ Two mul(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+  }
+  static __device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+  }
+  // x[i] = exps(x[i] - b, k)
+  template <int N> static __device__ __forceinline__ void exps_of(float* x, float b, Scale k) {
+    const Two minus = two(-b, -b), hi = two(k.hi, k.hi), lo = two(k.lo, k.lo), raise = two(RAISE, RAISE);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const Two d = add(two(x[i], x[i + 1]), minus);
+      float t0, t1;
+      split(fma(d, hi, fma(d, lo, raise)), &t0, &t1);
+      x[i] = ex2(t0);
+      x[i + 1] = ex2(t1);
+    }
+  }
+  // Two chains, of the even and the odd elements: half the rounding of one long chain, and half its latency.
+  template <int N> static __device__ __forceinline__ float sum(const float* x) {
+    Two s = two(x[0], x[1]);
+#pragma unroll
+    for (int i = 2; i < N; i += 2) s = add(s, two(x[i], x[i + 1]));
+    float s0, s1;
+    split(s, &s0, &s1);
+    return s0 + s1;
+  }
+  template <int N> static __device__ __forceinline__ void times(float* x, float f) {
+    const Two both = two(f, f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) split(mul(two(x[i], x[i + 1]), both), &x[i], &x[i + 1]);
   }
   static __device__ __forceinline__ float ex(float v) { return expf(v); }
   static __device__ __forceinline__ float ln(float v) { return logf(v); }
   static __device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }  // a NaN gives the other
-  static float factor(double scale) { return (float)(scale * 1.4426950408889634074); }
+  static Scale factor(double scale) {
+    const double k = scale * 1.4426950408889634074;
+    float hi = (float)k;
+    if ((double)hi >= k) hi = std::nextafter(hi, 0.0f);
+    return {hi, (float)(k - (double)hi), -126.0f / hi};
+  }
 };
 template <> struct Num<double> {
   static constexpr int VEC = 2;
@@ -89,12 +171,15 @@ template <> struct Num<double> {
   // degree 11 that equals it at 12 Chebyshev nodes (off by 4.3e-18 relatively; 1.2 u with Horner's roundings).
   // Below 2^-1022 it is 0. (7 x 129 x 10007 without gradient: 28.6 us, with exp() 32.6. The power of two put in by integer
   // operations, 14 instead of 17 double ones: 8192 x 8192 in 190 instead of 165 us, so not those alone bound it.)
-  static __device__ __forceinline__ double exps(double d, double k) {
+  struct Scale {
+    double k;
+  };
+  static __device__ __forceinline__ double exps(double d, Scale k) {
     constexpr double C[12] = {0x1.0000000000000p+0,  0x1.62e42fefa39efp-1,  0x1.ebfbdff82c5aep-3,  0x1.c6b08d704a0c6p-5,
                               0x1.3b2ab6fb9f1a5p-7,  0x1.5d87fe78a3f9cp-10, 0x1.430913112c61bp-13, 0x1.ffcbfc6da6ed1p-17,
                               0x1.62bfc2c86d700p-20, 0x1.b524ebd13a55fp-24, 0x1.e6228acd1c6e5p-28, 0x1.e9ec1fcb69a7fp-32};
     constexpr double WHOLE = 6755399441055744.0;  // 3 * 2^51: adding it rounds to a whole number, in the low bits
-    const double t = d * k, w = t + WHOLE, f = t - (w - WHOLE);
+    const double t = d * k.k, w = t + WHOLE, f = t - (w - WHOLE);
     double r = C[11];
 #pragma unroll
     for (int i = 10; i >= 0; --i) r = __fma_rn(r, f, C[i]);
@@ -102,11 +187,29 @@ template <> struct Num<double> {
     const double two_n = __hiloint2double(__double2hiint(t) >= 0x40900000 ? 0x7ff00000 : (__double2loint(w) + 1023) << 20, 0);
     return t < -1022.0 ? 0.0 : r * two_n;
   }
+  static __device__ __forceinline__ double near(double d, Scale k) { return exps(d, k); }
+  static __device__ __forceinline__ double share(double d, Scale k) { return exps(d, k); }
+  template <int N> static __device__ __forceinline__ void exps_of(double* x, double b, Scale k) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = exps(x[i] - b, k);
+  }
+  template <int N> static __device__ __forceinline__ double sum(const double* x) {
+    double s0 = 0, s1 = 0;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) s0 += x[i], s1 += x[i + 1];
+    return s0 + s1;
+  }
+  template <int N> static __device__ __forceinline__ void times(double* x, double f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= f;
+  }
   static __device__ __forceinline__ double ex(double v) { return exp(v); }
   static __device__ __forceinline__ double ln(double v) { return log(v); }
   static __device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
-  static double factor(double scale) { return scale * 1.4426950408889634074; }
+  static Scale factor(double scale) { return {scale * 1.4426950408889634074}; }
 };
+
+template <typename T> using Scale = typename Num<T>::Scale;
 
 template <typename T> __device__ __forceinline__ T neg_inf() { return -(T)INFINITY; }
 // What exponentials are taken relative to: the maximum, or 0 where there is no finite one yet.
@@ -122,13 +225,14 @@ template <typename T> struct alignas(2 * sizeof(T)) Pair {
   T m, s;
 };
 
-template <int G, typename T> __device__ __forceinline__ Stat<T> join(Stat<T> a, T k) {
+template <int G, bool LONG = false, typename T> __device__ __forceinline__ Stat<T> join(Stat<T> a, Scale<T> k) {
   T m = a.m;
 #pragma unroll
   for (int d = G / 2; d; d >>= 1) {
     m = Num<T>::most(m, __shfl_xor_sync(~0u, m, d));
   }
-  T s = a.s * Num<T>::exps(a.m - base(m), k);
+  const T d = a.m - base(m);
+  T s = a.s * (LONG ? Num<T>::share(d, k) : Num<T>::exps(d, k));
 #pragma unroll
   for (int d = G / 2; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
   return {m, s};
@@ -388,7 +492,7 @@ template <typename T> struct DistillRow {
   const T *teacher, *weight;
   long long k;
   double inverse;  // 1 / T
-  T tk;            // Num<T>::factor(1 / T)
+  Scale<T> tk;     // of 1 / T
   T wt;            // T
   T* terms;
   struct Meta {
@@ -507,38 +611,24 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;
 constexpr int GROUP_THREADS = 256;
 
 // The maximum of a thread's N logits, their exponentials in place and the sum of these.
-template <typename T, int N> __device__ __forceinline__ Stat<T> exponentials(T* x, T k) {
+template <typename T, int N> __device__ __forceinline__ Stat<T> exponentials(T* x, Scale<T> k) {
   Stat<T> a;
 #pragma unroll
   for (int i = 0; i < N; ++i) a.m = Num<T>::most(x[i], a.m);
-  const T b = base(a.m);
-  // Two sums: half the rounding of one long chain, and half its latency.
-  T s0 = (T)0, s1 = (T)0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    x[i] = Num<T>::exps(x[i] - b, k);
-    if (i % 2) s1 += x[i];
-    else s0 += x[i];
-  }
-  a.s = s0 + s1;
+  Num<T>::template exps_of<N>(x, base(a.m), k);
+  a.s = Num<T>::template sum<N>(x);
   return a;
 }
 
 // The same for N more logits of a thread's running maximum and sum: relative to the maximum of both, so one of the two sums
 // needs no factor. (8192 x 8192 doubles 165 us, 180 with two sums joined.)
-template <typename T, int N> __device__ __forceinline__ void extend(Stat<T>& a, T* x, T k) {
+template <typename T, int N> __device__ __forceinline__ void extend(Stat<T>& a, T* x, Scale<T> k) {
   T m = a.m;
 #pragma unroll
   for (int i = 0; i < N; ++i) m = Num<T>::most(x[i], m);
   const T b = base(m);
-  T s0 = (T)0, s1 = (T)0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const T e = Num<T>::exps(x[i] - b, k);
-    if (i % 2) s1 += e;
-    else s0 += e;
-  }
-  a.s = a.s * Num<T>::exps(a.m - b, k) + (s0 + s1);
+  Num<T>::template exps_of<N>(x, b, k);
+  a.s = a.s * Num<T>::near(a.m - b, k) + Num<T>::template sum<N>(x);
   a.m = m;
 }
 
@@ -547,7 +637,7 @@ template <typename T, int N> __device__ __forceinline__ void extend(Stat<T>& a, 
 // its row's lane, so no lane looks for it.
 // What a row needs once is some 400 instructions: with a lane of every group doing it per row, 131072 x 96 took 62 us.
 template <typename T, int G, int E, int B, class Obj, bool GRAD>
-__global__ void __launch_bounds__(GROUP_THREADS, B == 1 && E <= 12 ? 3 : 2) k_group(const View<T> x, const long long rows, const Obj obj, const T k, const Out<T> g) {
+__global__ void __launch_bounds__(GROUP_THREADS, B == 1 && E <= 12 ? 3 : 2) k_group(const View<T> x, const long long rows, const Obj obj, const Scale<T> k, const Out<T> g) {
   constexpr int VEC = Num<T>::VEC, R = 32 / G, ROWS = B * R;
   static_assert(ROWS <= 32, "a lane per row");
   pdl_wait();
@@ -580,8 +670,7 @@ __global__ void __launch_bounds__(GROUP_THREADS, B == 1 && E <= 12 ? 3 : 2) k_gr
 #pragma unroll
       for (int b = 0; b < B; ++b) {
         const T m = __shfl_sync(~0u, st.m, (b * R + group) % 32);
-#pragma unroll
-        for (int q = 0; q < E * VEC; ++q) y[b][q] = Num<T>::exps(y[b][q] - m, k);
+        Num<T>::template exps_of<E * VEC>(y[b], m, k);
       }
     } else {
 #pragma unroll
@@ -630,7 +719,7 @@ __global__ void __launch_bounds__(GROUP_THREADS, B == 1 && E <= 12 ? 3 : 2) k_gr
 // The gradients at the entries are written a second time, over what the row's lanes have stored; the first entry of an
 // index writes its element, with the probabilities of all of that index.
 template <typename T, int G, int E, int B, class Obj, bool GRAD>
-__global__ void __launch_bounds__(GROUP_THREADS, E * B <= 8 ? 4 : E * B <= 10 ? 3 : 2) k_group_targets(const View<T> x, const long long rows, const Obj obj, const T k, const Out<T> g, const int slots) {
+__global__ void __launch_bounds__(GROUP_THREADS, E * B <= 8 ? 4 : E * B <= 10 ? 3 : 2) k_group_targets(const View<T> x, const long long rows, const Obj obj, const Scale<T> k, const Out<T> g, const int slots) {
   constexpr int VEC = Num<T>::VEC, R = 32 / G, ROWS = B * R, TEAM = 32 / ROWS;
   static_assert(ROWS <= 32, "a lane per row");
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -755,11 +844,11 @@ constexpr int MAX_CLUSTER = 8;
 template <typename T, int N> struct Table {
   Pair<T> slot[2][N];
   // By a warp: what the first n of N slots hold together.
-  __device__ __forceinline__ Stat<T> read(int half, int n, T k) const {
+  __device__ __forceinline__ Stat<T> read(int half, int n, Scale<T> k) const {
     Stat<T> a;
     const int lane = threadIdx.x % 32;
     if (lane < n) a = {slot[half][lane].m, slot[half][lane].s};
-    return join<32>(a, k);
+    return join<32, true>(a, k);
   }
 };
 template <typename T> __device__ __forceinline__ Pair<T> pair(Stat<T> a) { return {a.m, a.s}; }
@@ -817,7 +906,7 @@ template <typename T> constexpr int STREAM_UNROLL = 16 / Num<T>::VEC;
 
 // A block, or a cluster of blocks, per row: a running maximum and sum per thread.
 template <typename T, int NT, bool CLUSTER, class Obj>
-__global__ void __launch_bounds__(NT) k_stream(View<T> x, long long rows, Obj obj, T k, int slice) {
+__global__ void __launch_bounds__(NT) k_stream(View<T> x, long long rows, Obj obj, Scale<T> k, int slice) {
   constexpr int VEC = Num<T>::VEC, U = STREAM_UNROLL<T>;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Table<T, NT / 32> table;
@@ -861,7 +950,7 @@ __global__ void __launch_bounds__(NT) k_stream(View<T> x, long long rows, Obj ob
         entries.keep(kept);
       }
     }
-    const Stat<T> of_warp = join<32>(a, k);
+    const Stat<T> of_warp = join<32, true>(a, k);
     if (lane == 0) table.slot[half][warp] = pair(of_warp);
     __syncthreads();
     if constexpr (CLUSTER) {
@@ -894,7 +983,7 @@ __global__ void __launch_bounds__(NT) k_stream(View<T> x, long long rows, Obj ob
 // of 48 warps fit an SM, and 8192 x 8192 took 100 instead of 83 us.
 constexpr int GRAD_THREADS = 256, GRAD_UNROLL = 2, GRAD_VECTORS = 32 * GRAD_UNROLL;
 template <typename T>
-__global__ void __launch_bounds__(GRAD_THREADS, 6) k_grad(View<T> x, long long rows, GivenRow<T> obj, T k, Out<T> g, int pieces) {
+__global__ void __launch_bounds__(GRAD_THREADS, 6) k_grad(View<T> x, long long rows, GivenRow<T> obj, Scale<T> k, Out<T> g, int pieces) {
   constexpr int VEC = Num<T>::VEC, U = GRAD_UNROLL;
   pdl_wait();
   const int lane = threadIdx.x % 32;
@@ -922,12 +1011,16 @@ __global__ void __launch_bounds__(GRAD_THREADS, 6) k_grad(View<T> x, long long r
         }
       }
     }
-    const T f = -q.c / q.s;
+    if (q.live()) {
+      Num<T>::template exps_of<U * VEC>(y, q.m, k);
+      Num<T>::template times<U * VEC>(y, -q.c / q.s);
+    } else {
+#pragma unroll
+      for (int c = 0; c < U * VEC; ++c) y[c] = (T)0;
+    }
     const int l = (int)clamp_label(q.label, x.v) + row.off;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) y[u * VEC + c] = q.live() ? Num<T>::exps(y[u * VEC + c] - q.m, k) * f : (T)0;
       if (q.live() && warp0 + lane + 32 * u == l / VEC) {
 #pragma unroll
         for (int c = 0; c < VEC; ++c)
@@ -961,7 +1054,7 @@ __device__ __forceinline__ double2 load_keep(const double2* p, unsigned long lon
 // 32 warps to an SM with 4 vectors a lane under way: with 48 and 2 16384 logits run at 75 %, with 24 and 8 at 84 %. Doubles:
 // 24 warps and 4 vectors, 8192 x 8192 in 290 us; with 32 and 2 341.
 template <typename T, int NT, bool CLUSTER, class Obj>
-__global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 768) / NT) k_rows(const View<T> x, const long long rows, const __grid_constant__ Obj obj, const T k, const Out<T> g, const int slice) {
+__global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 768) / NT) k_rows(const View<T> x, const long long rows, const __grid_constant__ Obj obj, const Scale<T> k, const Out<T> g, const int slice) {
   constexpr int VEC = Num<T>::VEC, NW = NT / 32, U = 4;
   using Vec = typename Num<T>::Vec;
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -1025,7 +1118,7 @@ __global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 768) / NT) k_rows
         if (first * VEC >= row.hi) entries.gather();
         some = entries.keep(kept);
       }
-      const Stat<T> of_warp = join<32>(a, k);
+      const Stat<T> of_warp = join<32, true>(a, k);
       if (lane == 0) table.slot[half][warp] = pair(of_warp);
       if constexpr (Obj::TARGETS) zero = !__syncthreads_or(some);  // a row without entries counts nothing
       else __syncthreads();
@@ -1056,8 +1149,8 @@ __global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 768) / NT) k_rows
 #pragma unroll
         for (int q = 0; q < U * VEC; ++q) y[q] = (T)0;
       }
-#pragma unroll
-      for (int q = 0; q < U * VEC; ++q) y[q] = Num<T>::exps(y[q] - m_all, k) * f;
+      Num<T>::template exps_of<U * VEC>(y, m_all, k);
+      Num<T>::template times<U * VEC>(y, f);
       if (!zero && l >= i * VEC && l < (i + 32 * U) * VEC) {
 #pragma unroll
         for (int q = 0; q < U * VEC; ++q)
@@ -1284,7 +1377,7 @@ template <typename K, typename... A> cudaError_t go_group(K* kernel, long long r
 // Rows of at most 640 vectors, by the fewest lanes that hold one; some 16 vectors a lane in all, or one row. (516 vectors,
 // 65536 x 2064: 184 us here, 260 by a block per row; with 24 vectors a lane for 750, 65536 x 3000: 273 us here, 269.)
 constexpr long long GROUP_VECTORS = 640;
-template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, const Obj& obj, T k, const RowOut& g, cudaStream_t s) {
+template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, const Obj& obj, Scale<T> k, const RowOut& g, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
   if constexpr (Obj::TARGETS) {
     // Slots for a row's entries: vectors of four, an odd number of them, so that rows begin in different banks.
@@ -1328,7 +1421,7 @@ template <typename T, class Obj> size_t target_bytes(const Obj& obj) {
 }
 
 template <typename T, int NT, bool CLUSTER, class Obj>
-cudaError_t go_rows(const RowView& x, const Obj& obj, T k, const RowOut& g, long long slice, unsigned cluster, cudaStream_t s) {
+cudaError_t go_rows(const RowView& x, const Obj& obj, Scale<T> k, const RowOut& g, long long slice, unsigned cluster, cudaStream_t s) {
   auto* kernel = k_rows<T, NT, CLUSTER, Obj>;
   const size_t smem = target_bytes<T>(obj);
   const long long clusters = std::min(x.rows(), resident(kernel, NT, smem, cluster));
@@ -1337,7 +1430,7 @@ cudaError_t go_rows(const RowView& x, const Obj& obj, T k, const RowOut& g, long
 
 constexpr long long L2_ROWS_BYTES = 80ll << 20;
 // Rows with a gradient that no group holds.
-template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& obj, T k, const RowOut& g, cudaStream_t s) {
+template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& obj, Scale<T> k, const RowOut& g, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
   unsigned c = split(x.rows(), v);
   // Rows under way at once that do not fit the L2 (its two halves hold copies of what the other half's SMs read):
@@ -1357,7 +1450,7 @@ template <typename T, class Obj> cudaError_t block(const RowView& x, const Obj& 
 }
 
 template <typename T, int NT, bool CLUSTER, class Obj>
-cudaError_t go_stream(const RowView& x, const Obj& obj, T k, long long slice, unsigned cluster, cudaStream_t s) {
+cudaError_t go_stream(const RowView& x, const Obj& obj, Scale<T> k, long long slice, unsigned cluster, cudaStream_t s) {
   auto* kernel = k_stream<T, NT, CLUSTER, Obj>;
   const size_t smem = target_bytes<T>(obj);
   const long long clusters = std::min(x.rows(), resident(kernel, NT, smem, cluster));
@@ -1365,7 +1458,7 @@ cudaError_t go_stream(const RowView& x, const Obj& obj, T k, long long slice, un
 }
 
 // Rows without a gradient that no group holds.
-template <typename T, class Obj> cudaError_t stream(const RowView& x, const Obj& obj, T k, cudaStream_t s) {
+template <typename T, class Obj> cudaError_t stream(const RowView& x, const Obj& obj, Scale<T> k, cudaStream_t s) {
   const long long v = most_vectors<T>(x);
   const unsigned c = split(x.rows(), v);
   if (c > 1) return go_stream<T, 256, true>(x, obj, k, pieces_of(v, c), c, s);
@@ -1379,14 +1472,14 @@ template <typename T, class Obj> cudaError_t stream(const RowView& x, const Obj&
 // An objective's rows, with or without their gradient. scale: what the logits are multiplied by.
 template <typename T, class Obj> cudaError_t rows_of(const RowView& x, const Obj& obj, double scale, const RowOut& g, cudaStream_t s) {
   if (x.rows() == 0) return cudaSuccess;
-  const T k = Num<T>::factor(scale);
+  const Scale<T> k = Num<T>::factor(scale);
   if (most_vectors<T>(x) <= GROUP_VECTORS) return g.data ? group<T, Obj, true>(x, obj, k, g, s) : group<T, Obj, false>(x, obj, k, g, s);
   return g.data ? block<T, Obj>(x, obj, k, g, s) : stream<T, Obj>(x, obj, k, s);
 }
 
 template <typename T> cudaError_t given_grad(const RowView& x, const GivenRow<T>& obj, const RowOut& g, cudaStream_t s) {
   if (x.rows() == 0) return cudaSuccess;
-  const T k = Num<T>::factor(1.0);
+  const Scale<T> k = Num<T>::factor(1.0);
   const long long v = most_vectors<T>(x);
   if (v <= GROUP_VECTORS) return group<T, GivenRow<T>, true>(x, obj, k, g, s);
   const long long pieces = pieces_of(v, GRAD_VECTORS), blocks = pieces_of(x.rows() * pieces, GRAD_THREADS / 32);
@@ -1403,7 +1496,7 @@ template <typename T> cudaError_t sum_terms(const void* terms, long long n, void
 template <typename T> cudaError_t log_prob_rows(const RowView& x, const int32_t* labels, const T* weight, T* logp, T* stats, cudaStream_t s) {
   const LogProbRow<T> obj{labels, weight, logp, stats};
   if (x.rows() == 0) return cudaSuccess;
-  const T k = Num<T>::factor(1.0);
+  const Scale<T> k = Num<T>::factor(1.0);
   return most_vectors<T>(x) <= GROUP_VECTORS ? group<T, LogProbRow<T>, false>(x, obj, k, RowOut{}, s) : stream<T, LogProbRow<T>>(x, obj, k, s);
 }
 

@@ -1,0 +1,41 @@
+"""The objectives over logits on the device: errors that all rows share, which a bound per row cannot see, and
+what happens at borders (clip bounds, infinite margins, NaN among the operands)."""
+import numpy as np
+import pytest
+import torch
+
+import objective_reference as R
+from rustautograd_b200 import losses
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def on_device(cuda):
+    pass
+
+
+def put(*arrays):
+    return [torch.from_numpy(np.ascontiguousarray(a)).cuda() for a in arrays]
+
+
+def get(t):
+    return t.cpu().numpy()
+
+
+@pytest.mark.parametrize("rows,v,std", [(4096, 50257, 2.5), (4096, 50257, 1.0), (4096, 131072, 2.5), (8192, 8192, 2.5), (16384, 2049, 2.5), (32768, 1000, 2.5),
+                                        (65536, 96, 2.5)])
+def test_row_sums_have_no_error_in_common(rows, v, std):
+    # A loss is a sum of terms of both signs. The roundings of N rows (u = 6e-8 each) average out as 1 / sqrt(N); an error that
+    # is the same in all of them does not. Allowed: 1e-8, a sixth of u, and four standard errors of the mean.
+    g = torch.Generator("cuda").manual_seed(v + rows)
+    x = torch.randn((rows, v), generator=g, device="cuda") * std
+    _, stats = losses.token_log_prob(x, torch.zeros(rows, dtype=torch.int32, device="cuda"), stats=True)
+    off = []
+    for a in range(0, rows, 1024):
+        y = x[a:a + 1024].double()
+        m = y.amax(-1, keepdim=True)
+        assert torch.equal(stats[a:a + 1024, 0].double(), m[:, 0])
+        off.append(stats[a:a + 1024, 1].double() / torch.exp(y - m).sum(-1) - 1)
+    off = torch.cat(off)
+    assert abs(off.mean().item()) <= 1e-8 + 4 * off.std().item() / rows ** 0.5, (off.mean().item(), off.std().item())
