@@ -940,8 +940,8 @@ template <typename T> void attn_bwd(const Instr& i, std::vector<Buf>& s) {
 }
 
 // Objectives over rows of logits (the device's own ops, no counterpart in rg): the CPU definition
-// the device's kernels are checked against. Row statistics run in index order in T, per-sequence
-// and per-batch sums in double.
+// the device's kernels are checked against. Row statistics run in index order in T; a row's terms
+// are computed from them in double, as are per-sequence and per-batch sums.
 template <typename T> struct LogitRow {
   T m = -std::numeric_limits<T>::infinity(), s = (T)0;
   LogitRow(const T* x, size_t v, T scale) {
@@ -987,24 +987,25 @@ template <typename T> void objective(const Instr& i, std::vector<Buf>& s) {
       }
       break;
     case OpKind::PolicyLoss: {
-      const T low = (T)(1 - objective_attr(i.op, 0)), high = (T)(1 + objective_attr(i.op, 1)), kl = (T)objective_attr(i.op, 2);
+      const double low = 1 - objective_attr(i.op, 0), high = 1 + objective_attr(i.op, 1), kl = objective_attr(i.op, 2);
       double total = 0;
       for (size_t r = 0; r < rows; ++r) {
-        const T w = arg(4)[r], a = arg(3)[r];
-        if (w == (T)0) continue;
+        const double w = arg(4)[r], a = arg(3)[r];
+        if (w == 0) continue;
         const LogitRow<T> st(X + r * v, v, (T)1);
-        const T lp = logp_of(r, st), ratio = std::exp(lp - arg(2)[r]), held = ratio < low ? low : ratio > high ? high : ratio;
-        T term = ratio * a > held * a ? -(held * a) : -(ratio * a);
-        T c = (a >= (T)0 ? ratio <= high : ratio >= low) ? -(ratio * a) : (T)0;
-        if (kl != (T)0) {
-          const T d = arg(5)[r] - lp, e = std::exp(d);
-          term = term + kl * (e - d - (T)1);
-          c = c + kl * ((T)1 - e);
+        const double lp = ((double)X[r * v + label_of(r)] - (double)st.m) - std::log((double)st.s), ratio = std::exp(lp - (double)arg(2)[r]);
+        const double held = ratio < low ? low : ratio > high ? high : ratio;
+        double term = ratio * a > held * a ? -(held * a) : -(ratio * a);
+        double c = (a >= 0 ? ratio <= high : ratio >= low) ? -(ratio * a) : 0;
+        if (kl != 0) {
+          const double d = (double)arg(5)[r] - lp, e = std::exp(d);
+          term = term + kl * (e - d - 1);
+          c = c + kl * (1 - e);
         }
-        out[1][r] = w * term;
-        out[2][r] = lp;
+        out[1][r] = (T)(w * term);
+        out[2][r] = (T)lp;
         total += (double)out[1][r];
-        target_grad(out[3].data() + r * v, X + r * v, v, label_of(r), w * c, st.m, st.s);
+        target_grad(out[3].data() + r * v, X + r * v, v, label_of(r), (T)(w * c), st.m, st.s);
       }
       out[0][0] = (T)total;
       break;

@@ -405,7 +405,7 @@ template <typename T> struct PolicyRow {
   static constexpr bool TARGETS = false, GIVEN = false;
   const int32_t* labels;
   const T *old_logp, *ref_logp, *advantage, *weight;
-  T low, high, kl;  // the ratio's bounds 1 - clip_low and 1 + clip_high
+  double low, high, kl;  // the ratio's bounds 1 - clip_low and 1 + clip_high: as floats, 1.28 and 0.8 are 2e-8 off in every clipped token
   T *terms, *logp;
   struct Meta {
     int label;
@@ -418,7 +418,7 @@ template <typename T> struct PolicyRow {
     m.label = labels[r];
     m.a = advantage[r];
     m.old = old_logp[r];
-    m.ref = kl != (T)0 ? ref_logp[r] : (T)0;
+    m.ref = kl != 0 ? ref_logp[r] : (T)0;
     return m;
   }
   __device__ void skip(long long r) const {
@@ -427,18 +427,18 @@ template <typename T> struct PolicyRow {
   }
   __device__ __forceinline__ T coef(const Meta& m, T xl, Stat<T> st) const {
     const T lp = (xl - st.m) - Num<T>::ln(st.s), ratio = Num<T>::ex(lp - m.old);
-    T c = (m.a >= (T)0 ? ratio <= high : ratio >= low) ? -(ratio * m.a) : (T)0;
-    if (kl != (T)0) c += kl * ((T)1 - Num<T>::ex(m.ref - lp));
+    T c = (m.a >= (T)0 ? ratio <= (T)high : ratio >= (T)low) ? -(ratio * m.a) : (T)0;
+    if (kl != 0) c += (T)kl * ((T)1 - Num<T>::ex(m.ref - lp));
     return m.w * c;
   }
   __device__ __forceinline__ void report(long long r, const Meta& m, T xl, Stat<T> st) const {
     const double lp = ((double)xl - (double)st.m) - log((double)st.s), ratio = exp(lp - (double)m.old), a = m.a;
-    const double held = ratio < (double)low ? (double)low : ratio > (double)high ? (double)high : ratio;
+    const double held = ratio < low ? low : ratio > high ? high : ratio;
     // A NaN ratio or advantage stays NaN through both comparisons.
     double term = ratio * a > held * a ? -(held * a) : -(ratio * a);
-    if (kl != (T)0) {
+    if (kl != 0) {
       const double d = (double)m.ref - lp;
-      term += (double)kl * (exp(d) - d - 1);
+      term += kl * (exp(d) - d - 1);
     }
     terms[r] = (T)((double)m.w * term);
     if (logp) logp[r] = (T)lp;
@@ -1518,9 +1518,9 @@ cudaError_t Objectives<T>::policy(const RowView& x, const int32_t* labels, const
                          (const T*)a.ref_logp,
                          (const T*)a.advantage,
                          (const T*)a.weight,
-                         (T)(1 - a.clip_low),
-                         (T)(1 + a.clip_high),
-                         (T)a.kl,
+                         1 - a.clip_low,
+                         1 + a.clip_high,
+                         a.kl,
                          (T*)terms,
                          (T*)logp};
   const cudaError_t e = rows_of<T>(x, obj, 1.0, g, s);

@@ -39,3 +39,14 @@ def test_row_sums_have_no_error_in_common(rows, v, std):
         off.append(stats[a:a + 1024, 1].double() / torch.exp(y - m).sum(-1) - 1)
     off = torch.cat(off)
     assert abs(off.mean().item()) <= 1e-8 + 4 * off.std().item() / rows ** 0.5, (off.mean().item(), off.std().item())
+
+
+def test_clip_bounds_are_not_rounded():
+    # A clipped token's term is the bound times the advantage, rounded once: half a step, 2^-24 relatively.
+    from test_objectives_exactness import clipped_tokens
+    for v in (8, 3000, 20000):
+        x, lab, old, adv, want = clipped_tokens(np.random.default_rng(v), 512, v)
+        one = torch.ones(512, device="cuda")
+        for grad in (False, True):
+            terms = get(losses.policy_loss(*put(x, lab, old, adv), one, clip_low=0.2, clip_high=0.28, grad=grad).terms)
+            assert (np.abs(terms.astype("f8") - want) <= 2.0 ** -24 * (1 + 1e-6) * np.abs(want)).all(), v
