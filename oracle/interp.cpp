@@ -1023,7 +1023,9 @@ template <typename T> void objective(const Instr& i, std::vector<Buf>& s) {
       for (size_t k = 0; k < pairs; ++k) {
         const double h = beta * ((sum[k] - (double)arg(3)[k]) - (sum[pairs + k] - (double)arg(3)[pairs + k]));
         const double tail = std::log1p(std::exp(-std::fabs(h))), up = 1 / (1 + std::exp(-h)), down = 1 / (1 + std::exp(h));
-        total += std::isnan(h) ? h : (1 - eps) * (tail + std::max(-h, 0.0)) + eps * (tail + std::max(h, 0.0));
+        // A side without weight counts nothing: its logarithm may be infinite.
+        const double chosen = eps < 1 ? (1 - eps) * (tail + std::max(-h, 0.0)) : 0, other = eps > 0 ? eps * (tail + std::max(h, 0.0)) : 0;
+        total += std::isnan(h) ? h : chosen + other;
         out[1][k] = (T)h;
         const T c = (T)(beta * (eps * up - (1 - eps) * down) / (double)pairs);
         for (size_t side = 0; side < 2; ++side)

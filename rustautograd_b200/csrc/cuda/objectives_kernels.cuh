@@ -1273,7 +1273,9 @@ __global__ void __launch_bounds__(PAIR_THREADS) k_pairs(const T* __restrict__ to
     const double e = exp(-fabs(h)), up = h >= 0 ? 1 / (1 + e) : e / (1 + e), down = h >= 0 ? e / (1 + e) : 1 / (1 + e);
     const double tail = log1p(e);
     // -log sigma(h) = tail + max(-h, 0), -log sigma(-h) = tail + max(h, 0)
-    if (lane == 0) terms += h != h ? h : (1 - smoothing) * (tail + (h < 0 ? -h : 0)) + smoothing * (tail + (h > 0 ? h : 0));
+    // (A side without weight counts nothing, however far its answer is out of reach: 0 times infinity would be NaN.)
+    const double chosen = smoothing < 1 ? (1 - smoothing) * (tail + (h < 0 ? -h : 0)) : 0, other = smoothing > 0 ? smoothing * (tail + (h > 0 ? h : 0)) : 0;
+    if (lane == 0) terms += h != h ? h : chosen + other;
     const double dh = beta * (smoothing * up - (1 - smoothing) * down) / (double)pairs;
     if (lane < 2) {
       coef[k + lane * pairs] = (T)(lane ? -dh : dh);

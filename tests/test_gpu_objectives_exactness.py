@@ -50,3 +50,22 @@ def test_clip_bounds_are_not_rounded():
         for grad in (False, True):
             terms = get(losses.policy_loss(*put(x, lab, old, adv), one, clip_low=0.2, clip_high=0.28, grad=grad).terms)
             assert (np.abs(terms.astype("f8") - want) <= 2.0 ** -24 * (1 + 1e-6) * np.abs(want)).all(), v
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("smoothing", [0.0, 0.25, 1.0])
+def test_infinite_margins(smoothing, dtype):
+    from test_objectives_exactness import check_infinite_margins, infinite_margins
+    for v, t in ((6, 3), (3000, 3)):
+        x, lab, w, ref, seq = infinite_margins(dtype, v, t)
+        for pairs, signs in (([0, 2], (np.inf, 0)), ([1, 2], (-np.inf, 0)), ([0, 1, 2], (np.inf, -np.inf, 0))):
+            rows = pairs + [p + 3 for p in pairs]
+            r = losses.preference_loss(*put(x[rows], lab[rows], w[rows], ref[rows]), beta=0.5, smoothing=smoothing)
+            check_infinite_margins(get(r.loss), get(r.margins), get(r.grad), signs, seq, smoothing, np.finfo(dtype).eps / 2 * (v / 32 + 40 + 100))
+            alone = losses.preference_loss(*put(x[rows], lab[rows], w[rows], ref[rows]), beta=0.5, smoothing=smoothing, grad=False)
+            assert torch.equal(alone.loss, r.loss)
+    # Long sequences, where a block takes a pair.
+    x, lab = torch.zeros((2, 300, 4), device="cuda"), torch.zeros((2, 300), dtype=torch.int32, device="cuda")
+    x[1, 7, 0] = -float("inf")
+    r = losses.preference_loss(x, lab, torch.ones((2, 300), device="cuda"), torch.zeros(2, device="cuda"), smoothing=smoothing)
+    assert r.loss.item() == (0 if smoothing == 0 else float("inf")) and r.margins.item() == float("inf")

@@ -35,3 +35,52 @@ def test_clip_bounds_are_not_rounded(cpu):
     one = F.tensor(np.ones(512, "float32"))
     terms = run(lambda x: F.nn.policy_loss(x, F.tensor(lab), F.tensor(old), F.tensor(adv), one, clip_low=0.2, clip_high=0.28)[1], x).numpy()
     assert (np.abs(terms.astype("f8") - want) <= 2.0 ** -24 * (1 + 1e-6) * np.abs(want)).all()
+
+
+# Pairs of which one answer holds a token that its logits ban: margins of +inf (the rejected one), of -inf (the chosen one) and a
+# finite one. By definition the first costs 0 with smoothing 0, the second with smoothing 1; otherwise both cost infinity.
+def infinite_margins(dtype, v=6, t=3):
+    x = np.random.default_rng(2).normal(size=(6, t, v)).astype(dtype)
+    lab = np.zeros((6, t), "int32")
+    x[3, 1, 0] = x[1, 2, 0] = -np.inf  # pairs are (0, 3), (1, 4), (2, 5)
+    z = x.astype("f8")
+    with np.errstate(divide="ignore"):
+        lp = z[..., 0] - np.log(np.exp(z).sum(-1))
+    return x, lab, np.ones((6, t), dtype), np.zeros(6, dtype), lp.sum(1)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("smoothing", [0.0, 0.25, 1.0])
+def test_infinite_margins(cpu, smoothing, dtype):
+    x, lab, w, ref, seq = infinite_margins(dtype)
+    for pairs, signs in (([0, 2], (np.inf, 0)), ([1, 2], (-np.inf, 0)), ([0, 1, 2], (np.inf, -np.inf, 0))):
+        rows = pairs + [p + 3 for p in pairs]
+
+        def f(x):
+            out = F.nn.preference_loss(x, F.tensor(lab[rows]), F.tensor(w[rows]), F.tensor(ref[rows]), 0.5, smoothing)
+            return out[0], out[1]
+        (loss, margins), g = run(F.value_and_grad(f, has_aux=True), x[rows])
+        check_infinite_margins(loss.numpy(), margins.numpy(), g.numpy(), signs, seq, smoothing, 20 * np.finfo(dtype).eps)
+
+
+def check_infinite_margins(loss, margins, g, signs, seq, smoothing, off):
+    n = len(signs)
+    assert np.array_equal(margins[:-1], signs[:-1])
+    h = 0.5 * (seq[2] - seq[5])
+    terms = [np.inf if s and not (s > 0 and smoothing == 0 or s < 0 and smoothing == 1) else 0 for s in signs]
+    terms[-1] = (1 - smoothing) * np.logaddexp(0, -h) + smoothing * np.logaddexp(0, h)
+    want = sum(terms) / n
+    # Two sums of three log-probabilities, each off by `off` at most, times beta (the loss's slope is below 1). For a row of v logits
+    # within 12 of each other that is u (additions + 2.3 * 12 + 4 for the exponentials + 4 log s + 2 |lp|): 40 u for 6 logits.
+    assert loss == want if np.isinf(want) else abs(loss - want) <= 0.5 * 6 * off, (loss, want)
+    assert np.isfinite(g).all()
+    for k, s in enumerate(signs[:-1]):  # the slope of a side that costs nothing is 0, of one that costs infinity +-beta / n
+        still = s > 0 and smoothing == 0 or s < 0 and smoothing == 1
+        assert (not g[[k, n + k]].any()) == still
+
+
+def test_answers_both_out_of_reach_have_no_margin(cpu):
+    x, lab, w, ref, _ = infinite_margins("float32")
+    rows = [1, 2, 3, 5]  # the banned answers against each other, and a pair of others
+    loss, margins, _ = run(lambda x: F.nn.preference_loss(x, F.tensor(lab[rows]), F.tensor(w[rows]), F.tensor(ref[rows])), x[rows])
+    assert np.isnan(loss.numpy()) and np.isnan(margins.numpy()[0]) and np.isfinite(margins.numpy()[1])
