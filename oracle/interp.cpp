@@ -994,9 +994,10 @@ template <typename T> void objective(const Instr& i, std::vector<Buf>& s) {
         if (w == 0) continue;
         const LogitRow<T> st(X + r * v, v, (T)1);
         const double lp = ((double)X[r * v + label_of(r)] - (double)st.m) - std::log((double)st.s), ratio = std::exp(lp - (double)arg(2)[r]);
-        const double held = ratio < low ? low : ratio > high ? high : ratio;
-        double term = ratio * a > held * a ? -(held * a) : -(ratio * a);
-        double c = (a >= 0 ? ratio <= high : ratio >= low) ? -(ratio * a) : 0;
+        // A NaN ratio or advantage is not clipped: the term and the gradient are NaN.
+        const bool clipped = a >= 0 ? ratio > high : a < 0 && ratio < low;
+        double term = clipped ? -((a >= 0 ? high : low) * a) : -(ratio * a);
+        double c = clipped ? 0 : -(ratio * a);
         if (kl != 0) {
           const double d = (double)arg(5)[r] - lp, e = std::exp(d);
           term = term + kl * (e - d - 1);

@@ -425,17 +425,17 @@ template <typename T> struct PolicyRow {
     terms[r] = (T)0;
     if (logp) logp[r] = (T)0;
   }
+  // Whether the bound counts in the ratio's place. A NaN ratio or advantage is not clipped: the term and the gradient are NaN.
+  template <typename F> __device__ __forceinline__ bool clipped(F ratio, F a) const { return a >= 0 ? ratio > (F)high : a < 0 && ratio < (F)low; }
   __device__ __forceinline__ T coef(const Meta& m, T xl, Stat<T> st) const {
     const T lp = (xl - st.m) - Num<T>::ln(st.s), ratio = Num<T>::ex(lp - m.old);
-    T c = (m.a >= (T)0 ? ratio <= (T)high : ratio >= (T)low) ? -(ratio * m.a) : (T)0;
+    T c = clipped(ratio, m.a) ? (T)0 : -(ratio * m.a);
     if (kl != 0) c += (T)kl * ((T)1 - Num<T>::ex(m.ref - lp));
     return m.w * c;
   }
   __device__ __forceinline__ void report(long long r, const Meta& m, T xl, Stat<T> st) const {
     const double lp = ((double)xl - (double)st.m) - log((double)st.s), ratio = exp(lp - (double)m.old), a = m.a;
-    const double held = ratio < low ? low : ratio > high ? high : ratio;
-    // A NaN ratio or advantage stays NaN through both comparisons.
-    double term = ratio * a > held * a ? -(held * a) : -(ratio * a);
+    double term = clipped(ratio, a) ? -((a >= 0 ? high : low) * a) : -(ratio * a);
     if (kl != 0) {
       const double d = (double)m.ref - lp;
       term += kl * (exp(d) - d - 1);

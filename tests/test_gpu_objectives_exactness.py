@@ -69,3 +69,19 @@ def test_infinite_margins(smoothing, dtype):
     x[1, 7, 0] = -float("inf")
     r = losses.preference_loss(x, lab, torch.ones((2, 300), device="cuda"), torch.zeros(2, device="cuda"), smoothing=smoothing)
     assert r.loss.item() == (0 if smoothing == 0 else float("inf")) and r.margins.item() == float("inf")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("v", [40, 3000, 70000])
+def test_nan_among_the_operands_reaches_the_gradient(v, dtype):
+    from test_objectives_exactness import check_nan_operands, nan_operands
+    x, lab, good, bad = nan_operands(np.random.default_rng(v), v, dtype)
+    for kl in (0.0, 0.1):
+        def policy(o):
+            r = losses.policy_loss(*put(x, lab, o["old"], o["adv"], o["w"]), ref_logp=put(o["ref"])[0] if kl else None, kl=kl)
+            return [get(t) for t in r]
+        check_nan_operands(policy(good), policy(bad), kl)
+    # A = 0 and a ratio past the largest number: the bound counts, and the term and its gradient are 0.
+    one = torch.ones(1, dtype=torch.from_numpy(x).dtype, device="cuda")
+    r = losses.policy_loss(*put(x[:1], lab[:1]), one * -1000, one * 0, one)
+    assert r.loss.item() == 0 and not r.grad.any()

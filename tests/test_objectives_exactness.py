@@ -84,3 +84,45 @@ def test_answers_both_out_of_reach_have_no_margin(cpu):
     rows = [1, 2, 3, 5]  # the banned answers against each other, and a pair of others
     loss, margins, _ = run(lambda x: F.nn.preference_loss(x, F.tensor(lab[rows]), F.tensor(w[rows]), F.tensor(ref[rows])), x[rows])
     assert np.isnan(loss.numpy()) and np.isnan(margins.numpy()[0]) and np.isfinite(margins.numpy()[1])
+
+
+def nan_operands(rng, v, dtype):
+    """Operands of a policy loss of 8 rows with kl, of which rows 1 to 6 hold a NaN: in old_logp (with advantages of both signs), in the
+    advantage (with ratios above and below the bounds), in the weight and in the reference."""
+    x, lab = rng.normal(size=(8, v)).astype(dtype), rng.integers(0, v, 8).astype("int32")
+    z = x.astype("f8")
+    lp = z[np.arange(8), lab] - np.log(np.exp(z).sum(1))
+    ops = {"old": lp - np.array([0, 0, 0, 1, -1, 0, 0, 0.0]), "adv": np.array([1.0, 1, -1, 1, -1, 1, 1, -1]), "w": np.ones(8), "ref": lp + 0.1}
+    bad = {k: a.copy() for k, a in ops.items()}
+    bad["old"][1:3] = bad["adv"][3:5] = bad["w"][5] = bad["ref"][6] = np.nan
+    return x, lab, *({k: a.astype(dtype) for k, a in o.items()} for o in (ops, bad))
+
+
+def check_nan_operands(good, bad, kl):
+    rows = [1, 2, 3, 4, 5] + ([6] if kl else [])
+    fine = [r for r in range(8) if r not in rows]
+    (loss, terms, logp, g), (_, good_terms, good_logp, good_g) = bad, good
+    assert np.isnan(loss) and np.isnan(terms[rows]).all() and np.isnan(g[rows]).all()
+    assert np.array_equal(logp, good_logp) and np.array_equal(terms[fine], good_terms[fine]) and np.array_equal(g[fine], good_g[fine])
+    assert np.isfinite(good_g).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("kl", [0.0, 0.1])
+def test_nan_among_the_operands_reaches_the_gradient(cpu, kl, dtype):
+    x, lab, good, bad = nan_operands(np.random.default_rng(3), 9, dtype)
+
+    def policy(o):
+        def f(x):
+            out = F.nn.policy_loss(x, F.tensor(lab), F.tensor(o["old"]), F.tensor(o["adv"]), F.tensor(o["w"]), F.tensor(o["ref"]) if kl else None, kl=kl)
+            return out[0], out[1:]
+        (loss, (terms, logp)), g = run(F.value_and_grad(f, has_aux=True), x)
+        return loss.numpy(), terms.numpy(), logp.numpy(), g.numpy()
+    check_nan_operands(policy(good), policy(bad), kl)
+
+
+def test_no_advantage_costs_nothing_at_any_ratio(cpu):
+    # A = 0 and a ratio past the largest number: the bound counts, and the term and its gradient are 0.
+    x, lab, one = np.zeros((1, 4), "float64"), F.tensor(np.zeros(1, "int32")), F.tensor(np.ones(1))
+    loss, g = run(F.value_and_grad(lambda x: F.nn.policy_loss(x, lab, one * -1000.0, one * 0.0, one)[0]), x)
+    assert loss.numpy() == 0 and not g.numpy().any()
