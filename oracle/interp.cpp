@@ -999,9 +999,9 @@ template <typename T> void objective(const Instr& i, std::vector<Buf>& s) {
         double term = clipped ? -((a >= 0 ? high : low) * a) : -(ratio * a);
         double c = clipped ? 0 : -(ratio * a);
         if (kl != 0) {
-          const double d = (double)arg(5)[r] - lp, e = std::exp(d);
-          term = term + kl * (e - d - 1);
-          c = c + kl * (1 - e);
+          const double d = (double)arg(5)[r] - lp, e = std::expm1(d);
+          term = term + kl * (e - d);
+          c = c - kl * e;
         }
         out[1][r] = (T)(w * term);
         out[2][r] = (T)lp;

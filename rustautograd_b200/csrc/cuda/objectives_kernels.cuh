@@ -155,6 +155,7 @@ template <> struct Num<float> {
     for (int i = 0; i < N; i += 2) split(mul(two(x[i], x[i + 1]), both), &x[i], &x[i + 1]);
   }
   static __device__ __forceinline__ float ex(float v) { return expf(v); }
+  static __device__ __forceinline__ float exm1(float v) { return expm1f(v); }
   static __device__ __forceinline__ float ln(float v) { return logf(v); }
   static __device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }  // a NaN gives the other
   static Scale factor(double scale) {
@@ -204,6 +205,7 @@ template <> struct Num<double> {
     for (int i = 0; i < N; ++i) x[i] *= f;
   }
   static __device__ __forceinline__ double ex(double v) { return exp(v); }
+  static __device__ __forceinline__ double exm1(double v) { return expm1(v); }
   static __device__ __forceinline__ double ln(double v) { return log(v); }
   static __device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
   static Scale factor(double scale) { return {scale * 1.4426950408889634074}; }
@@ -425,20 +427,29 @@ template <typename T> struct PolicyRow {
     terms[r] = (T)0;
     if (logp) logp[r] = (T)0;
   }
+  __device__ __forceinline__ double log_prob(T xl, Stat<T> st) const { return ((double)xl - (double)st.m) - log((double)st.s); }
   // Whether the bound counts in the ratio's place. A NaN ratio or advantage is not clipped: the term and the gradient are NaN.
   template <typename F> __device__ __forceinline__ bool clipped(F ratio, F a) const { return a >= 0 ? ratio > (F)high : a < 0 && ratio < (F)low; }
   __device__ __forceinline__ T coef(const Meta& m, T xl, Stat<T> st) const {
-    const T lp = (xl - st.m) - Num<T>::ln(st.s), ratio = Num<T>::ex(lp - m.old);
-    T c = clipped(ratio, m.a) ? (T)0 : -(ratio * m.a);
-    if (kl != 0) c += (T)kl * ((T)1 - Num<T>::ex(m.ref - lp));
+    const T ls = Num<T>::ln(st.s), lp = (xl - st.m) - ls, d = lp - m.old, ratio = Num<T>::ex(d);
+    bool bound = clipped(ratio, m.a);
+    if constexpr (sizeof(T) == 4) {
+      // The term's ratio is the double one, and the gradient is the term's: a ratio so close to its bound that the roundings decide is
+      // computed again. With u = 2^-24: x - m, lp and d are off by u of themselves, the logarithm and the exponential by 2 u and
+      // 4 u, the bound by u; |x - m| is at most |lp| + log s.
+      const T edge = (T)(m.a >= (T)0 ? high : low);
+      if (fabsf(ratio - edge) <= edge * 0x1p-22f * (fabsf(lp) + ls + fabsf(d) + 2.0f)) bound = clipped(exp(log_prob(xl, st) - (double)m.old), (double)m.a);
+    }
+    T c = bound ? (T)0 : -(ratio * m.a);
+    if (kl != 0) c -= (T)kl * Num<T>::exm1(m.ref - lp);
     return m.w * c;
   }
   __device__ __forceinline__ void report(long long r, const Meta& m, T xl, Stat<T> st) const {
-    const double lp = ((double)xl - (double)st.m) - log((double)st.s), ratio = exp(lp - (double)m.old), a = m.a;
+    const double lp = log_prob(xl, st), ratio = exp(lp - (double)m.old), a = m.a;
     double term = clipped(ratio, a) ? -((a >= 0 ? high : low) * a) : -(ratio * a);
     if (kl != 0) {
       const double d = (double)m.ref - lp;
-      term += kl * (exp(d) - d - 1);
+      term += kl * (expm1(d) - d);
     }
     terms[r] = (T)((double)m.w * term);
     if (logp) logp[r] = (T)lp;

@@ -85,3 +85,43 @@ def test_nan_among_the_operands_reaches_the_gradient(v, dtype):
     one = torch.ones(1, dtype=torch.from_numpy(x).dtype, device="cuda")
     r = losses.policy_loss(*put(x[:1], lab[:1]), one * -1000, one * 0, one)
     assert r.loss.item() == 0 and not r.grad.any()
+
+
+@pytest.mark.parametrize("v", [8, 96, 1000, 2048])
+def test_gradient_is_that_of_the_term_at_a_clip_bound(v):
+    # Ratios within the roundings of a bound: a token is clipped in the gradient where it is in the term, by the ratio of the row's
+    # statistics in double. Float logits; old values a few steps around the one that gives the bound.
+    n, rng = 8192, np.random.default_rng(v)
+    x = rng.normal(size=(n, v)).astype("float32")
+    lab = rng.integers(0, v, n).astype("int32")
+    dx, dl = put(x, lab)
+    stats = get(losses.token_log_prob(dx, dl, stats=True)[1]).astype("f8")
+    lp = (x[np.arange(n), lab].astype("f8") - stats[:, 0]) - np.log(stats[:, 1])
+    up = np.arange(n) % 2 == 0
+    edge = np.where(up, 1 + 0.28, 1 - 0.2)
+    old = (lp - np.log(edge)).astype("float32")
+    for _ in range(3):
+        old = np.where(rng.random(n) < 0.5, np.nextafter(old, np.float32(-100)), old)
+    ratio = np.exp(lp - old.astype("f8"))
+    clipped, sure = np.where(up, ratio > edge, ratio < edge), np.abs(ratio - edge) > 1e-14
+    adv = np.where(up, 1, -1).astype("float32")
+    r = losses.policy_loss(dx, dl, *put(old, adv, np.ones(n, "float32")), clip_low=0.2, clip_high=0.28)
+    assert 0.1 < clipped.mean() < 0.9 and sure.mean() > 0.99
+    assert np.array_equal((get(r.grad) == 0).all(1)[sure], clipped[sure])
+
+
+@pytest.mark.parametrize("v", [40, 3000])
+def test_small_divergences_in_double(v):
+    # A reference next to the policy: exp(d) - d - 1 = d^2 / 2 and its slope -d, by differences that cancel.
+    n, rng = 64, np.random.default_rng(v)
+    x, lab = rng.normal(size=(n, v)), rng.integers(0, v, n).astype("int32")
+    lp = R.log_prob(x, lab)
+    ref = (lp + rng.uniform(0.5, 2, n) * 10.0 ** rng.uniform(-7, -5, n)).astype("f8")
+    d, u, zero = ref.astype(R.L) - lp, 2.0 ** -53, np.zeros(n)
+    r = losses.policy_loss(*put(x, lab, lp.astype("f8"), zero, np.ones(n), ), ref_logp=put(ref)[0], kl=1.0)
+    # d is off by what lp is: u (additions + 2.3 * 12 + 4 for the sum, 4 log s, 4 |lp|), below 300 u here; then expm1 and a difference.
+    off = u * (v / 32 + 40 + 28 + 4 + 4 * 9 + 4 * 12) + 8 * u * np.abs(d)
+    want = np.expm1(d) - d
+    assert (np.abs(get(r.terms) - want) <= np.abs(d) * off).all()
+    slope = get(r.grad)[np.arange(n), lab] / (1 - np.exp(lp.astype("f8")))
+    assert (np.abs(slope + np.expm1(d)) <= off + 16 * u * np.abs(d)).all()
