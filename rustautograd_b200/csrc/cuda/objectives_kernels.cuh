@@ -575,7 +575,7 @@ template <typename T> struct DistillRow {
   // q of an entry with teacher logit t, of all entries' part.
   __device__ __forceinline__ T share(T t, T m, T inverse_s) const { return Num<T>::exps(t - base(m), tk) * inverse_s; }
   __device__ __forceinline__ void report(long long r, const Meta& m, const Part& p, Stat<T> st) const {
-    const double term = (p.a / p.s + ((double)st.m - (double)p.from)) * inverse + (double)Num<T>::ln(st.s) - (double)Num<T>::ln((T)p.s);
+    const double term = (p.a / p.s + ((double)st.m - (double)p.from)) * inverse + log((double)st.s / p.s);
     terms[r] = p.s != 0 ? (T)((double)m.w * (double)wt * (double)wt * term) : (T)0;
   }
 };

@@ -125,3 +125,14 @@ def test_small_divergences_in_double(v):
     assert (np.abs(get(r.terms) - want) <= np.abs(d) * off).all()
     slope = get(r.grad)[np.arange(n), lab] / (1 - np.exp(lp.astype("f8")))
     assert (np.abs(slope + np.expm1(d)) <= off + 16 * u * np.abs(d)).all()
+
+
+@pytest.mark.parametrize("v,k", [(33, 31), (96, 64), (1040, 1000), (3001, 1024), (40000, 1024)])
+def test_distillation_terms_are_rounded_once(v, k):
+    # Equal logits and equal entries: both sums are whole numbers, computed without rounding, and the term is log(v / k): half a
+    # step of its own, 2^-24, with no rounding of the two logarithms (4.8e-7 of a term of 0.04).
+    x, teacher = torch.full((5, v), 3.0, device="cuda"), torch.full((5, k), -2.0, device="cuda")
+    index = torch.arange(k, dtype=torch.int32, device="cuda").flip(0).repeat(5, 1)
+    for grad in (False, True):
+        terms = get(losses.distillation_loss(x, index, teacher, torch.ones(5, device="cuda"), grad=grad).terms).astype("f8")
+        assert (np.abs(terms - np.log(v / k)) <= 2.0 ** -24 * (1 + 1e-6) * np.log(v / k)).all(), (grad, terms)
