@@ -703,6 +703,7 @@ struct Builder {
     if (i.op.kind == OpKind::LogProbGrad) {
       const size_t dst = i.dst;
       fits(dst, o.rows * o.vocab, dt);
+      l.kernels = o.rows ? 1 : 0;
       l.run = [=](Ctx& c) {
         RowView v = x;
         v.data = c.f->ptr[a[0]];
@@ -725,7 +726,11 @@ struct Builder {
     const size_t terms_out = i.op.kind == OpKind::PolicyLoss || i.op.kind == OpKind::DistillLoss ? 1 : SIZE_MAX;
     if (terms_out != SIZE_MAX && out[terms_out] == SIZE_MAX) scratch = std::max(scratch, o.rows * rg::dtype_size(dt));
     if (i.op.kind == OpKind::PreferenceLoss) scratch = std::max(scratch, preference_workspace_bytes(t, x.outer, x.inner));
-    l.kernels = i.op.kind == OpKind::LogProb ? 1 : i.op.kind == OpKind::PreferenceLoss ? 3 + grad : 2;
+    // The rows (statistics; gradient too, but for a preference's, which follows its pairs), then the pairs, or the sum if a step reads it.
+    const int over_rows = o.rows ? 1 : 0;
+    if (i.op.kind == OpKind::LogProb) l.kernels = over_rows;
+    else if (i.op.kind == OpKind::PreferenceLoss) l.kernels = over_rows + 1 + (grad ? over_rows : 0);
+    else l.kernels = over_rows + (out[0] != SIZE_MAX);
     const rg::Op op = i.op;
     const long long teacher = (long long)o.k;
     const size_t grad_out = o.grad_out;

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import objective_reference as R
+from rustautograd_b200 import frontend as F
 from rustautograd_b200 import losses
 
 pytestmark = pytest.mark.gpu
@@ -12,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 @pytest.fixture(autouse=True)
 def on_device(cuda):
-    pass
+    F.use(cuda, "cuda")
 
 
 def put(*arrays):
@@ -136,3 +137,41 @@ def test_distillation_terms_are_rounded_once(v, k):
     for grad in (False, True):
         terms = get(losses.distillation_loss(x, index, teacher, torch.ones(5, device="cuda"), grad=grad).terms).astype("f8")
         assert (np.abs(terms - np.log(v / k)) <= 2.0 ** -24 * (1 + 1e-6) * np.log(v / k)).all(), (grad, terms)
+
+
+def test_launch_counts():
+    # What a program says it launches is what the direct calls launch (the nodes of their captured graphs); a step whose loss
+    # nobody reads has no sum.
+    import ctypes
+    n, t, v = 4, 3, 50
+    rng = np.random.default_rng(0)
+    x, lab = rng.normal(size=(n, t, v)).astype("float32"), rng.integers(0, v, (n, t)).astype("int32")
+    index, row, seq = rng.integers(0, v, (n, t, 5)).astype("int32"), np.ones((n, t), "float32"), np.ones(n, "float32")
+    teacher = rng.normal(size=(n, t, 5)).astype("float32")
+    dx, dl, di, dr, ds, dt = put(x, lab, index, row, seq, teacher)
+    tx, tl, ti, tr, ts, tt = (F.tensor(a) for a in (x, lab, index, row, seq, teacher))
+    cudart = ctypes.CDLL("libcudart.so.12")
+
+    def nodes(call):
+        call()
+        g = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(g):
+            call()
+        count = ctypes.c_size_t()
+        assert cudart.cudaGraphGetNodes(ctypes.c_void_p(g.raw_cuda_graph()), None, ctypes.byref(count)) == 0
+        return count.value
+
+    def launches(f):
+        c = F.compile(f, (tx,), validate="none", device="cuda")
+        c(tx)
+        before = c._n.launches()
+        c(tx)
+        return c._n.launches() - before
+    logp, policy = lambda x: F.nn.token_log_prob(x, tl), lambda x: F.nn.policy_loss(x, tl, tr, tr, tr)[0]
+    preference, distill = lambda x: F.nn.preference_loss(x, tl, tr, ts)[0], lambda x: F.nn.distillation_loss(x, ti, tt, tr)[0]
+    assert launches(logp) == nodes(lambda: losses.token_log_prob(dx, dl)) == 1
+    for grad, of in ((False, lambda f: f), (True, F.value_and_grad)):
+        assert launches(of(policy)) == nodes(lambda: losses.policy_loss(dx, dl, dr, dr, dr, grad=grad)) == 2
+        assert launches(of(distill)) == nodes(lambda: losses.distillation_loss(dx, di, dt, dr, grad=grad)) == 2
+        assert launches(of(preference)) == nodes(lambda: losses.preference_loss(dx, dl, dr, ds, grad=grad)) == 2 + grad
+    assert launches(F.grad(policy)) == launches(F.grad(distill)) == 1 and launches(F.grad(preference)) == 3
