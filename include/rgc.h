@@ -196,7 +196,7 @@ int rgc_policy_loss(const rgc_logits* logits, const int32_t* labels, const rgc_p
  * h = beta ((S - ref_logp) of pair k's chosen sequence - the same of its rejected one), loss = mean over
  * pairs of -(1 - smoothing) log sigma(h) - smoothing log sigma(-h). ref_logp: one per sequence. margins (n,
  * may be NULL) = h, logp (2 n, may be NULL) = S. workspace: rgc_preference_workspace bytes that no
- * other call uses at the same time; its contents need not survive between calls. */
+ * other call uses at the same time (0 for sizes that are refused); its contents need not survive between calls. */
 typedef struct {
   const void *weight, *ref_logp;
   double beta, smoothing;

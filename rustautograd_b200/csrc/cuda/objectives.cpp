@@ -19,6 +19,7 @@ cudaError_t policy_loss(EType t, const RowView& x, const int32_t* labels, const 
                          : Objectives<float>::policy(x, labels, a, loss, terms, logp, grad, s);
 }
 
+// A log-probability and the statistics of each row, a coefficient of each sequence (and a number of each pair that is spare).
 size_t preference_workspace_bytes(EType t, long long sequences, long long length) {
   return (size_t)(3 * sequences * length + 3 * (sequences / 2)) * esize(t);
 }

@@ -70,7 +70,8 @@ Rows check_logits(const rgc_logits* x) {
   if (x->outer < 0 || x->inner < 0) refuse("negative row count");
   if (x->vocab < 1 || x->vocab > (int64_t(1) << 30)) refuse("vocab must be between 1 and 2^30");
   constexpr int64_t LIMIT = int64_t(1) << 40;
-  if (x->inner && x->outer > INT32_MAX / x->inner) refuse("too many rows (at most 2^31 - 1)");
+  // Each of them too: sequences without positions have their pairs all the same.
+  if (x->outer > INT32_MAX || x->inner > INT32_MAX || (x->inner && x->outer > INT32_MAX / x->inner)) refuse("too many rows (at most 2^31 - 1)");
   if (x->outer_stride < 0 || x->inner_stride < 0 || x->outer_stride > LIMIT || x->inner_stride > LIMIT) refuse("strides must be between 0 and 2^40");
   if (x->outer > 0 && x->inner > 0 && extent(*x, x->outer_stride, x->inner_stride) >= int64_t(1) << 60) refuse("the rows span 2^60 elements or more");
   Rows r;
@@ -198,7 +199,7 @@ RGC_EXPORT int rgc_policy_loss(const rgc_logits* logits, const int32_t* labels, 
 }
 
 RGC_EXPORT size_t rgc_preference_workspace(int64_t sequences, int64_t length, int dtype) {
-  if (sequences < 0 || length < 0 || (dtype != 0 && dtype != 1)) return 0;
+  if (sequences < 0 || length < 0 || sequences > INT32_MAX || length > INT32_MAX || (length && sequences > INT32_MAX / length) || (dtype != 0 && dtype != 1)) return 0;
   return preference_workspace_bytes(dtype == 1 ? EType::F64 : EType::F32, sequences, length);
 }
 

@@ -126,3 +126,23 @@ def test_no_advantage_costs_nothing_at_any_ratio(cpu):
     x, lab, one = np.zeros((1, 4), "float64"), F.tensor(np.zeros(1, "int32")), F.tensor(np.ones(1))
     loss, g = run(F.value_and_grad(lambda x: F.nn.policy_loss(x, lab, one * -1000.0, one * 0.0, one)[0]), x)
     assert loss.numpy() == 0 and not g.numpy().any()
+
+
+def test_sizes_past_31_bits_are_refused_without_positions_too(product):
+    # Sequences without positions have no rows, but pairs: as many as would wrap the workspace's size around. Before any CUDA call.
+    import ctypes
+
+    import rustautograd_b200
+    from test_objectives import Logits, Preference
+    lib = ctypes.CDLL(rustautograd_b200.LIBRARY)
+    lib.rgc_last_error.restype = ctypes.c_char_p
+    lib.rgc_preference_workspace.restype = ctypes.c_size_t
+    fake = ctypes.c_void_p(1 << 20)  # never dereferenced
+    for outer, inner in ((1 << 62, 0), (1 << 31, 0), (0, 1 << 31)):
+        for dtype in (0, 1, 256, 257):
+            x, p = Logits(1 << 20, outer, inner, 8, 8, 8, dtype), Preference(fake, fake, 0.1, 0.0)
+            rc = lib.rgc_preference_loss(ctypes.byref(x), fake, ctypes.byref(p), fake, None, None, None, fake, ctypes.c_size_t(0), None)
+            assert rc == -1 and b"too many rows" in lib.rgc_last_error(), (outer, inner, lib.rgc_last_error())
+    for n, t in ((1 << 62, 0), (1 << 31, 0), (1 << 16, 1 << 15), (2, 1 << 62)):
+        assert lib.rgc_preference_workspace(ctypes.c_int64(n), ctypes.c_int64(t), 1) == 0
+    assert lib.rgc_preference_workspace(ctypes.c_int64(2), ctypes.c_int64(0), 1) > 0
