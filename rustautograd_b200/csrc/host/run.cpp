@@ -7,6 +7,7 @@
 #include <tuple>
 
 #include "exec.h"
+#include "objective.h"
 #include "rowchain.h"
 
 namespace rg {
@@ -122,14 +123,24 @@ std::vector<StepCost> step_costs(const Plan& p) {
       c.flops = 2.0 * batch * t * t * (i.op.kind == OpKind::AttnFwd ? d + dv : 3.0 * d + 2.0 * dv);
       c.bytes = in_bytes + (double)i.n * es;
     } else if (i.op.is_objective()) {
-      // The logits once (a preference's gradient reads them again), the gradient, and the small
-      // operands; an exponential, a maximum and a sum per element, a product more for a gradient.
+      // The operands and the results that the plan keeps, once each; a preference's gradient reads the logits again. An
+      // exponential, a maximum and a sum per logit, a product more for a gradient.
       c.kind = "objective";
+      std::vector<DType> dts;
+      for (size_t a : i.args) dts.push_back(p.slots[a].first);
+      Objective o;
+      std::string why;
+      objective_of(i.op, i.arg_shapes, dts, &o, &why);
       const double logits = (double)product(i.arg_shapes[0]);
       bool grad = i.op.kind == OpKind::LogProbGrad;
-      for (auto& o : i.outs) grad = grad || p.slots[o.second].second >= product(i.arg_shapes[0]);
-      const bool twice = grad && i.op.kind == OpKind::PreferenceLoss;
-      c.bytes = in_bytes + (grad ? logits * es : 0.0) + (twice ? logits * es : 0.0);
+      c.bytes = grad ? logits * es : 0.0;
+      for (size_t k = 0; k < i.args.size(); ++k) c.bytes += (double)(product(i.arg_shapes[k]) * dtype_size(dts[k]));
+      for (auto& [index, slot] : i.outs) {
+        (void)slot;
+        grad = grad || index == o.grad_out;
+        c.bytes += (double)product(o.outs.at(index)) * es;
+      }
+      if (grad && i.op.kind == OpKind::PreferenceLoss) c.bytes += logits * es;
       c.flops = logits * (grad ? 6.0 : 3.0);
     } else if (i.op.kind == OpKind::Reduce) {
       c.flops = in_bytes / es;

@@ -146,3 +146,27 @@ def test_sizes_past_31_bits_are_refused_without_positions_too(product):
     for n, t in ((1 << 62, 0), (1 << 31, 0), (1 << 16, 1 << 15), (2, 1 << 62)):
         assert lib.rgc_preference_workspace(ctypes.c_int64(n), ctypes.c_int64(t), 1) == 0
     assert lib.rgc_preference_workspace(ctypes.c_int64(2), ctypes.c_int64(0), 1) > 0
+
+
+def test_step_costs(oracle):
+    # Operands and kept results once each, by their own types, whatever the slots' sizes (a row of one logit is as large as its term).
+    F.use(oracle, "cuda-plan")
+    for v in (1, 2, 50):
+        for es, dtype in ((4, "float32"), (8, "float64")):
+            n, t, k = 6, 5, 3
+            x, row, seq = (F.tensor(np.zeros(s, dtype)) for s in ((n, t, v), (n, t), (n,)))
+            lab, index, teacher = F.zeros((n, t), "int32"), F.zeros((n, t, k), "int32"), F.tensor(np.zeros((n, t, k), dtype))
+
+            def cost(f):
+                (got,) = [c for c in F.compile(f, (x,), validate="none")._n.step_costs() if c[0] == "objective"]
+                return got[1:]
+            rows, logits = n * t, n * t * v
+            cases = [(lambda x: F.nn.policy_loss(x, lab, row, row, row)[0], 4 * rows + 3 * rows * es + es, 1),
+                     (lambda x: F.nn.preference_loss(x, lab, row, seq)[0], 4 * rows + (rows + n) * es + es, 2),
+                     (lambda x: F.nn.distillation_loss(x, index, teacher, row)[0], 4 * rows * k + (rows * k + rows) * es + es, 1)]
+            for f, small, reads in cases:
+                assert cost(f) == (3.0 * logits, logits * es + small)
+                assert cost(F.value_and_grad(f)) == (6.0 * logits, logits * es * (reads + 1) + small)
+            terms = lambda x: F.nn.policy_loss(x, lab, row, row, row)[:2]
+            assert cost(terms) == (3.0 * logits, logits * es + 4 * rows + 3 * rows * es + es + rows * es)
+            assert cost(lambda x: F.nn.token_log_prob(x, lab)) == (3.0 * logits, logits * es + 4 * rows + rows * es)
