@@ -591,7 +591,11 @@ PYBIND11_MODULE(RG_MODULE_NAME, m) {
             j["out"] = Json(outs);
           } else {
             j["in"] = Json(st.instr.args);
-            j["out"] = Json(std::vector<size_t>{st.instr.dst});
+            std::vector<size_t> outs;
+            if (st.instr.op.multi_output())
+              for (auto& o : st.instr.outs) outs.push_back(o.second);
+            else outs.push_back(st.instr.dst);
+            j["out"] = Json(outs);
             j["op"] = st.instr.op.name();
             j["shape"] = Json(st.instr.shape);
             Json args = Json::array();

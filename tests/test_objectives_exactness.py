@@ -170,3 +170,11 @@ def test_step_costs(oracle):
             terms = lambda x: F.nn.policy_loss(x, lab, row, row, row)[:2]
             assert cost(terms) == (3.0 * logits, logits * es + 4 * rows + 3 * rows * es + es + rows * es)
             assert cost(lambda x: F.nn.token_log_prob(x, lab)) == (3.0 * logits, logits * es + 4 * rows + rows * es)
+
+
+def test_plan_summary_names_the_slots_of_every_result(oracle):
+    import json
+    F.use(oracle, "cuda-plan")
+    x, lab, w = F.zeros((3, 7)), F.zeros((3,), "int32"), F.ones((3,))
+    (step,) = json.loads(F.compile(F.value_and_grad(lambda x: F.nn.policy_loss(x, lab, w, w, w)[0]), (x,), validate="none")._n.plan_summary())
+    assert len(step["out"]) == 2 and max(step["out"]) < 100 and len(set(step["out"] + step["in"])) == len(step["out"]) + len(set(step["in"]))
