@@ -1094,6 +1094,14 @@ __global__ void k_index_outside(const int32_t* idx, long long n, long long dim, 
   }
 }
 
+// The same for `per` indices of each row, without rows of weight 0 and teacher entries (null: none) of -inf.
+template <typename T> __global__ void k_index_outside_counted(const int32_t* idx, long long n, long long per, long long dim, const T* weight, const T* teacher, int* flag) {
+  pdl_wait();
+  GRID_STRIDE(i, n) {
+    if ((idx[i] < 0 || idx[i] >= dim) && weight[i / per] != (T)0 && !(teacher && teacher[i] == -(T)INFINITY)) *flag = 1;
+  }
+}
+
 template <typename T> __global__ void k_nonfinite(const T* a, long long n, int* flag) {
   pdl_wait();
   GRID_STRIDE(i, n) {
@@ -1517,6 +1525,16 @@ void write_count(int32_t* dst, const long long* count, cudaStream_t s) { launch(
 void index_outside(const int32_t* idx, long long n, long long dim, int* flag, cudaStream_t s) {
   if (n <= 0) return;
   launch(k_index_outside, grid_k(k_index_outside, n), 256, 0, s, idx, n, dim, flag);
+}
+
+void index_outside_counted(const int32_t* idx, long long n, long long per, long long dim, const void* weight, const void* teacher, EType t, int* flag, cudaStream_t s) {
+  if (n <= 0) return;
+  auto go = [&](auto* kernel, auto one) {
+    using T = decltype(one);
+    launch(kernel, grid_k(kernel, n), 256, 0, s, idx, n, per, dim, (const T*)weight, (const T*)teacher, flag);
+  };
+  if (t == EType::F64) go(k_index_outside_counted<double>, 0.0);
+  else go(k_index_outside_counted<float>, 0.0f);
 }
 
 void any_nonfinite(const void* src, EType t, long long n, int* flag, cudaStream_t s) {

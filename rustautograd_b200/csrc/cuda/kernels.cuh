@@ -127,6 +127,8 @@ void set_conditional(cudaGraphConditionalHandle h, const void* pred, EType t, lo
 void write_count(int32_t* dst, const long long* count, cudaStream_t s);
 // Any index outside [0, dim) -> *flag = 1.
 void index_outside(const int32_t* idx, long long n, long long dim, int* flag, cudaStream_t s);
+// The same for `per` indices of each row, without rows of weight 0 and teacher entries (null: none) of -inf.
+void index_outside_counted(const int32_t* idx, long long n, long long per, long long dim, const void* weight, const void* teacher, EType t, int* flag, cudaStream_t s);
 
 // Up to SEGMENTS_MAX float segments copied in one launch (the gradients of a data-parallel
 // step gathered into one contiguous buffer for a single all-reduce, and scattered back).

@@ -2086,6 +2086,16 @@ __attribute__((visibility("default"))) int rgc_exec_step_checked(rgc_exec* e, in
         const size_t dim = i.op.kind == OpKind::Take ? i.arg_shapes[0][i.op.index] : i.arg_shapes[0].back();
         index_outside((const int32_t*)e->f->ptr[i.args[1]], (long long)rg::product(i.arg_shapes[1]), (long long)dim, dflags + n + k, s);
       }
+      if (!st.fused && st.instr.op.is_objective()) {
+        const Instr& i = st.instr;
+        std::vector<DType> dts;
+        for (size_t a : i.args) dts.push_back(plan.slots[a].first);
+        rg::Objective o;
+        std::string why;
+        if (rg::objective_of(i.op, i.arg_shapes, dts, &o, &why) && o.weight_arg != SIZE_MAX)
+          index_outside_counted((const int32_t*)e->f->ptr[i.args[1]], (long long)rg::product(i.arg_shapes[1]), (long long)o.k, (long long)o.vocab,
+                                e->f->ptr[i.args[o.weight_arg]], o.teacher_arg == SIZE_MAX ? nullptr : e->f->ptr[i.args[o.teacher_arg]], et(dts[0]), dflags + n + k, s);
+      }
       p->steps[k].run(c);
       if (st.fused) {
         for (auto& o : st.group.outputs) check(o.second, st.group.n, dflags + k);

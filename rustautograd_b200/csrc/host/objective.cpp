@@ -63,6 +63,7 @@ bool objective_of(const Op& op, const std::vector<std::vector<size_t>>& s, const
       if ((objective_attr(op, 2) != 0) != (s.size() == 6)) return no("reference_log_probabilities_go_with_a_kl_coefficient");
       o.outs = {{}, lead, lead, s[0]};
       o.grad_out = 3;
+      o.weight_arg = 4;
       break;
     }
     case OpKind::PreferenceLoss:
@@ -74,6 +75,7 @@ bool objective_of(const Op& op, const std::vector<std::vector<size_t>>& s, const
       o.inner = lead[1];
       o.outs = {{}, {lead[0] / 2}, {lead[0]}, s[0]};
       o.grad_out = 3;
+      o.weight_arg = 2;
       break;
     default:
       if (s[1].empty() || s[1].back() == 0 || s[1].back() > MAX_TEACHER) return no("teacher_needs_between_1_and_1024_entries_per_row");
@@ -83,6 +85,8 @@ bool objective_of(const Op& op, const std::vector<std::vector<size_t>>& s, const
       if (!attrs_ok(op, 1) || !(objective_attr(op, 0) >= 0x1p-60 && objective_attr(op, 0) <= 0x1p60)) return no("temperature_must_be_between_2^-60_and_2^60");
       o.outs = {{}, lead, s[0]};
       o.grad_out = 2;
+      o.weight_arg = 3;
+      o.teacher_arg = 2;
   }
   *out = std::move(o);
   return true;

@@ -12,11 +12,14 @@ namespace rg {
 struct Objective {
   size_t rows = 0, vocab = 0;
   size_t outer = 0, inner = 0;  // rows as outer x inner: PreferenceLoss's sequences x positions, else rows x 1
-  size_t k = 0;                 // DistillLoss: teacher entries per row
+  size_t k = 1;                 // indices per row: DistillLoss's teacher entries
   std::vector<std::vector<size_t>> outs;  // the shapes of outputs 0, 1, ... (none for LogProbGrad)
   // Output 0 is the value that is differentiated; this output is its gradient with respect to the
   // logits (SIZE_MAX for LogProb, whose gradient is the LogProbGrad operation).
   size_t grad_out = SIZE_MAX;
+  // The operands that say which indices (operand 1, k to a row) count: rows with weight 0 do not, nor do teacher entries of -inf.
+  // SIZE_MAX: all do.
+  size_t weight_arg = SIZE_MAX, teacher_arg = SIZE_MAX;
 };
 
 // The objective `op` on operands of the given shapes and dtypes; false and the reason when they do not fit.

@@ -1,6 +1,8 @@
 // Restates src/validate.rs (line references below are to that file).
 #include "validate.h"
 
+#include "objective.h"
+
 #include <algorithm>
 #include <chrono>
 #include <cmath>
@@ -71,6 +73,15 @@ Stats stats(const Buf& b, size_t n) {
     if (!s.first_bad) s.first_bad = i;
   }
   return s;
+}
+
+// An objective's indices with those that do not count as 0.
+Buf counted(const Objective& obj, Buf index, size_t n, const Buf& weight, const Buf& teacher) {
+  for (size_t r = 0; r < n; ++r) {
+    const bool absent = obj.teacher_arg != SIZE_MAX && teacher.get(r) == -INFINITY;
+    if (absent || weight.get(r / obj.k) == 0.0) index.i32()[r] = 0;
+  }
+  return index;
 }
 
 bool any_nonfinite(const Buf& b, size_t n) {
@@ -250,13 +261,21 @@ Compiled::Observed Compiled::observed(const std::vector<Tensor>& inputs) const {
     const Step& st = raw_plan.steps[k];
     if (st.fused) continue;  // reference plans have no groups
     const Instr& i = st.instr;
-    // Index check (validate.rs:177-190).
+    // Index check (validate.rs:177-190); an objective's indices that count (objective.h).
     size_t dim = 0;
+    std::vector<DType> dts;
+    for (size_t a : i.args) dts.push_back(raw_plan.slots[a].first);
+    Objective obj;
+    std::string why;
     if (i.op.kind == OpKind::Take) dim = i.arg_shapes[0][i.op.index];
-    else if (i.op.kind == OpKind::TakeAlong || i.op.kind == OpKind::LogProb) dim = i.arg_shapes[0].back();
+    else if (i.op.kind == OpKind::TakeAlong) dim = i.arg_shapes[0].back();
+    else if (i.op.is_objective() && objective_of(i.op, i.arg_shapes, dts, &obj, &why)) dim = obj.vocab;
     if (dim) {
       size_t n = product(i.arg_shapes[1]);
-      Stats s = stats(e->prefix(i.args[1], n), n);
+      Buf index = e->prefix(i.args[1], n);
+      if (obj.weight_arg != SIZE_MAX) index = counted(obj, index, n, e->prefix(i.args[obj.weight_arg], obj.rows),
+                                                      obj.teacher_arg == SIZE_MAX ? Buf() : e->prefix(i.args[obj.teacher_arg], n));
+      Stats s = stats(index, n);
       if (n > 0 && (s.min < 0.0 || s.max >= (double)dim) && o.hard.size() < MAX_ROOTS) {
         Json obs = Json::object();
         obs["index_min"] = s.min;

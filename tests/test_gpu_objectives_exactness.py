@@ -175,3 +175,8 @@ def test_launch_counts():
         assert launches(of(distill)) == nodes(lambda: losses.distillation_loss(dx, di, dt, dr, grad=grad)) == 2
         assert launches(of(preference)) == nodes(lambda: losses.preference_loss(dx, dl, dr, ds, grad=grad)) == 2 + grad
     assert launches(F.grad(policy)) == launches(F.grad(distill)) == 1 and launches(F.grad(preference)) == 3
+
+
+def test_labels_that_count_are_checked():
+    from test_objectives_exactness import check_labels
+    check_labels("cuda")

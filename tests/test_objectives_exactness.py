@@ -178,3 +178,39 @@ def test_plan_summary_names_the_slots_of_every_result(oracle):
     x, lab, w = F.zeros((3, 7)), F.zeros((3,), "int32"), F.ones((3,))
     (step,) = json.loads(F.compile(F.value_and_grad(lambda x: F.nn.policy_loss(x, lab, w, w, w)[0]), (x,), validate="none")._n.plan_summary())
     assert len(step["out"]) == 2 and max(step["out"]) < 100 and len(set(step["out"] + step["in"])) == len(step["out"]) + len(set(step["in"]))
+
+
+def label_cases():
+    """(what, function of the logits, whether the engine's check refuses its labels) for logits (4, 3, 6): an index outside the vocabulary
+    at a position that counts, and at positions that do not (weight 0, an absent teacher entry)."""
+    rng = np.random.default_rng(5)
+    row, seq = F.tensor(rng.random((4, 3)).astype("float32")), F.tensor(np.zeros(4, "float32"))
+    lab, index, w = rng.integers(0, 6, (4, 3)).astype("int32"), rng.integers(0, 6, (4, 3, 2)).astype("int32"), np.ones((4, 3), "float32")
+    teacher = rng.normal(size=(4, 3, 2)).astype("float32")
+    for bad in (None, -100, -1, 6):
+        for weight in (1.0, -1.0, 0.0):
+            l, i, ww, t = lab.copy(), index.copy(), w.copy(), teacher.copy()
+            if bad is not None:
+                l[2, 1] = i[2, 1, 1] = bad
+            ww[2, 1] = weight
+            refused = bad is not None and weight != 0
+            l, i, ww = F.tensor(l), F.tensor(i), F.tensor(ww)
+            yield ("policy", bad, weight), lambda x, l=l, ww=ww: F.nn.policy_loss(x, l, row, row, ww)[0], refused
+            yield ("preference", bad, weight), lambda x, l=l, ww=ww: F.nn.preference_loss(x, l, ww, seq)[0], refused
+            yield ("distillation", bad, weight), lambda x, i=i, ww=ww: F.nn.distillation_loss(x, i, F.tensor(teacher), ww)[0], refused
+            t[2, 1, 1] = -np.inf
+            yield ("absent", bad, weight), lambda x, i=i, ww=ww, t=t: F.nn.distillation_loss(x, i, F.tensor(t), ww)[0], False
+
+
+def check_labels(device):
+    x = F.tensor(np.random.default_rng(6).normal(size=(4, 3, 6)).astype("float32"))
+    for what, f, refused in label_cases():
+        report = F.compile(lambda x: F.value_and_grad(f)(x), (x,), validate="standard", device=device).report
+        codes = [d["code"] for d in report["diagnostics"]]
+        assert ("INDEX_OUT_OF_RANGE" in codes) == refused and (report["status"] == "validation_failed") == refused, (what, report)
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda-plan"])
+def test_labels_that_count_are_checked(oracle, device):
+    F.use(oracle, device)
+    check_labels(device)
