@@ -180,3 +180,45 @@ def test_launch_counts():
 def test_labels_that_count_are_checked():
     from test_objectives_exactness import check_labels
     check_labels("cuda")
+
+
+def check_step(names, before, gpu, cpu, what):
+    """A step's outputs (count, first and second moments, parameters, then the loss and what goes with it) against the interpreter's, each
+    leaf at its own size. From zero moments the first one is a tenth of the gradient."""
+    from helpers import max_rel
+    from test_gpu_baseline_configs import TOL, check_gradient, check_parameter
+    n = len(names)
+    assert gpu[0] == cpu[0] == 1
+    for k in range(n):
+        check_gradient(f"{what}: mu {names[k]}", gpu[1 + k], cpu[1 + k])
+        check_gradient(f"{what}: nu {names[k]}", gpu[1 + n + k], cpu[1 + n + k])
+        check_parameter(f"{what}: {names[k]}", before[k], gpu[1 + 2 * n + k], cpu[1 + 2 * n + k], gpu[1 + k], gpu[1 + n + k], cpu[1 + k] / 0.1)
+    assert len(gpu) > 1 + 3 * n
+    for g, w in zip(gpu[1 + 3 * n:], cpu[1 + 3 * n:]):
+        assert max_rel(g, w) <= TOL, (what, g, w)
+
+
+def test_training_steps_against_the_interpreter(oracle):
+    from helpers import np_of, triple
+    from test_gpu_baseline_configs import leaf_paths
+    from test_objectives import gpt_batches
+    rng = np.random.default_rng(13)
+    model = F.gpt.GPT(vocab=40, block=16, d=32, heads=4, layers=2)
+    params, opt = model.init(F.random.key(0)), F.optim.adamw(1e-3)
+    state, names = {"params": params, "opt": opt.init(params)}, leaf_paths(params)
+    policy, preference, distill = gpt_batches(rng, 6, 16, 40, 5)
+    for what, step, batch in (("policy", F.gpt.make_policy_step(model, opt, kl=0.05), policy), ("preference", F.gpt.make_preference_step(model, opt), preference),
+                              ("distillation", F.gpt.make_distillation_step(model, opt, 2.0), distill)):
+        c = F.compile(step, (state, batch), validate="none", device="cuda")
+        leaves = [F.tensor(leaf) for leaf in F.flatten((state, batch))[0]]
+        cpu = [np_of(o) for o in oracle.run_plan_blob(c.plan_blob(), [triple(leaf) for leaf in leaves])]
+        gpu = [F.Tensor(o).numpy() for o in c._n.call([leaf._t for leaf in leaves])]
+        before = [t.numpy() for t in F.tree_leaves(params)]
+        check_step(names, before, gpu, cpu, what)
+        # The check sees a gradient that is missing or off by a thousandth in any leaf, and an update that was left out.
+        for k in range(len(names)):
+            for wrong in (0.0, 1.001):
+                with pytest.raises(AssertionError):
+                    check_step(names, before, gpu, [a * np.float32(wrong) if j == 1 + k else a for j, a in enumerate(cpu)], what)
+            with pytest.raises(AssertionError):
+                check_step(names, before, [before[k] if j == 1 + 2 * len(names) + k else a for j, a in enumerate(gpu)], cpu, what)
