@@ -63,7 +63,7 @@ class _Call:
     """The logits of a call, where their gradient goes, and the stream it runs on. `sequences`: the leading
     axes are (sequences, positions) as they are."""
 
-    __slots__ = ("logits", "index", "dtype", "lead", "grad", "args", "grad_args")
+    __slots__ = ("logits", "index", "dtype", "lead", "grad", "args", "grad_args", "out")
 
     def __init__(self, logits, grad=False, out=None, sequences=False):
         if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
@@ -75,7 +75,7 @@ class _Call:
         shape = logits.shape
         if sequences and len(shape) != 3:
             raise ValueError("logits must be (sequences, positions, vocabulary)")
-        self.logits, self.index, self.lead = logits, logits.get_device(), shape[:-1]
+        self.logits, self.index, self.lead, self.out = logits, logits.get_device(), shape[:-1], out
         if out is not None:
             if not grad:
                 raise ValueError("out is given but no gradient is asked for")
@@ -117,6 +117,8 @@ class _Call:
         else:
             with torch.cuda.device(self.index):
                 call(self.args, *args, _stream(self.index))
+        if self.out is not None:  # autograd refuses what it has saved of the tensor's former contents
+            torch.autograd.graph.increment_version(self.out)
 
 
 def token_log_prob(logits, labels, *, stats=False):

@@ -222,3 +222,20 @@ def test_training_steps_against_the_interpreter(oracle):
                     check_step(names, before, gpu, [a * np.float32(wrong) if j == 1 + k else a for j, a in enumerate(cpu)], what)
             with pytest.raises(AssertionError):
                 check_step(names, before, [before[k] if j == 1 + 2 * len(names) + k else a for j, a in enumerate(gpu)], cpu, what)
+
+
+def test_overwritten_logits_are_known_to_autograd():
+    # exp keeps its result for its gradient; once that memory holds the loss's gradient, going back through it is refused.
+    lab, w = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.ones(4, device="cuda")
+    stats = losses.token_log_prob(torch.ones(4, 9, device="cuda"), lab, stats=True)[1]
+    calls = [lambda x: losses.token_log_prob_grad(x, lab, stats, w, out=x), lambda x: losses.policy_loss(x, lab, -w, w, w, out=x),
+             lambda x: losses.preference_loss(x.view(2, 2, 9), lab.view(2, 2), w.view(2, 2), w[:2], out=x.view(2, 2, 9)),
+             lambda x: losses.distillation_loss(x, lab[:, None], w[:, None], w, out=x)]
+    for call in calls:
+        x = torch.zeros(4, 9, device="cuda", requires_grad=True)
+        y = x.exp()
+        losses.token_log_prob(y.detach(), lab)
+        y.sum().backward(retain_graph=True)
+        call(y.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
