@@ -1043,17 +1043,6 @@ __global__ void __launch_bounds__(GRAD_THREADS, 6) k_grad(View<T> x, long long r
   }
 }
 
-// Loads that the L2 holds on to longer than what is stored meanwhile: 32000 logits 86 -> 88 % of the copy rate.
-__device__ __forceinline__ float4 load_keep(const float4* p, unsigned long long policy) {
-  float4 z;
-  asm volatile("ld.global.L2::cache_hint.v4.f32 {%0,%1,%2,%3}, [%4], %5;" : "=f"(z.x), "=f"(z.y), "=f"(z.z), "=f"(z.w) : "l"(p), "l"(policy));
-  return z;
-}
-__device__ __forceinline__ double2 load_keep(const double2* p, unsigned long long policy) {
-  double2 z;
-  asm volatile("ld.global.L2::cache_hint.v2.f64 {%0,%1}, [%2], %3;" : "=d"(z.x), "=d"(z.y) : "l"(p), "l"(policy));
-  return z;
-}
 // ---- longer rows with a gradient ----
 
 // A block of NT threads, or a cluster of such blocks (`slice` vectors each), per row: one pass for the statistics and
@@ -1063,7 +1052,9 @@ __device__ __forceinline__ double2 load_keep(const double2* p, unsigned long lon
 // way): 83 against 57 % of the copy rate at 50257 logits and 88 against 69 % at 32000, where a row needs a cluster of
 // blocks and each waits for the slowest; 91 against 85 % at 16384, where one block holds it.
 // 32 warps to an SM with 4 vectors a lane under way: with 48 and 2 16384 logits run at 75 %, with 24 and 8 at 84 %. Doubles:
-// 24 warps and 4 vectors, 8192 x 8192 in 290 us; with 32 and 2 341.
+// 24 warps and 4 vectors, 8192 x 8192 in 290 us; with 32 and 2 341. The first pass asks the L2 for nothing special: lines marked to
+// be evicted last gain 2 of 183 us at 4096 x 32000, nothing at 16384 x 50257, and stay behind: two sums over the same 64 MB
+// after the loss then take 53 us instead of 46.
 template <typename T, int NT, bool CLUSTER, class Obj>
 __global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 768) / NT) k_rows(const View<T> x, const long long rows, const __grid_constant__ Obj obj, const Scale<T> k, const Out<T> g, const int slice) {
   constexpr int VEC = Num<T>::VEC, NW = NT / 32, U = 4;
@@ -1076,8 +1067,6 @@ __global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 768) / NT) k_rows
   const int slots = Entries<T, NT, Obj>::slots(obj);
   pdl_wait();
   if constexpr (CLUSTER) cluster_sync();  // every block's shared memory is there before another writes to it
-  unsigned long long policy;
-  asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
   const long long step = gridDim.x / blocks;
   long long r = blockIdx.x / blocks;
   int half = 0;
@@ -1094,7 +1083,7 @@ __global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 768) / NT) k_rows
         const Vec* from = reinterpret_cast<const Vec*>(row.base) + (i + lane);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const Vec z = last ? __ldcs(from + 32 * u) : load_keep(from + 32 * u, policy);
+          const Vec z = last ? __ldcs(from + 32 * u) : from[32 * u];
           memcpy(y + u * VEC, &z, 16);
         }
       } else {
