@@ -60,7 +60,6 @@ cudaError_t preference_loss(EType t, const RowView& x, const int32_t* labels, co
 // q = softmax(teacher / T) over the k entries of a row (entries of -inf are absent), p = softmax(x / T);
 // terms[r] = w T^2 sum_k q_k (log q_k - log p_{i_k}), loss their sum. An index given twice counts twice;
 // rows with w = 0 or without entries give 0. Indices are clamped to [0, V).
-constexpr long long DISTILL_MAX_K = 1024;
 struct DistillArgs {
   const int32_t* index = nullptr;
   const void *teacher = nullptr, *weight = nullptr;

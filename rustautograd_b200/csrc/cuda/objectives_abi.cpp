@@ -6,6 +6,7 @@
 #include <exception>
 #include <string>
 
+#include "objective.h"
 #include "objectives.cuh"
 #include "rgc.h"
 
@@ -62,16 +63,21 @@ int64_t extent(const rgc_logits& x, int64_t so, int64_t si) {
   return all < 0x1p60 ? (x.outer - 1) * so + (x.inner - 1) * si + x.vocab : int64_t(1) << 60;
 }
 
+// Rows, or either factor of them: sequences without positions have their pairs all the same.
+bool too_many(int64_t outer, int64_t inner) {
+  constexpr int64_t most = rg::OBJECTIVE_MAX_ROWS;
+  return outer > most || inner > most || (inner && outer > most / inner);
+}
+
 // The sizes, types and strides (before any CUDA call).
 Rows check_logits(const rgc_logits* x) {
   if (!x) refuse("null argument");
   const int dtype = x->dtype & ~RGC_VOUCHED;
   if (dtype != 0 && dtype != 1) refuse("dtype must be 0 (float32) or 1 (float64)");
   if (x->outer < 0 || x->inner < 0) refuse("negative row count");
-  if (x->vocab < 1 || x->vocab > (int64_t(1) << 30)) refuse("vocab must be between 1 and 2^30");
+  if (x->vocab < 1 || x->vocab > (int64_t)rg::OBJECTIVE_MAX_VOCAB) refuse("vocab must be between 1 and 2^30");
   constexpr int64_t LIMIT = int64_t(1) << 40;
-  // Each of them too: sequences without positions have their pairs all the same.
-  if (x->outer > INT32_MAX || x->inner > INT32_MAX || (x->inner && x->outer > INT32_MAX / x->inner)) refuse("too many rows (at most 2^31 - 1)");
+  if (too_many(x->outer, x->inner)) refuse("too many rows (at most 2^31 - 1)");
   if (x->outer_stride < 0 || x->inner_stride < 0 || x->outer_stride > LIMIT || x->inner_stride > LIMIT) refuse("strides must be between 0 and 2^40");
   if (x->outer > 0 && x->inner > 0 && extent(*x, x->outer_stride, x->inner_stride) >= int64_t(1) << 60) refuse("the rows span 2^60 elements or more");
   Rows r;
@@ -199,7 +205,7 @@ RGC_EXPORT int rgc_policy_loss(const rgc_logits* logits, const int32_t* labels, 
 }
 
 RGC_EXPORT size_t rgc_preference_workspace(int64_t sequences, int64_t length, int dtype) {
-  if (sequences < 0 || length < 0 || sequences > INT32_MAX || length > INT32_MAX || (length && sequences > INT32_MAX / length) || (dtype != 0 && dtype != 1)) return 0;
+  if (sequences < 0 || length < 0 || too_many(sequences, length) || (dtype != 0 && dtype != 1)) return 0;
   return preference_workspace_bytes(dtype == 1 ? EType::F64 : EType::F32, sequences, length);
 }
 
@@ -237,7 +243,7 @@ RGC_EXPORT int rgc_distillation_loss(const rgc_logits* logits, const rgc_distill
   return entry("rgc_distillation_loss", [&] {
     const Rows r = check_logits(logits);
     if (!p) refuse("null argument");
-    if (p->entries < 1 || p->entries > DISTILL_MAX_K) refuse("teacher entries per row must be between 1 and " + std::to_string(DISTILL_MAX_K));
+    if (p->entries < 1 || p->entries > (int64_t)rg::OBJECTIVE_MAX_ENTRIES) refuse("teacher entries per row must be between 1 and " + std::to_string(rg::OBJECTIVE_MAX_ENTRIES));
     if (!(p->temperature >= 0x1p-60 && p->temperature <= 0x1p60)) refuse("temperature must be between 2^-60 and 2^60");  // 1 / T and T^2 in a float
     const RowOut g = check_gradient(*logits, r, grad);
     const int dev = device_of(r);

@@ -1208,7 +1208,7 @@ __device__ double block_sum(double v, double* sh) {
 // A cluster's blocks, or one block, add up the terms: eight of a thread at a time, then threads, warps and blocks in order.
 // (131072 terms: 6 us; sixteen at a time with a bound on each load 11.)
 constexpr int SUM_THREADS = 512, SUM_CLUSTER = 8, SUM_AHEAD = 8;
-template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms(const T* __restrict__ terms, long long n, T* loss, double scale) {
+template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms(const T* __restrict__ terms, long long n, T* loss) {
   pdl_wait();
   __shared__ double sh[SUM_THREADS / 32];
   __shared__ Pair<double> of_block[SUM_CLUSTER];
@@ -1235,7 +1235,7 @@ template <typename T> __global__ void __launch_bounds__(SUM_THREADS) k_sum_terms
     v = 0;
     for (unsigned b = 0; b < blocks; ++b) v += of_block[b].m;
   }
-  if (rank == 0 && threadIdx.x == 0) *loss = (T)(v * scale);
+  if (rank == 0 && threadIdx.x == 0) *loss = (T)v;
 }
 
 // The pairs, a warp for each (or a block, LONG), over the warps (blocks) of a cluster or one block: both sequences' sums, the margin, the
@@ -1489,9 +1489,9 @@ template <typename T> cudaError_t given_grad(const RowView& x, const GivenRow<T>
                 out<T>(x, g), (int)pieces);
 }
 
-template <typename T> cudaError_t sum_terms(const void* terms, long long n, void* loss, double scale, cudaStream_t s) {
+template <typename T> cudaError_t sum_terms(const void* terms, long long n, void* loss, cudaStream_t s) {
   const unsigned blocks = n > SUM_AHEAD * SUM_THREADS ? SUM_CLUSTER : 1;
-  return launch(k_sum_terms<T>, dim3(blocks), dim3(SUM_THREADS), 0, blocks, s, (const T*)terms, n, (T*)loss, scale);
+  return launch(k_sum_terms<T>, dim3(blocks), dim3(SUM_THREADS), 0, blocks, s, (const T*)terms, n, (T*)loss);
 }
 
 // weight: null, or rows with weight 0 are not read and give nothing.
@@ -1527,7 +1527,7 @@ cudaError_t Objectives<T>::policy(const RowView& x, const int32_t* labels, const
                          (T*)logp};
   const cudaError_t e = rows_of<T>(x, obj, 1.0, g, s);
   if (e != cudaSuccess || !loss) return e;
-  return sum_terms<T>(terms, x.rows(), loss, 1.0, s);
+  return sum_terms<T>(terms, x.rows(), loss, s);
 }
 
 template <typename T>
@@ -1557,7 +1557,7 @@ template <typename T> cudaError_t Objectives<T>::distill(const RowView& x, const
   const DistillRow<T> obj{a.index, (const T*)a.teacher, (const T*)a.weight, a.k, inverse, Num<T>::factor(inverse), (T)a.temperature, (T*)terms};
   const cudaError_t e = rows_of<T>(x, obj, inverse, g, s);
   if (e != cudaSuccess || !loss) return e;
-  return sum_terms<T>(terms, x.rows(), loss, 1.0, s);
+  return sum_terms<T>(terms, x.rows(), loss, s);
 }
 
 }  // namespace rgc

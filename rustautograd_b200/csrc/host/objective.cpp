@@ -6,9 +6,6 @@ namespace rg {
 
 namespace {
 
-constexpr size_t MAX_TEACHER = 1024;  // teacher entries per row the device's kernel holds
-constexpr size_t MAX_VOCAB = size_t(1) << 30, MAX_ROWS = 0x7fffffff;
-
 bool attrs_ok(const Op& op, size_t n) {
   if (!op.value || op.value->n() != n) return false;
   for (size_t i = 0; i < n; ++i)
@@ -35,12 +32,12 @@ bool objective_of(const Op& op, const std::vector<std::vector<size_t>>& s, const
   if (d[0] == DType::I32) return no("logits_must_be_floating");
   for (size_t i = 1; i < d.size(); ++i)
     if (d[i] != (i == 1 ? DType::I32 : d[0])) return no(i == 1 ? "index_must_be_int32" : "implicit_promotion_not_allowed");
-  if (s[0].empty() || s[0].back() == 0 || s[0].back() > MAX_VOCAB) return no("logits_need_a_nonempty_last_axis");
+  if (s[0].empty() || s[0].back() == 0 || s[0].back() > OBJECTIVE_MAX_VOCAB) return no("logits_need_a_nonempty_last_axis");
   Objective o;
   const std::vector<size_t> lead(s[0].begin(), s[0].end() - 1);
   o.vocab = s[0].back();
   o.rows = o.outer = product(lead);
-  if (o.rows > MAX_ROWS) return no("too_many_rows");
+  if (o.rows > OBJECTIVE_MAX_ROWS || (op.kind == OpKind::PreferenceLoss && !lead.empty() && lead[0] > OBJECTIVE_MAX_ROWS)) return no("too_many_rows");
   o.inner = 1;
   auto with = [&](size_t n) {
     auto v = lead;
@@ -78,7 +75,7 @@ bool objective_of(const Op& op, const std::vector<std::vector<size_t>>& s, const
       o.weight_arg = 2;
       break;
     default:
-      if (s[1].empty() || s[1].back() == 0 || s[1].back() > MAX_TEACHER) return no("teacher_needs_between_1_and_1024_entries_per_row");
+      if (s[1].empty() || s[1].back() == 0 || s[1].back() > OBJECTIVE_MAX_ENTRIES) return no("teacher_needs_between_1_and_1024_entries_per_row");
       o.k = s[1].back();
       if (s[1] != with(o.k) || s[2] != s[1] || s[3] != lead) return no("operands_do_not_fit_the_logits");
       // Beyond these bounds 1 / T or T^2 leaves the range of a float.

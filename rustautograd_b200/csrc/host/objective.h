@@ -9,6 +9,9 @@
 
 namespace rg {
 
+// The vocabulary, the rows (and a preference's sequences) and the teacher entries of a row that the device's kernels take.
+constexpr size_t OBJECTIVE_MAX_VOCAB = size_t(1) << 30, OBJECTIVE_MAX_ROWS = 0x7fffffff, OBJECTIVE_MAX_ENTRIES = 1024;
+
 struct Objective {
   size_t rows = 0, vocab = 0;
   size_t outer = 0, inner = 0;  // rows as outer x inner: PreferenceLoss's sequences x positions, else rows x 1
