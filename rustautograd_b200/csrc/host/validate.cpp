@@ -269,7 +269,7 @@ Compiled::Observed Compiled::observed(const std::vector<Tensor>& inputs) const {
     std::string why;
     if (i.op.kind == OpKind::Take) dim = i.arg_shapes[0][i.op.index];
     else if (i.op.kind == OpKind::TakeAlong) dim = i.arg_shapes[0].back();
-    else if (i.op.is_objective() && objective_of(i.op, i.arg_shapes, dts, &obj, &why)) dim = obj.vocab;
+    else if (i.op.is_objective() && i.op.multi_output() && objective_of(i.op, i.arg_shapes, dts, &obj, &why)) dim = obj.vocab;  // a gradient's labels are its forward's
     if (dim) {
       size_t n = product(i.arg_shapes[1]);
       Buf index = e->prefix(i.args[1], n);

@@ -198,6 +198,7 @@ def label_cases():
             yield ("policy", bad, weight), lambda x, l=l, ww=ww: F.nn.policy_loss(x, l, row, row, ww)[0], refused
             yield ("preference", bad, weight), lambda x, l=l, ww=ww: F.nn.preference_loss(x, l, ww, seq)[0], refused
             yield ("distillation", bad, weight), lambda x, i=i, ww=ww: F.nn.distillation_loss(x, i, F.tensor(teacher), ww)[0], refused
+            yield ("logp", bad, weight), lambda x, l=l: F.nn.token_log_prob(x, l).sum(), bad is not None
             t[2, 1, 1] = -np.inf
             yield ("absent", bad, weight), lambda x, i=i, ww=ww, t=t: F.nn.distillation_loss(x, i, F.tensor(t), ww)[0], False
 
@@ -207,7 +208,7 @@ def check_labels(device):
     for what, f, refused in label_cases():
         report = F.compile(lambda x: F.value_and_grad(f)(x), (x,), validate="standard", device=device).report
         codes = [d["code"] for d in report["diagnostics"]]
-        assert ("INDEX_OUT_OF_RANGE" in codes) == refused and (report["status"] == "validation_failed") == refused, (what, report)
+        assert codes.count("INDEX_OUT_OF_RANGE") == refused and (report["status"] == "validation_failed") == refused, (what, report)
 
 
 @pytest.mark.parametrize("device", ["cpu", "cuda-plan"])
