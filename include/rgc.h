@@ -152,8 +152,10 @@ int rgc_sum_noalloc(const void* src, int64_t n, int dtype, void* dst, void* stre
  * Work is enqueued on `stream` (a cudaStream_t of that device; NULL = the legacy default stream);
  * nothing is allocated, nothing synchronises and nothing is kept between calls, so calls may be
  * captured into CUDA graphs and run at the same time on several streams as long as they write
- * different outputs (and workspaces). The same inputs give the same bits on every call. Refused
- * arguments return RGC_ERR_INVALID before any launch.
+ * different outputs (and workspaces). The same call gives the same bits every time: the same values,
+ * strides and alignment of the logits, the same results asked for, the same model of GPU. (Otherwise a
+ * row's sum may be split differently, and its last bits differ.) Refused arguments return
+ * RGC_ERR_INVALID before any launch.
  *
  * Logits: outer x inner rows of `vocab` adjacent elements, row (a, b) at data + a * outer_stride +
  * b * inner_stride elements. dtype 0 = float32, 1 = float64. Labels and indices are clamped to
@@ -161,6 +163,8 @@ int rgc_sum_noalloc(const void* src, int64_t n, int dtype, void* dst, void* stre
  * A gradient goes to outer x inner rows of its own strides; it may be the logits themselves (same
  * data and strides), and must not overlap them otherwise. Rows with weight 0 are not read: they count
  * nothing, whatever they hold, and their gradient is 0.
+ * A NaN among the operands of a row that counts makes its results NaN (the gradient where the formula
+ * has it: all of the row, or a NaN teacher entry's own element), and no other row's.
  * With RGC_VOUCHED added to dtype the caller vouches that every pointer is the current device's memory; otherwise each is
  * looked up first, some 0.3 us a pointer. */
 #define RGC_VOUCHED 256

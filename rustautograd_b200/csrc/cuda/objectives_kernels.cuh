@@ -8,9 +8,9 @@
 //    the L2;
 //  - k_stream (longer rows, no gradient): a running maximum and sum, nothing is held;
 //  - k_grad (longer rows): gradients whose coefficients need more than their row (token_log_prob_grad, preferences).
-// Of the rate of a plain copy they reach, in floats: k_stream 99 % (8192 to 131072 logits), k_grad 97 %, k_rows 91 %
-// (4096 to 16384), 88 % (32000), 83 % (50257) and 78 % (131072), k_group 88 to 95 % where its vectors are full and there are
-// 1000 logits, 61 % at 96.
+// Of the rate of a plain copy (6563 GB/s) they reach, in floats: k_stream 90 % (8192 logits), 96 % (32000), 98 % (50257), k_grad 96 %,
+// k_rows 87 % (4096, 8192), 91 % (16384), 87 % (32000), 82 % (50257, 131072), k_group with 1000 logits 81 % (policy), 74 % (without
+// a gradient), 92 % (with statistics given), and 61 % at 96.
 //
 // Numbers. Row statistics are held in the logits' type. For float, exp(x - m) is computed as
 // 2^((x - m) * log2 e) with the hardware's ex2: the difference and the product are rounded, 2 u |x - m|
@@ -18,12 +18,15 @@
 // a row's logits is taken out, since it is the same in every row of a batch and a loss is a sum of terms of both
 // signs: log2 e has two parts (as one float it is 1.3e-8 too small), ex2's mean error is put into its argument, and
 // the factors between parts of a row are a polynomial's (Num<float>::share). Row sums of normal logits, deviation 1 and 2.5, are then
-// off by 3e-9 to 9e-9 on average (8192 to 50257 logits; 7e-9 at 96; before, -2e-8 to -9e-8), with a spread of 4.5e-8. Two
-// floats to an instruction, so all this costs 2.8 % of k_stream's time at 50257 logits, 1 % of k_group's at 96, nothing of k_rows',
-// and k_grad gains 6 %. For double it is a polynomial (Num<double>). What a row reports (its log-probability's
-// terms) is computed from the statistics in double by one lane, and sums over rows are double.
-// Everything is summed in a fixed order: the same inputs give the same bits on every call. The bits of a row do
-// depend on how it is split over lanes and blocks, which goes by the vocabulary and the row count.
+// off by 3e-9 to 9e-9 on average (8192 to 50257 logits; 7e-9 at 96; without all that -2e-8 to -9e-8), with a spread of 4.5e-8. Two
+// floats to an instruction, this costs 1 to 4 % of the time of k_stream, 2 % of that of k_group and k_rows (5 % more by single
+// ones in k_stream; from 131072 logits on k_rows gains 4 %, k_grad up to 10 %). For double it is a polynomial (Num<double>).
+// What a row reports (a log-probability, a term of a loss) is computed from its statistics in double by one lane, and sums
+// over rows are double. A gradient's coefficient is computed in the logits' type, but a clipped ratio next to its bound in
+// double too, so that the gradient is that of the term.
+// Everything is summed in a fixed order: the same call gives the same bits. What a row's bits depend on beside its values is how it
+// is split over lanes and blocks: by the vocabulary, the row count, the alignment of base and strides to 16 bytes, the SM count and
+// what the call computes (k_rows with a gradient, k_stream without).
 #pragma once
 #include "objectives.cuh"
 
@@ -169,7 +172,8 @@ template <> struct Num<double> {
   static constexpr int VEC = 2;
   using Vec = double2;
   // exp(d * scale) for d <= 0: 2^t with t = d * scale * log2 e = n + f, n whole and |f| <= 1/2; 2^f by the polynomial of
-  // degree 11 that equals it at 12 Chebyshev nodes (off by 4.3e-18 relatively; 1.2 u with Horner's roundings).
+  // degree 11 that equals it at 12 Chebyshev nodes (off by 2.0e-17 relatively with its coefficients as doubles; 1.2 u with
+  // Horner's roundings).
   // Below 2^-1022 it is 0. (7 x 129 x 10007 without gradient: 28.6 us, with exp() 32.6. The power of two put in by integer
   // operations, 14 instead of 17 double ones: 8192 x 8192 in 190 instead of 165 us, so not those alone bound it.)
   struct Scale {
@@ -1387,7 +1391,12 @@ template <typename T, class Obj, bool GRAD> cudaError_t group(const RowView& x, 
     auto go = [&](auto* kernel, int rows) {
       return go_group(kernel, rows, GROUP_THREADS / 32 * rows * kept_bytes<T>((size_t)slots), x, s, view<T>(x), x.rows(), obj, k, out<T>(x, g), slots);
     };
-    if (obj.k <= 64) {  // the entries of several rows to a warp leave room for two blocks to an SM
+    // Up to 128 vectors: four vectors a lane, two rows to a group of lanes (8, 4 or 2 rows to a warp, whose entries 4, 8 or 16 lanes
+    // take). 131072 x 96 with 8 entries: 44 us, 49 with one row to a group, 45 with four (32 entries: 110, 112 and 155), 147 with
+    // one row to a warp; 32768 x 500 with 8: 42, 49 and 41. With more entries than 64 one row to a warp: at 65 that is slower (131072 x 96
+    // 453 us, 294 by eight rows to a warp), at 128 faster (914 and 1184), and the entries of a double row leave room for two blocks.
+    // Wider rows: the fewest vectors a lane that hold one.
+    if (obj.k <= 64) {
       if (v <= 8) return go(k_group_targets<T, 8, 1, 2, Obj, GRAD>, 8);
       if (v <= 16) return go(k_group_targets<T, 8, 2, 2, Obj, GRAD>, 8);
       if (v <= 32) return go(k_group_targets<T, 8, 4, 2, Obj, GRAD>, 8);

@@ -139,7 +139,7 @@ def make_train_step(model, opt, batch, world=1, rank=0):
 
 # Training steps after pretraining (no counterpart in rg), of the same contract as make_train_step:
 # `(state, batch) -> (state, aux)` with state {"params", "opt"}. Token rows hold T + 1 tokens; position t
-# predicts token t + 1, so the other per-position arrays have T columns.
+# predicts token t + 1, so the other per-position arrays have T columns. They are for one GPU: no shards, no all-reduce.
 
 def _updated(opt, state, grads):
     params, opt_state = opt.update(grads, state["opt"], state["params"])

@@ -12,7 +12,8 @@ of the leading shape (clamped to [0, V), as indices are everywhere) and operands
 the logits' dtype. Gradients flow to the logits only; the other operands are data. Only the first result
 of a loss is differentiable, the others are for reporting (differentiating them is an error). Positions
 with weight 0 count nothing, whatever they hold. A loss computes its gradient in the same pass over the
-logits, so it is an output of the forward step; a loss that is only evaluated does not compute it.
+logits, so it is an output of the forward step; a loss that is only evaluated does not compute it. A loss with
+a factor multiplies that gradient afterwards, one more pass over it: the weights take a factor for nothing.
 """
 import math
 
