@@ -93,7 +93,8 @@ template <> struct Num<float> {
   }
   // exp(d * scale)
   static __device__ __forceinline__ float exps(float d, Scale k) { return ex2(__fmaf_rn(d, k.hi, __fmaf_rn(d, k.lo, RAISE))); }
-  // The same for differences of about 1, with half the raise: 2e-8 too small on average below -1 / log2 e, 1e-8 too large above.
+  // The same for differences of about 1, without lo and with half the raise: on average off by 2.5e-8 at most on either side of -1, and 1
+  // at d = 0. For a thread's running sum, at each of its turns over a row (by share instead 16 x 511 x 50257 takes 1.4 % longer).
   static __device__ __forceinline__ float near(float d, Scale k) { return ex2(__fmaf_rn(d, k.hi, RAISE / 2)); }
   // The same for d <= 0 without ex2's share, for the factors between parts of a row (each element meets several): 2^t with
   // t = n + f, n whole and |f| <= 1/2; 2^f by the polynomial of degree 6 that equals it at 7 Chebyshev nodes (with Horner's

@@ -239,3 +239,65 @@ def test_overwritten_logits_are_known_to_autograd():
         call(y.detach())
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("v", [5, 96, 3001, 40000])
+def test_ends_of_the_temperature(v, dtype):
+    # Cold: all of p and q at the largest logits, so a row whose teacher agrees costs nothing and one whose teacher does not costs the gap in
+    # logits times T. Hot: p and q are uniform, the term is T^2 log(v / k) and the gradient T (1 / v - 1 / k at the entries).
+    rng = np.random.default_rng(v)
+    n, k = 6, 3
+    x = rng.permuted(np.tile(np.arange(v) * (8.0 / v), (n, 1)), axis=1).astype(dtype)
+    order = np.argsort(-x, 1)
+    index = order[:, [0, 1, 2]].astype("int32")
+    teacher = np.tile(np.array([5, 4, 3], dtype), (n, 1))
+    teacher[3:] = teacher[3:, ::-1]  # the third largest is the teacher's choice
+    dx, di, dt = put(x, index, teacher)
+    one = torch.ones(n, dtype=dx.dtype, device="cuda")
+    u, at = np.finfo(dtype).eps / 2, np.arange(n)
+    gap = x[at, index[:, 0]].astype("f8") - x[at, index[:, 2]]
+    for temp in (2.0 ** -60, 2.0 ** -20):
+        for grad in (False, True):
+            r = losses.distillation_loss(dx, di, dt, one, temperature=temp, grad=grad)
+            terms = get(r.terms)
+            assert not terms[:3].any() and (np.abs(terms[3:] / temp - gap[3:]) <= 8 * u * gap[3:]).all(), (temp, terms)
+        g = get(r.grad)
+        want = np.zeros((n, v))
+        want[at[3:], index[3:, 0]], want[at[3:], index[3:, 2]] = temp, -temp
+        # The logits next to the largest are 8 / v below it: T exp(-8 / (v T)) of gradient, the others a power of that factor each (their
+        # sum is below twice the first). It is 0 in either type at 2^-60, 8e-98 in double at 2^-20 and v = 40000.
+        assert (np.abs(g - want.astype(dtype)) <= 2 * temp * np.exp(-8.0 / (v * temp))).all(), temp
+    for temp in (2.0 ** 30, 2.0 ** 60):
+        for grad in (False, True):
+            r = losses.distillation_loss(dx, di, dt, one, temperature=temp, grad=grad)
+            # The logits are within 8 / T of each other: 8e-9 of a term at most, and the sum of v ones is off by its additions.
+            want = np.log(v / k)
+            off = u * (v / 32 + 40 + 4 * want) + 8.0 / temp
+            assert (np.abs(get(r.terms) / temp / temp - want) <= off).all(), temp
+        g = get(r.grad).astype("f8") / temp
+        want = np.full((n, v), 1.0 / v)
+        np.subtract.at(want, (at[:, None], index), 1.0 / k)
+        assert (np.abs(g - want) <= (u * (v / 32 + 60) + 16.0 / temp) * np.maximum(np.abs(want), 1 / v)).all(), temp
+
+
+@pytest.mark.parametrize("v", [6, 3000, 40000])
+def test_nan_in_one_pair_stays_in_it(v):
+    # A NaN or +inf logit, a NaN weight or reference: loss and that pair's margin and gradients are NaN, the other pairs' are as they were.
+    rng = np.random.default_rng(v)
+    x, lab = rng.normal(size=(6, 4, v)).astype("float32"), rng.integers(0, v, (6, 4)).astype("int32")
+    w, ref = np.ones((6, 4), "float32"), np.zeros(6, "float32")
+    good = losses.preference_loss(*put(x, lab, w, ref))
+    assert torch.isfinite(good.grad).all()
+    for what in ("nan", "inf", "weight", "reference"):
+        bx, bw, br = x.copy(), w.copy(), ref.copy()
+        if what in ("nan", "inf"):
+            bx[4, 2, v // 2] = float(what)
+        elif what == "weight":
+            bw[4, 2] = np.nan
+        else:
+            br[4] = np.nan
+        r = losses.preference_loss(*put(bx, lab, bw, br))
+        assert torch.isnan(r.loss) and torch.isnan(r.margins[1]) and torch.equal(r.margins[[0, 2]], good.margins[[0, 2]]), what
+        assert torch.isnan(r.grad[[1, 4]]).all() if what != "inf" else torch.isnan(r.grad[1]).all(), what
+        assert torch.equal(r.grad[[0, 2, 3, 5]], good.grad[[0, 2, 3, 5]]), what
